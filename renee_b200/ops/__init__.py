@@ -16,6 +16,9 @@ import torch
 
 from . import reference as ref
 from ..utils import guard
+from .relative import (Gelu8Saved, RelativeWorkspace, gelu8_bwd, gelu8_fwd, gelu8_saved, gelu8_workspace,  # noqa: F401
+                       qk_norm_rotary_bwd, qk_norm_rotary_fwd, qk_norm_rotary_workspace, relative_attention_bwd,
+                       relative_attention_fwd, relative_attention_workspace, relative_buckets, rotary_table)
 from .rng import DropoutRNG, keep_mask  # noqa: F401
 
 

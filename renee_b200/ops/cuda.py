@@ -405,6 +405,68 @@ def bias_gelu_bwd(da, x, bias, dbias, dx_out):
           _p(dbias), _I(T), _I(Fd), _stream())
 
 
+# ----------------------------------------------------------------------------- relative positions (arguments: ops/relative.py)
+def _ld(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def qk_norm_rotary_blocks(T: int, nh: int, hd: int) -> int:
+    return lib().rb_qk_norm_rotary_blocks(_LL(T), _I(nh), _I(hd))
+
+
+def qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions=None):
+    T, hd = x.shape[0], gq.numel()
+    _call("rb_qk_norm_rotary_fwd", _I(DT[x.dtype]), _p(x), _LL(_ld(x)), _p(gq), _p(gk), _p(table), _p(positions), _p(out), _LL(_ld(out)),
+          _LL(T), _I(table.shape[0]), _I(S), _I(nh), _I(hd), _F(eps), _stream(), launches=1 if T else 0)
+
+
+def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions=None):
+    T, hd = x.shape[0], gq.numel()
+    need = qk_norm_rotary_blocks(T, nh, hd) * 2 * hd
+    if ws.numel() < need or ws.device != x.device:
+        raise ValueError(f"the workspace is for fewer tokens: {ws.numel()} values on {ws.device}, the call needs {need} on {x.device}")
+    _call("rb_qk_norm_rotary_bwd", _I(DT[x.dtype]), _p(dy), _LL(_ld(dy)), _p(x), _LL(_ld(x)), _p(gq), _p(gk), _p(table), _p(positions), _p(ws),
+          _p(dx), _LL(_ld(dx)), _p(dgq), _p(dgk), _LL(T), _I(table.shape[0]), _I(S), _I(nh), _I(hd), _F(eps), _stream(),
+          launches=3 if T else 2)
+
+
+def relative_tiles(S: int) -> int:
+    return lib().rb_relative_tiles(_I(S))
+
+
+def _relative_args(q, k, v, mask, table, buckets, nh, hd, p, rng, stream):
+    b, S = mask.shape
+    return (_p(q), _LL(_ld(q)), _p(k), _LL(_ld(k)), _p(v), _LL(_ld(v)), _p(mask), _p(table), _p(buckets), _I((buckets.numel() - 1) // 2),
+            _I(table.shape[0]), _I(b), _I(S), _I(nh), _I(hd), _F(p), _p(rng.dev if p > 0 else None), _U(stream))
+
+
+def relative_attention_fwd(q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx_out, ws):
+    _call("rb_relative_fwd", _I(DT[q.dtype]), *_relative_args(q, k, v, mask, table, buckets, nh, hd, p, rng, stream), _p(ctx_out),
+          _p(None if ws is None else ws.lse), _stream(), launches=1 if mask.shape[0] else 0)
+
+
+def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx, ws, dq, dk, dv, dtable):
+    _call("rb_relative_bwd", _I(DT[q.dtype]), _p(dctx), *_relative_args(q, k, v, mask, table, buckets, nh, hd, p, rng, stream), _p(ctx),
+          _p(ws.lse), _p(ws.delta), _p(ws.dwin), _p(dq), _LL(_ld(dq)), _p(dk), _LL(_ld(dk)), _p(dv), _LL(_ld(dv)), _p(dtable), _stream(),
+          launches=3 if mask.shape[0] else 1)
+
+
+def gelu8_splits(T: int, F: int) -> int:
+    return lib().rb_gelu8_splits(_LL(T), _I(F))
+
+
+def gelu8_fwd(x, bias, out, saved):
+    T, F = x.shape
+    _call("rb_gelu8_fwd", _I(DT[x.dtype]), _p(x), _p(bias), _p(out), _p(saved.q), _p(saved.scale), _LL(T), _I(F), _stream(),
+          launches=1 if T else 0)
+
+
+def gelu8_bwd(da, saved, ws, dbias, dx, act_out):
+    T, F = da.shape
+    _call("rb_gelu8_bwd", _I(DT[da.dtype]), _p(da), _p(saved.q), _p(saved.scale), _p(ws), _p(dbias), _p(dx), _p(act_out), _LL(T), _I(F),
+          _stream(), launches=2 if T else 1)
+
+
 # ----------------------------------------------------------------------------- encoder GEMMs (tcgen05, fused epilogues)
 L_NT, L_NN, L_TN = 0, 1, 2
 E_STORE, E_BIAS_GELU, E_BIAS_DROPOUT_RESID, E_ADD, E_GELU_BWD, E_SPLITK = 0, 1, 2, 3, 4, 5

@@ -107,6 +107,90 @@ def attention_bwd(dctx, qkv, bqkv, mask, probs, nh, p, seed, stream):
     return out.reshape(b * S, 3 * H).to(qkv.dtype)
 
 
+# ----------------------------------------------------------------------------- relative positions
+def _wide(t):
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def _rotary_parts(x, table, S, nh, positions):
+    T = x.shape[0]
+    hd = x.shape[1] // (2 * nh)
+    if positions is None:
+        pos = torch.arange(T, device=x.device) % S
+    else:
+        pos = positions.long().clamp(0, table.shape[0] - 1)
+    rot = table[pos].to(x.dtype)[:, None, None, :]
+    return x.view(T, 2, nh, hd), rot[..., :hd // 2], rot[..., hd // 2:]
+
+
+def qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, positions=None):
+    """x[T,2H] = queries, keys.  RMS norm of every head, times gq / gk, rotated by position (kernel: rotary.cu)."""
+    xf, cos, sin = _rotary_parts(_wide(x), table, S, nh, positions)
+    n = xf * torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps) * torch.stack([gq, gk]).to(xf.dtype)[:, None, :]
+    n1, n2 = n.chunk(2, -1)
+    return torch.cat([n1 * cos - n2 * sin, n2 * cos + n1 * sin], -1).reshape(x.shape).to(x.dtype)
+
+
+def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, positions=None):
+    """Returns ``(dx, dgq, dgk)``."""
+    xf, cos, sin = _rotary_parts(_wide(x), table, S, nh, positions)
+    d1, d2 = _wide(dy).view(xf.shape).chunk(2, -1)
+    dn = torch.cat([d1 * cos + d2 * sin, d2 * cos - d1 * sin], -1)
+    r = torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps)
+    u = xf * r
+    dg = (dn * u).sum((0, 2))
+    du = dn * torch.stack([gq, gk]).to(xf.dtype)[:, None, :]
+    dx = r * (du - u * (du * u).mean(-1, keepdim=True))
+    return dx.reshape(x.shape).to(x.dtype), dg[0].to(gq.dtype), dg[1].to(gk.dtype)
+
+
+def _relative_probs(q, k, mask, table, buckets, nh):
+    """(heads of q, heads of k, P[b,nh,S,S], bucket[S,S], whether a sequence has an attended key, mask as bool)."""
+    b, S = mask.shape
+    hd = q.shape[1] // nh
+    qh, kh = (_wide(t).reshape(b, S, nh, hd).transpose(1, 2) for t in (q, k))
+    seen = (mask != 0)[:, None, None, :]
+    some = seen.any(-1, keepdim=True)
+    kh = torch.where((seen | ~some).transpose(-1, -2), kh, torch.zeros_like(kh))
+    far = (buckets.numel() - 1) // 2
+    at = torch.arange(S, device=q.device)
+    bucket = buckets.long().clamp(0, table.shape[0] - 1)[(at[None, :] - at[:, None]).clamp(-far, far) + far]
+    s = torch.matmul(qh, kh.transpose(-1, -2)) / math.sqrt(hd) + table.to(qh.dtype)[bucket].permute(2, 0, 1)
+    s = torch.where(some, s.masked_fill(~seen, float("-inf")), torch.zeros_like(s))
+    return qh, kh, torch.softmax(s, -1), bucket, some, seen
+
+
+def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, seed, stream):
+    """Attention with a bias by buckets of key - query; masked keys count as absent, a sequence without an attended key
+    attends to all of its tokens alike (kernels: relative.cu).  Returns ``ctx[b S, nh hd]``."""
+    b, S = mask.shape
+    _, _, w, _, some, seen = _relative_probs(q, k, mask, table, buckets, nh)
+    vh = _wide(v).reshape(b, S, nh, -1).transpose(1, 2)
+    vh = torch.where((seen | ~some).transpose(-1, -2), vh, torch.zeros_like(vh))
+    if p > 0:
+        w = w * _mask(seed, stream, w.shape, p, w.device) / (1.0 - p)
+    return torch.matmul(w, vh).transpose(1, 2).reshape(q.shape).to(q.dtype)
+
+
+def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, seed, stream):
+    """Returns ``(dq, dk, dv, dtable)``."""
+    b, S = mask.shape
+    hd = q.shape[1] // nh
+    qh, kh, w, bucket, some, seen = _relative_probs(q, k, mask, table, buckets, nh)
+    vh, do = (_wide(t).reshape(b, S, nh, hd).transpose(1, 2) for t in (v, dctx))
+    vh = torch.where((seen | ~some).transpose(-1, -2), vh, torch.zeros_like(vh))
+    keep = _mask(seed, stream, w.shape, p, w.device) / (1.0 - p) if p > 0 else torch.ones_like(w)
+    dv = torch.matmul((w * keep).transpose(-1, -2), do)
+    dp = torch.matmul(do, vh.transpose(-1, -2)) * keep
+    ds = torch.where(some, w * (dp - (dp * w).sum(-1, keepdim=True)), torch.zeros_like(w))
+    dq = torch.matmul(ds, kh) / math.sqrt(hd)
+    dk = torch.matmul(ds.transpose(-1, -2), qh) / math.sqrt(hd)
+    dtable = torch.zeros(table.shape, dtype=ds.dtype, device=q.device)
+    dtable.index_add_(0, bucket.reshape(-1), ds.sum(0).permute(1, 2, 0).reshape(S * S, nh))
+    rows = lambda t: t.transpose(1, 2).reshape(q.shape).to(q.dtype)
+    return rows(dq), rows(dk), rows(dv), dtable.to(table.dtype)
+
+
 # ----------------------------------------------------------------------------- bias+dropout+residual+LN
 def bias_dropout_add_ln_fwd(x, bias, resid, gamma, beta, eps, p, seed, stream):
     """``pre = resid + dropout(x + bias)``; ``y = LN(pre)``.  Returns ``(y, pre, mean, rstd)``."""
@@ -149,6 +233,28 @@ def bias_gelu_bwd(da, x, bias, dbias):
     dx = (da.float() * (cdf + z * pdf)).to(x.dtype)
     dbias.copy_(dx.float().sum(0).to(dbias.dtype))
     return dx
+
+
+def gelu8_fwd(x, bias, block=128):
+    """Returns ``(gelu(z), q int8, scale)`` of z = x + bias; blocks of 128 values of a row share a scale (kernel: gelu8.cu)."""
+    z = _wide(x) + bias.to(_wide(x).dtype)
+    T, Fd = z.shape
+    zb = F.pad(z, (0, -Fd % block)).view(T, -1, block)
+    top = zb.abs().amax(-1, keepdim=True)
+    bad, none = ~torch.isfinite(top), top < 2.0 ** -100
+    inv = torch.where(bad | none, torch.zeros_like(top), 127.0 / top)
+    q = torch.where(bad, torch.zeros_like(zb), torch.round(zb * inv)).to(torch.int8).view(T, -1)[:, :Fd]
+    scale = torch.where(bad, torch.full_like(top, float("nan")), torch.where(none, torch.zeros_like(top), top / 127.0))
+    return F.gelu(z).to(x.dtype), q, scale[..., 0].float()
+
+
+def gelu8_bwd(da, q, scale, block=128):
+    """Returns ``(dx, act, dbias)`` of the values that q and scale stand for."""
+    T, Fd = q.shape
+    z = q.to(_wide(da).dtype) * scale.to(_wide(da).dtype).repeat_interleave(block, 1)[:, :Fd]
+    cdf = 0.5 * torch.special.erfc(z * -math.sqrt(0.5))
+    dx = _wide(da) * (cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi))
+    return dx.to(da.dtype), (z * cdf).to(da.dtype), dx.sum(0).to(da.dtype)
 
 
 def colsum(x, out):

@@ -1,0 +1,332 @@
+"""Operators of encoder layers with relative positions, forward and backward.
+
+* :func:`qk_norm_rotary_fwd` / :func:`qk_norm_rotary_bwd`: norms of queries and keys for each head with the rotation by position
+  (``csrc/rotary.cu``);
+* :func:`relative_attention_fwd` / :func:`relative_attention_bwd`: attention with a learned bias by buckets of the distance between
+  key and query, and the gradient of that table (``csrc/relative.cu``);
+* :func:`gelu8_fwd` / :func:`gelu8_bwd`: bias + GELU that keeps its pre-activation for the backward pass in 8 bits
+  (``csrc/gelu8.cu``).
+
+They write into the caller's buffers like the other ops of the package: kernels for CUDA tensors (on the current stream, without
+allocation or synchronisation), the oracles of :mod:`renee_b200.ops.reference` for CPU tensors.  Arguments that neither serves are
+refused with a ``ValueError`` on both.  A workspace belongs to one call at a time: calls that may overlap on the GPU (two streams,
+two captured graphs) take one each.  Results do not depend on the order in which CTAs run: no sum uses atomics.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import reference as ref
+from ..utils import guard
+
+HEAD_DIMS = (32, 64, 128)
+MAX_DISTANCE = 1024               # of the bucket map: the window of sums by distance lives in shared memory
+GELU8_BLOCK = 128                 # neighbouring values of a row that share a scale
+
+
+def _cuda():
+    from . import cuda as cu
+    return cu
+
+
+def _refuse(cond: bool, what: str) -> None:
+    if cond:
+        raise ValueError(what)
+
+
+def _same_place(first: torch.Tensor, **others) -> None:
+    for name, t in others.items():
+        _refuse(t.device != first.device, f"{name} is on {t.device}, the others on {first.device}")
+    if first.is_cuda:
+        _refuse(first.device.index != torch.cuda.current_device(),
+                f"the tensors are on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _rows(name: str, t: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> None:
+    """A matrix whose rows may lie apart, in whole 16-byte pieces."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} [{rows}, {cols}], not {t.dtype} {list(t.shape)}")
+    size = t.element_size()
+    if rows and ((t.stride(1) != 1 and cols > 1) or (rows > 1 and (t.stride(0) * size % 16 or t.stride(0) < cols)) or t.data_ptr() % 16):
+        raise ValueError(f"{name}: the columns must be adjacent, rows must start on 16-byte boundaries and not overlap")
+
+
+def _whole(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
+    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
+
+
+def _apart(outputs: dict, inputs: dict) -> None:
+    """No output may start where an input or another output does (what one kernel writes a later one would read)."""
+    seen = {t.data_ptr(): n for n, t in inputs.items() if t.numel()}
+    for n, t in outputs.items():
+        if t.numel():
+            _refuse(t.data_ptr() in seen, f"{n} is the same memory as {seen.get(t.data_ptr())}")
+            seen[t.data_ptr()] = n
+
+
+def _head_dim(cols: int, nh: int, on_gpu: bool) -> int:
+    _refuse(nh < 1 or cols % nh != 0, f"{cols} columns are no whole number of values for each of {nh} heads")
+    hd = cols // nh
+    _refuse(hd % 2 != 0 or (on_gpu and hd not in HEAD_DIMS), f"head dim {hd}: the kernels have {HEAD_DIMS}")
+    return hd
+
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+# ----------------------------------------------------------------------------- q/k norm + rotation
+def rotary_table(n_positions: int, hd: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """fp32 ``[n_positions, hd]``: the cosines of a position's ``hd / 2`` angles, then their sines.  Angles in 64 bits: in 32 the
+    one of position 100000 is off by 0.004."""
+    _refuse(hd % 2 != 0 or n_positions < 1, f"no rotation for head dim {hd} and {n_positions} positions")
+    speed = float(base) ** (-torch.arange(hd // 2, dtype=torch.float64) / (hd // 2))
+    angle = torch.arange(n_positions, dtype=torch.float64)[:, None] * speed
+    return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+
+
+def _check_rotary(x, gq, gk, table, S, nh, eps, positions, **like_x):
+    _refuse(x.dim() != 2 or x.dtype not in _FLOATS or x.shape[1] % (2 * nh if nh > 0 else 1) != 0,
+            f"x must be [T, 2 heads head dim] of {[str(d) for d in _FLOATS]}, not {x.dtype} {list(x.shape)}")
+    hd = _head_dim(x.shape[1] // 2, nh, x.is_cuda)
+    T = x.shape[0]
+    for name, t in like_x.items():
+        _rows(name, t, T, 2 * nh * hd, x.dtype)
+    _rows("x", x, T, 2 * nh * hd, x.dtype)
+    _whole("gq", gq, (hd,), x.dtype)
+    _whole("gk", gk, (hd,), x.dtype)
+    _refuse(table.dim() != 2 or table.shape[0] < 1, "table must have a row for each position")
+    _whole("table", table, (table.shape[0], hd), torch.float32)
+    _refuse(S < 1 or T % S != 0, f"{T} tokens are no whole number of sequences of {S}")
+    if positions is None:
+        _refuse(S > table.shape[0], f"table has {table.shape[0]} positions, the sequences {S}")
+    else:
+        _whole("positions", positions, (T,), torch.int32)
+        _same_place(x, positions=positions)
+    _refuse(not eps > 0.0, "eps must be above 0")
+    _refuse(T * nh * (hd // 16) >= 2 ** 31, f"{T} tokens with {nh} heads of {hd} are too many for one call")
+    if x.is_cuda:
+        for name, t in (("gq", gq), ("gk", gk), ("table", table)):
+            _refuse(t.data_ptr() % 16 != 0, f"{name} must start on a 16-byte boundary")
+    _same_place(x, gq=gq, gk=gk, table=table, **like_x)
+    return hd
+
+
+def qk_norm_rotary_workspace(T: int, nh: int, hd: int, device) -> torch.Tensor:
+    """Scratch of :func:`qk_norm_rotary_bwd` for up to ``T`` tokens (empty on the CPU)."""
+    if torch.device(device).type != "cuda":
+        return torch.empty(0)
+    with torch.cuda.device(device):
+        n = _cuda().qk_norm_rotary_blocks(T, nh, hd) * 2 * hd
+    return guard.empty(max(n, 1), dtype=torch.float32, device=device, name="qk_norm_rotary.workspace")
+
+
+def qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions=None) -> None:
+    """``x`` ``[T, 2H]`` (queries of all heads, then keys; rows may lie apart) -> ``out``: every head's ``hd`` values divided by
+    their root mean square (``eps`` is added to the mean square), times ``gq`` or ``gk`` ``[hd]``, rotated by the token's position:
+    value ``i`` with value ``i + hd/2`` by the angle whose cosine and sine ``table`` (:func:`rotary_table`) holds.  Token ``t`` of
+    the padded ``[b, S]`` batch stands at ``t % S``, or at ``positions[t]`` (int32; one outside the table counts as its nearest)."""
+    _check_rotary(x, gq, gk, table, S, nh, eps, positions, out=out)
+    _apart(dict(out=out), dict(x=x, gq=gq, gk=gk, table=table))
+    if x.is_cuda:
+        return _cuda().qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions)
+    out.copy_(ref.qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, positions))
+
+
+def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions=None) -> None:
+    """Gradients of :func:`qk_norm_rotary_fwd` from its own inputs: ``dx`` (may be ``dy`` itself), ``dgq``, ``dgk`` (all written,
+    not accumulated)."""
+    hd = _check_rotary(x, gq, gk, table, S, nh, eps, positions, dy=dy, dx=dx)
+    _whole("dgq", dgq, (hd,), x.dtype)
+    _whole("dgk", dgk, (hd,), x.dtype)
+    _same_place(x, dgq=dgq, dgk=dgk)
+    in_place = dx.data_ptr() == dy.data_ptr() and dx.stride() == dy.stride()
+    _apart(dict(dx=dx, dgq=dgq, dgk=dgk), dict(x=x, gq=gq, gk=gk, table=table, **({} if in_place else dict(dy=dy))))
+    if x.is_cuda:
+        return _cuda().qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions)
+    g = ref.qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, positions)
+    for out, t in zip((dx, dgq, dgk), g):
+        out.copy_(t)
+
+
+# ----------------------------------------------------------------------------- attention with a bias by buckets of distance
+def relative_buckets(num_buckets: int, max_distance: int, device=None) -> torch.Tensor:
+    """int32 ``[2 max_distance + 1]``: the bucket of distance (key - query) ``-max_distance .. max_distance``; distances beyond
+    count as the ends.  Keys behind the query have the upper half of the buckets; of a half, the first half holds one distance
+    each, the others grow with its logarithm and the last one reaches to ``max_distance`` and beyond."""
+    half, exact = num_buckets // 2, num_buckets // 4
+    _refuse(num_buckets < 4 or num_buckets % 2 != 0 or max_distance <= exact or max_distance > MAX_DISTANCE,
+            f"no buckets for {num_buckets} and a distance of {max_distance} (at most {MAX_DISTANCE})")
+    out = []
+    for d in range(-max_distance, max_distance + 1):
+        n = abs(d)
+        # the logarithm's steps, with a margin above rounding: at an exact border (n / exact a power of the ratio) the next begins
+        grown = exact + int(math.log(n / exact) / math.log(max_distance / exact) * (half - exact) + 1e-9) if n >= exact else n
+        out.append(min(grown, half - 1) + (half if d > 0 else 0))
+    return torch.tensor(out, dtype=torch.int32, device=device)
+
+
+@dataclass
+class RelativeWorkspace:
+    """What :func:`relative_attention_fwd` leaves for its backward pass (``lse``) and the scratch of that pass."""
+    lse: torch.Tensor
+    delta: torch.Tensor
+    dwin: torch.Tensor
+
+
+def relative_attention_workspace(b: int, S: int, nh: int, hd: int, max_distance: int, dtype, device, scratch=None) -> RelativeWorkspace:
+    """Buffers for ``b`` sequences of ``S`` tokens.  Each forward call whose backward pass is still to come needs an ``lse`` of its
+    own; ``scratch`` (another workspace of the same sizes) lends its other buffers, which live within one backward call."""
+    if torch.device(device).type == "cpu":
+        return RelativeWorkspace(*[torch.empty(0)] * 3)
+    e = lambda n, name: guard.empty(max(n, 1), dtype=torch.float32, device=device, name=f"relative_attention.{name}")
+    lse = e(b * nh * S, "lse")
+    if scratch is not None:
+        return RelativeWorkspace(lse, scratch.delta, scratch.dwin)
+    tiles = _cuda().relative_tiles(S)
+    return RelativeWorkspace(lse, e(b * nh * S, "delta"), e(b * tiles * nh * (2 * min(max_distance, S - 1) + 1), "dwin"))
+
+
+def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
+    _refuse(mask.dim() != 2 or mask.shape[1] < 1, "mask must be [b, S] with S >= 1")
+    b, S = mask.shape
+    _refuse(q.dim() != 2 or q.dtype not in _FLOATS or (q.is_cuda and q.dtype == torch.float32),
+            f"q must be [b S, heads head dim] in 16 bits, not {q.dtype} {list(q.shape)}")
+    hd = _head_dim(q.shape[1], nh, q.is_cuda)
+    for name, t in dict(q=q, k=k, v=v, **like_q).items():
+        _rows(name, t, b * S, nh * hd, q.dtype)
+    _whole("mask", mask, (b, S), torch.int32)
+    _refuse(table.dim() != 2 or table.shape[0] < 1, "table must be [buckets, heads]")
+    _whole("table", table, (table.shape[0], nh), q.dtype)
+    n = buckets.numel()
+    _refuse(n % 2 == 0 or n > 2 * MAX_DISTANCE + 1, f"buckets must be [2 far + 1] with far <= {MAX_DISTANCE}, not [{n}]")
+    _whole("buckets", buckets, (n,), torch.int32)
+    _refuse(not 0.0 <= p < 1.0, f"dropout probability {p}")
+    _refuse(p > 0.0 and rng is None, "dropout needs the step's seed")
+    if q.is_cuda:
+        _refuse(p > 0.0 and (rng.dev is None or rng.dev.dtype != torch.int32 or rng.dev.device != q.device),
+                "dropout needs the step's seed as an int32 tensor on the device")
+        _refuse(b * nh * ((S + 15) // 16) >= 2 ** 31, f"{b} sequences of {S} tokens with {nh} heads are too many for one call")
+    _same_place(q, k=k, v=v, mask=mask, table=table, buckets=buckets, **like_q)
+    return b, S, hd
+
+
+def _check_ws(ws, device, **need):
+    for name, n in need.items():
+        t = getattr(ws, name)
+        _refuse(t.numel() < n or t.device != device, f"the workspace is for smaller sizes: {name} has {t.numel()} values on {t.device}, "
+                f"the call needs {n} on {device}")
+
+
+def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ctx_out, ws=None) -> None:
+    """``ctx = softmax(q k^T / sqrt(hd) + table[buckets[clamp(key - query)], head])`` (dropout of the probabilities) ``v``.
+
+    ``q``, ``k``, ``v`` ``[b S, nh hd]``, biases added, rows may lie apart (views of one projection); ``mask`` ``[b, S]`` int32, 0 =
+    masked key: it counts as absent, whatever its row holds.  A sequence without any attended key attends to all of its tokens
+    alike, as :func:`renee_b200.ops.attention_fwd` has it.  ``table`` ``[buckets, nh]`` in the activations' type, ``buckets`` from
+    :func:`relative_buckets` (or any int32 map of ``2 far + 1`` distances).  ``ctx_out`` ``[b S, nh hd]``, contiguous.  ``ws``
+    receives what the backward pass needs; None where there is none."""
+    b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng)
+    _whole("ctx_out", ctx_out, (b * S, nh * hd), q.dtype)
+    _same_place(q, ctx_out=ctx_out)
+    _apart(dict(ctx_out=ctx_out), dict(q=q, k=k, v=v, table=table))
+    if q.is_cuda:
+        if ws is not None:
+            _check_ws(ws, q.device, lse=b * nh * S)
+        return _cuda().relative_attention_fwd(q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx_out, ws)
+    ctx_out.copy_(ref.relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream))
+
+
+def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stream, ctx, ws, dq, dk, dv, dtable) -> None:
+    """Gradients of :func:`relative_attention_fwd` from its inputs, its output ``ctx`` and the workspace it filled: ``dq``, ``dk``,
+    ``dv`` (rows may lie apart) and ``dtable`` ``[buckets, nh]``, all written, not accumulated."""
+    b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng, dq=dq, dk=dk, dv=dv)
+    _whole("dctx", dctx, (b * S, nh * hd), q.dtype)
+    _whole("ctx", ctx, (b * S, nh * hd), q.dtype)
+    _whole("dtable", dtable, tuple(table.shape), q.dtype)
+    _same_place(q, dctx=dctx, ctx=ctx, dtable=dtable)
+    _apart(dict(dq=dq, dk=dk, dv=dv, dtable=dtable), dict(q=q, k=k, v=v, dctx=dctx, ctx=ctx, table=table))
+    if q.is_cuda:
+        far = (buckets.numel() - 1) // 2
+        _check_ws(ws, q.device, lse=b * nh * S, delta=b * nh * S,
+                  dwin=b * _cuda().relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
+        return _cuda().relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx, ws, dq, dk, dv, dtable)
+    g = ref.relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream)
+    for out, t in zip((dq, dk, dv, dtable), g):
+        out.copy_(t)
+
+
+# ----------------------------------------------------------------------------- bias + GELU with its pre-activation in 8 bits
+@dataclass
+class Gelu8Saved:
+    """A pre-activation in 8 bits: ``q`` int8 ``[T, F]`` and ``scale`` fp32 ``[T, ceil(F / 128)]``; it stands for ``q scale``."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    def __getitem__(self, rows) -> "Gelu8Saved":
+        return Gelu8Saved(self.q[rows], self.scale[rows])
+
+
+def gelu8_saved(T: int, F: int, device) -> Gelu8Saved:
+    return Gelu8Saved(guard.empty(T, F, dtype=torch.int8, device=device, name="gelu8.saved"),
+                      guard.empty(T, -(-F // GELU8_BLOCK), dtype=torch.float32, device=device, name="gelu8.scale"))
+
+
+def gelu8_workspace(T: int, F: int, device) -> torch.Tensor:
+    """Scratch of :func:`gelu8_bwd` for up to ``T`` rows (empty on the CPU)."""
+    if torch.device(device).type != "cuda":
+        return torch.empty(0)
+    with torch.cuda.device(device):
+        n = _cuda().gelu8_splits(T, F) * F
+    return guard.empty(max(n, 1), dtype=torch.float32, device=device, name="gelu8.workspace")
+
+
+def _check_gelu8(saved, **like_x):
+    x = next(iter(like_x.values()))
+    _refuse(x.dim() != 2 or x.dtype not in _FLOATS or x.shape[1] % 8 != 0 or x.shape[1] < 8,
+            f"rows must be a multiple of 8 values of {[str(d) for d in _FLOATS]}, not {x.dtype} {list(x.shape)}")
+    T, F = x.shape
+    for name, t in like_x.items():
+        _whole(name, t, (T, F), x.dtype)
+    _whole("saved.q", saved.q, (T, F), torch.int8)
+    _whole("saved.scale", saved.scale, (T, -(-F // GELU8_BLOCK)), torch.float32)
+    _refuse(T >= 2 ** 30 or T * F >= 2 ** 38, f"{T} rows of {F} are too many for one call")
+    if x.is_cuda and T:
+        for name, t in dict(like_x, **{"saved.q": saved.q}).items():
+            _refuse(t.data_ptr() % (8 if name == "saved.q" else 16) != 0, f"{name} must start on a 16-byte boundary (saved.q: 8)")
+    _same_place(x, **{"saved.q": saved.q, "saved.scale": saved.scale}, **like_x)
+    return T, F
+
+
+def gelu8_fwd(x, bias, out, saved) -> None:
+    """``out = gelu(x + bias)`` for ``x`` ``[T, F]`` (erf GELU); ``saved`` receives ``x + bias`` in 8 bits: 128 neighbouring
+    values of a row share a scale and are held to 1/254 of the largest of them.  A block with an infinity or a NaN stands
+    for NaNs.  ``out`` may be ``x`` itself."""
+    _, F = _check_gelu8(saved, x=x, out=out)
+    _whole("bias", bias, (F,), x.dtype)
+    _same_place(x, bias=bias)
+    _apart(dict(out=out), dict(bias=bias))
+    if x.is_cuda:
+        _refuse(bias.data_ptr() % 16 != 0, "bias must start on a 16-byte boundary")
+        return _cuda().gelu8_fwd(x, bias, out, saved)
+    y, q, scale = ref.gelu8_fwd(x, bias)
+    out.copy_(y); saved.q.copy_(q); saved.scale.copy_(scale)
+
+
+def gelu8_bwd(da, saved, ws, dbias, dx, act_out) -> None:
+    """From the gradient ``da`` of the activation and the 8 bits: ``dx = da gelu'(z)``, its column sums ``dbias``, and the
+    activation ``act_out = gelu(z)`` again (for the weight gradient of the linear that read it).  ``dx`` may be ``da`` itself."""
+    T, F = _check_gelu8(saved, da=da, dx=dx, act_out=act_out)
+    _whole("dbias", dbias, (F,), da.dtype)
+    _same_place(da, dbias=dbias)
+    _apart(dict(dx=dx, act_out=act_out, dbias=dbias), {})
+    _apart(dict(act_out=act_out, dbias=dbias), dict(da=da))
+    if da.is_cuda:
+        need = _cuda().gelu8_splits(T, F) * F
+        _refuse(ws.numel() < need or ws.device != da.device, f"the workspace is for fewer rows: {ws.numel()} values, the call needs {need}")
+        return _cuda().gelu8_bwd(da, saved, ws, dbias, dx, act_out)
+    d, a, db = ref.gelu8_bwd(da, saved.q, saved.scale)
+    dx.copy_(d); act_out.copy_(a); dbias.copy_(db)
