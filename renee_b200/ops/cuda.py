@@ -406,6 +406,34 @@ def bias_gelu_bwd(da, x, bias, dbias, dx_out):
 
 
 # ----------------------------------------------------------------------------- relative positions (arguments: ops/relative.py)
+# Entry points whose argument types are set, so that they take Python's numbers as they are (wrapping each costs 0.25 us, and the
+# kernels of a small call take 5): p = address, l = long long, i = int, u = unsigned, f = float.  The stream is the last argument.
+_KINDS = {"p": _VP, "l": _LL, "i": _I, "u": _U, "f": _F}
+_RELATIVE_INPUTS = "plplplpppiiiiiifpu"
+_TYPES = {
+    "rb_qk_norm_rotary_fwd": "iplppppplliiiifp",
+    "rb_qk_norm_rotary_bwd": "iplplpppppplpp" + "liiiifp",
+    "rb_relative_fwd": "i" + _RELATIVE_INPUTS + "ppp",
+    "rb_relative_bwd": "ip" + _RELATIVE_INPUTS + "pppp" + "plplpl" + "pp",
+    "rb_gelu8_fwd": "ippppplip",
+    "rb_gelu8_bwd": "ippppppplip",
+}
+_TYPED: dict = {}
+
+
+def _call_typed(name, device, *args, launches=1):
+    global _LAUNCHES
+    fn = _TYPED.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes = [_KINDS[k] for k in _TYPES[name]]
+        _TYPED[name] = fn
+    rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        raise KernelError(f"{name} failed with code {rc}")
+    _LAUNCHES += launches
+
+
 def _ld(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -414,41 +442,41 @@ def qk_norm_rotary_blocks(T: int, nh: int, hd: int) -> int:
     return lib().rb_qk_norm_rotary_blocks(_LL(T), _I(nh), _I(hd))
 
 
-def qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions=None):
-    T, hd = x.shape[0], gq.numel()
-    _call("rb_qk_norm_rotary_fwd", _I(DT[x.dtype]), _p(x), _LL(_ld(x)), _p(gq), _p(gk), _p(table), _p(positions), _p(out), _LL(_ld(out)),
-          _LL(T), _I(table.shape[0]), _I(S), _I(nh), _I(hd), _F(eps), _stream(), launches=1 if T else 0)
+def qk_norm_rotary_fwd(at, x, table, S, nh, hd, eps, out, positions):
+    y, x_, gq, gk, table_ = at
+    T = x.shape[0]
+    _call_typed("rb_qk_norm_rotary_fwd", x.device, DT[x.dtype], x_, _ld(x), gq, gk, table_, None if positions is None else positions.data_ptr(),
+                y, _ld(out), T, table.shape[0], S, nh, hd, eps, launches=1 if T else 0)
 
 
-def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions=None):
-    T, hd = x.shape[0], gq.numel()
-    need = qk_norm_rotary_blocks(T, nh, hd) * 2 * hd
-    if ws.numel() < need or ws.device != x.device:
-        raise ValueError(f"the workspace is for fewer tokens: {ws.numel()} values on {ws.device}, the call needs {need} on {x.device}")
-    _call("rb_qk_norm_rotary_bwd", _I(DT[x.dtype]), _p(dy), _LL(_ld(dy)), _p(x), _LL(_ld(x)), _p(gq), _p(gk), _p(table), _p(positions), _p(ws),
-          _p(dx), _LL(_ld(dx)), _p(dgq), _p(dgk), _LL(T), _I(table.shape[0]), _I(S), _I(nh), _I(hd), _F(eps), _stream(),
-          launches=3 if T else 2)
+def qk_norm_rotary_bwd(at, dy, x, table, S, nh, hd, eps, ws, dx, positions):
+    dx_, dgq, dgk, x_, gq, gk, table_ = at
+    T = x.shape[0]
+    _call_typed("rb_qk_norm_rotary_bwd", x.device, DT[x.dtype], dy.data_ptr(), _ld(dy), x_, _ld(x), gq, gk, table_,
+                None if positions is None else positions.data_ptr(), ws.data_ptr(), dx_, _ld(dx), dgq, dgk, T, table.shape[0], S, nh, hd, eps,
+                launches=3 if T else 2)
 
 
 def relative_tiles(S: int) -> int:
     return lib().rb_relative_tiles(_I(S))
 
 
-def _relative_args(q, k, v, mask, table, buckets, nh, hd, p, rng, stream):
+def _relative_inputs(at, q, k, v, mask, table, buckets, nh, p, rng, stream):
     b, S = mask.shape
-    return (_p(q), _LL(_ld(q)), _p(k), _LL(_ld(k)), _p(v), _LL(_ld(v)), _p(mask), _p(table), _p(buckets), _I((buckets.numel() - 1) // 2),
-            _I(table.shape[0]), _I(b), _I(S), _I(nh), _I(hd), _F(p), _p(rng.dev if p > 0 else None), _U(stream))
+    return (at[0], _ld(q), at[1], _ld(k), at[2], _ld(v), mask.data_ptr(), table.data_ptr(), buckets.data_ptr(), (buckets.shape[0] - 1) // 2,
+            table.shape[0], b, S, nh, q.shape[1] // nh, p, rng.dev.data_ptr() if p > 0 else None, stream)
 
 
-def relative_attention_fwd(q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx_out, ws):
-    _call("rb_relative_fwd", _I(DT[q.dtype]), *_relative_args(q, k, v, mask, table, buckets, nh, hd, p, rng, stream), _p(ctx_out),
-          _p(None if ws is None else ws.lse), _stream(), launches=1 if mask.shape[0] else 0)
+def relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):
+    _call_typed("rb_relative_fwd", q.device, DT[q.dtype], *_relative_inputs(at[1:4], q, k, v, mask, table, buckets, nh, p, rng, stream), at[0],
+                None if ws is None else ws.lse.data_ptr(), launches=1 if mask.shape[0] else 0)
 
 
-def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx, ws, dq, dk, dv, dtable):
-    _call("rb_relative_bwd", _I(DT[q.dtype]), _p(dctx), *_relative_args(q, k, v, mask, table, buckets, nh, hd, p, rng, stream), _p(ctx),
-          _p(ws.lse), _p(ws.delta), _p(ws.dwin), _p(dq), _LL(_ld(dq)), _p(dk), _LL(_ld(dk)), _p(dv), _LL(_ld(dv)), _p(dtable), _stream(),
-          launches=3 if mask.shape[0] else 1)
+def relative_attention_bwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws, dq, dk, dv):
+    dq_, dk_, dv_, dtable, _, _, _, dctx, ctx, _ = at
+    _call_typed("rb_relative_bwd", q.device, DT[q.dtype], dctx, *_relative_inputs(at[4:7], q, k, v, mask, table, buckets, nh, p, rng, stream), ctx,
+                ws.lse.data_ptr(), ws.delta.data_ptr(), ws.dwin.data_ptr(), dq_, _ld(dq), dk_, _ld(dk), dv_, _ld(dv), dtable,
+                launches=3 if mask.shape[0] else 1)
 
 
 def gelu8_splits(T: int, F: int) -> int:
@@ -457,14 +485,14 @@ def gelu8_splits(T: int, F: int) -> int:
 
 def gelu8_fwd(x, bias, out, saved):
     T, F = x.shape
-    _call("rb_gelu8_fwd", _I(DT[x.dtype]), _p(x), _p(bias), _p(out), _p(saved.q), _p(saved.scale), _LL(T), _I(F), _stream(),
-          launches=1 if T else 0)
+    _call_typed("rb_gelu8_fwd", x.device, DT[x.dtype], x.data_ptr(), bias.data_ptr(), out.data_ptr(), saved.q.data_ptr(), saved.scale.data_ptr(),
+                T, F, launches=1 if T else 0)
 
 
 def gelu8_bwd(da, saved, ws, dbias, dx, act_out):
     T, F = da.shape
-    _call("rb_gelu8_bwd", _I(DT[da.dtype]), _p(da), _p(saved.q), _p(saved.scale), _p(ws), _p(dbias), _p(dx), _p(act_out), _LL(T), _I(F),
-          _stream(), launches=2 if T else 1)
+    _call_typed("rb_gelu8_bwd", da.device, DT[da.dtype], da.data_ptr(), saved.q.data_ptr(), saved.scale.data_ptr(), ws.data_ptr(), dbias.data_ptr(),
+                dx.data_ptr(), act_out.data_ptr(), T, F, launches=2 if T else 1)
 
 
 # ----------------------------------------------------------------------------- encoder GEMMs (tcgen05, fused epilogues)

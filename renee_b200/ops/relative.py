@@ -37,6 +37,33 @@ def _refuse(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
+# Checks that depend on shapes, strides, types, devices and numbers alone are made once for each combination: they cost 25 us in
+# Python where the kernels of a small call take 5.  Pointers (alignment, outputs that are inputs) are looked at on every call.
+_CHECKED: set = set()
+
+
+def _sig(*tensors) -> list:
+    out = []
+    for t in tensors:
+        out += (t.shape, t.stride(), t.dtype, t.device)
+    return out
+
+
+def _first_time(key: tuple) -> bool:
+    return key not in _CHECKED
+
+
+def _passed(key: tuple) -> None:
+    if len(_CHECKED) >= 4096:
+        _CHECKED.clear()
+    _CHECKED.add(key)
+
+
+def _current(t: torch.Tensor) -> int:
+    """The device that a call's kernels would run on (part of the key: the tensors' must be the current one)."""
+    return torch.cuda.current_device() if t.is_cuda else -1
+
+
 def _same_place(first: torch.Tensor, **others) -> None:
     for name, t in others.items():
         _refuse(t.device != first.device, f"{name} is on {t.device}, the others on {first.device}")
@@ -50,8 +77,8 @@ def _rows(name: str, t: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) 
     if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype} [{rows}, {cols}], not {t.dtype} {list(t.shape)}")
     size = t.element_size()
-    if rows and ((t.stride(1) != 1 and cols > 1) or (rows > 1 and (t.stride(0) * size % 16 or t.stride(0) < cols)) or t.data_ptr() % 16):
-        raise ValueError(f"{name}: the columns must be adjacent, rows must start on 16-byte boundaries and not overlap")
+    if rows and ((t.stride(1) != 1 and cols > 1) or (rows > 1 and (t.stride(0) * size % 16 or t.stride(0) < cols))):
+        raise ValueError(f"{name}: the columns must be adjacent, rows must lie whole 16-byte pieces apart and not overlap")
 
 
 def _whole(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
@@ -59,13 +86,20 @@ def _whole(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None
         raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
 
 
-def _apart(outputs: dict, inputs: dict) -> None:
-    """No output may start where an input or another output does (what one kernel writes a later one would read)."""
-    seen = {t.data_ptr(): n for n, t in inputs.items() if t.numel()}
-    for n, t in outputs.items():
-        if t.numel():
-            _refuse(t.data_ptr() in seen, f"{n} is the same memory as {seen.get(t.data_ptr())}")
-            seen[t.data_ptr()] = n
+def _pointers(outputs: tuple, inputs: tuple) -> list:
+    """Addresses of outputs, then inputs.  All must be 16-byte aligned, and no output may start where an input or another output
+    does (what one kernel writes a later one would read); tensors without elements have none."""
+    out, inp = [t.data_ptr() for t in outputs], [t.data_ptr() for t in inputs]
+    every = 0
+    for a in out:
+        every |= a
+    for a in inp:
+        every |= a
+    _refuse(every & 15 != 0, "every tensor must start on a 16-byte boundary")
+    for i, a in enumerate(out):
+        if a and (a in inp or a in out[:i]):
+            raise ValueError("an output is the same memory as another tensor of the call")
+    return out + inp
 
 
 def _head_dim(cols: int, nh: int, on_gpu: bool) -> int:
@@ -108,9 +142,6 @@ def _check_rotary(x, gq, gk, table, S, nh, eps, positions, **like_x):
         _same_place(x, positions=positions)
     _refuse(not eps > 0.0, "eps must be above 0")
     _refuse(T * nh * (hd // 16) >= 2 ** 31, f"{T} tokens with {nh} heads of {hd} are too many for one call")
-    if x.is_cuda:
-        for name, t in (("gq", gq), ("gk", gk), ("table", table)):
-            _refuse(t.data_ptr() % 16 != 0, f"{name} must start on a 16-byte boundary")
     _same_place(x, gq=gq, gk=gk, table=table, **like_x)
     return hd
 
@@ -129,24 +160,35 @@ def qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions=None) -> Non
     their root mean square (``eps`` is added to the mean square), times ``gq`` or ``gk`` ``[hd]``, rotated by the token's position:
     value ``i`` with value ``i + hd/2`` by the angle whose cosine and sine ``table`` (:func:`rotary_table`) holds.  Token ``t`` of
     the padded ``[b, S]`` batch stands at ``t % S``, or at ``positions[t]`` (int32; one outside the table counts as its nearest)."""
-    _check_rotary(x, gq, gk, table, S, nh, eps, positions, out=out)
-    _apart(dict(out=out), dict(x=x, gq=gq, gk=gk, table=table))
+    key = ("rotary", _current(x), S, nh, eps, *_sig(x, gq, gk, table, out), *(_sig(positions) if positions is not None else ()))
+    if _first_time(key):
+        _check_rotary(x, gq, gk, table, S, nh, eps, positions, out=out)
+        _passed(key)
+    at = _pointers((out,), (x, gq, gk, table))
     if x.is_cuda:
-        return _cuda().qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions)
+        return _cuda().qk_norm_rotary_fwd(at, x, table, S, nh, gq.shape[0], eps, out, positions)
     out.copy_(ref.qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, positions))
 
 
 def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions=None) -> None:
     """Gradients of :func:`qk_norm_rotary_fwd` from its own inputs: ``dx`` (may be ``dy`` itself), ``dgq``, ``dgk`` (all written,
     not accumulated)."""
-    hd = _check_rotary(x, gq, gk, table, S, nh, eps, positions, dy=dy, dx=dx)
-    _whole("dgq", dgq, (hd,), x.dtype)
-    _whole("dgk", dgk, (hd,), x.dtype)
-    _same_place(x, dgq=dgq, dgk=dgk)
+    key = ("rotary'", _current(x), S, nh, eps, *_sig(x, gq, gk, table, dy, dx, dgq, dgk), ws.numel(), ws.device,
+           *(_sig(positions) if positions is not None else ()))
+    if _first_time(key):
+        hd = _check_rotary(x, gq, gk, table, S, nh, eps, positions, dy=dy, dx=dx)
+        _whole("dgq", dgq, (hd,), x.dtype)
+        _whole("dgk", dgk, (hd,), x.dtype)
+        _same_place(x, dgq=dgq, dgk=dgk)
+        if x.is_cuda:
+            need = _cuda().qk_norm_rotary_blocks(x.shape[0], nh, hd) * 2 * hd
+            _refuse(ws.numel() < need or ws.device != x.device or ws.dtype != torch.float32,
+                    f"the workspace is for fewer tokens: {ws.numel()} values on {ws.device}, the call needs {need} on {x.device}")
+        _passed(key)
     in_place = dx.data_ptr() == dy.data_ptr() and dx.stride() == dy.stride()
-    _apart(dict(dx=dx, dgq=dgq, dgk=dgk), dict(x=x, gq=gq, gk=gk, table=table, **({} if in_place else dict(dy=dy))))
+    at = _pointers((dx, dgq, dgk), (x, gq, gk, table) if in_place else (x, gq, gk, table, dy))
     if x.is_cuda:
-        return _cuda().qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions)
+        return _cuda().qk_norm_rotary_bwd(at[:7], dy, x, table, S, nh, gq.shape[0], eps, ws, dx, positions)
     g = ref.qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, positions)
     for out, t in zip((dx, dgq, dgk), g):
         out.copy_(t)
@@ -169,12 +211,12 @@ def relative_buckets(num_buckets: int, max_distance: int, device=None) -> torch.
     return torch.tensor(out, dtype=torch.int32, device=device)
 
 
-@dataclass
 class RelativeWorkspace:
     """What :func:`relative_attention_fwd` leaves for its backward pass (``lse``) and the scratch of that pass."""
-    lse: torch.Tensor
-    delta: torch.Tensor
-    dwin: torch.Tensor
+
+    def __init__(self, lse: torch.Tensor, delta: torch.Tensor, dwin: torch.Tensor):
+        self.lse, self.delta, self.dwin = lse, delta, dwin
+        self.sizes = (lse.device, lse.numel(), delta.numel(), dwin.numel())
 
 
 def relative_attention_workspace(b: int, S: int, nh: int, hd: int, max_distance: int, dtype, device, scratch=None) -> RelativeWorkspace:
@@ -214,11 +256,10 @@ def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
     return b, S, hd
 
 
-def _check_ws(ws, device, **need):
-    for name, n in need.items():
-        t = getattr(ws, name)
-        _refuse(t.numel() < n or t.device != device, f"the workspace is for smaller sizes: {name} has {t.numel()} values on {t.device}, "
-                f"the call needs {n} on {device}")
+def _check_ws(ws, device, *need) -> None:
+    at, *have = ws.sizes
+    _refuse(at != device or any(h < n for h, n in zip(have, need)),
+            f"the workspace is for smaller sizes: {have} values on {at}, the call needs {list(need)} on {device}")
 
 
 def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ctx_out, ws=None) -> None:
@@ -229,31 +270,39 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ct
     alike, as :func:`renee_b200.ops.attention_fwd` has it.  ``table`` ``[buckets, nh]`` in the activations' type, ``buckets`` from
     :func:`relative_buckets` (or any int32 map of ``2 far + 1`` distances).  ``ctx_out`` ``[b S, nh hd]``, contiguous.  ``ws``
     receives what the backward pass needs; None where there is none."""
-    b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng)
-    _whole("ctx_out", ctx_out, (b * S, nh * hd), q.dtype)
-    _same_place(q, ctx_out=ctx_out)
-    _apart(dict(ctx_out=ctx_out), dict(q=q, k=k, v=v, table=table))
+    key = ("relative", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, ctx_out), None if ws is None else ws.sizes,
+           *(_sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else ()))
+    if _first_time(key):
+        b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng)
+        _whole("ctx_out", ctx_out, (b * S, nh * hd), q.dtype)
+        _same_place(q, ctx_out=ctx_out)
+        if q.is_cuda and ws is not None:
+            _check_ws(ws, q.device, b * nh * S)
+        _passed(key)
+    at = _pointers((ctx_out,), (q, k, v, table))
     if q.is_cuda:
-        if ws is not None:
-            _check_ws(ws, q.device, lse=b * nh * S)
-        return _cuda().relative_attention_fwd(q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx_out, ws)
+        return _cuda().relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws)
     ctx_out.copy_(ref.relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream))
 
 
 def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stream, ctx, ws, dq, dk, dv, dtable) -> None:
     """Gradients of :func:`relative_attention_fwd` from its inputs, its output ``ctx`` and the workspace it filled: ``dq``, ``dk``,
     ``dv`` (rows may lie apart) and ``dtable`` ``[buckets, nh]``, all written, not accumulated."""
-    b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng, dq=dq, dk=dk, dv=dv)
-    _whole("dctx", dctx, (b * S, nh * hd), q.dtype)
-    _whole("ctx", ctx, (b * S, nh * hd), q.dtype)
-    _whole("dtable", dtable, tuple(table.shape), q.dtype)
-    _same_place(q, dctx=dctx, ctx=ctx, dtable=dtable)
-    _apart(dict(dq=dq, dk=dk, dv=dv, dtable=dtable), dict(q=q, k=k, v=v, dctx=dctx, ctx=ctx, table=table))
+    key = ("relative'", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, dctx, ctx, dq, dk, dv, dtable), ws.sizes,
+           *(_sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else ()))
+    if _first_time(key):
+        b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng, dq=dq, dk=dk, dv=dv)
+        _whole("dctx", dctx, (b * S, nh * hd), q.dtype)
+        _whole("ctx", ctx, (b * S, nh * hd), q.dtype)
+        _whole("dtable", dtable, tuple(table.shape), q.dtype)
+        _same_place(q, dctx=dctx, ctx=ctx, dtable=dtable)
+        if q.is_cuda:
+            far = (buckets.numel() - 1) // 2
+            _check_ws(ws, q.device, b * nh * S, b * nh * S, b * _cuda().relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
+        _passed(key)
+    at = _pointers((dq, dk, dv, dtable), (q, k, v, dctx, ctx, table))
     if q.is_cuda:
-        far = (buckets.numel() - 1) // 2
-        _check_ws(ws, q.device, lse=b * nh * S, delta=b * nh * S,
-                  dwin=b * _cuda().relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
-        return _cuda().relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, hd, p, rng, stream, ctx, ws, dq, dk, dv, dtable)
+        return _cuda().relative_attention_bwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws, dq, dk, dv)
     g = ref.relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream)
     for out, t in zip((dq, dk, dv, dtable), g):
         out.copy_(t)
@@ -294,9 +343,6 @@ def _check_gelu8(saved, **like_x):
     _whole("saved.q", saved.q, (T, F), torch.int8)
     _whole("saved.scale", saved.scale, (T, -(-F // GELU8_BLOCK)), torch.float32)
     _refuse(T >= 2 ** 30 or T * F >= 2 ** 38, f"{T} rows of {F} are too many for one call")
-    if x.is_cuda and T:
-        for name, t in dict(like_x, **{"saved.q": saved.q}).items():
-            _refuse(t.data_ptr() % (8 if name == "saved.q" else 16) != 0, f"{name} must start on a 16-byte boundary (saved.q: 8)")
     _same_place(x, **{"saved.q": saved.q, "saved.scale": saved.scale}, **like_x)
     return T, F
 
@@ -305,12 +351,16 @@ def gelu8_fwd(x, bias, out, saved) -> None:
     """``out = gelu(x + bias)`` for ``x`` ``[T, F]`` (erf GELU); ``saved`` receives ``x + bias`` in 8 bits: 128 neighbouring
     values of a row share a scale and are held to 1/254 of the largest of them.  A block with an infinity or a NaN stands
     for NaNs.  ``out`` may be ``x`` itself."""
-    _, F = _check_gelu8(saved, x=x, out=out)
-    _whole("bias", bias, (F,), x.dtype)
-    _same_place(x, bias=bias)
-    _apart(dict(out=out), dict(bias=bias))
+    key = ("gelu8", _current(x), *_sig(x, bias, out, saved.q, saved.scale))
+    if _first_time(key):
+        _, F = _check_gelu8(saved, x=x, out=out)
+        _whole("bias", bias, (F,), x.dtype)
+        _same_place(x, bias=bias)
+        _passed(key)
+    in_place = out.data_ptr() == x.data_ptr()
+    _pointers((out,), (bias,) if in_place else (bias, x))
+    _refuse(saved.q.data_ptr() % 8 != 0, "saved.q must start on an 8-byte boundary")
     if x.is_cuda:
-        _refuse(bias.data_ptr() % 16 != 0, "bias must start on a 16-byte boundary")
         return _cuda().gelu8_fwd(x, bias, out, saved)
     y, q, scale = ref.gelu8_fwd(x, bias)
     out.copy_(y); saved.q.copy_(q); saved.scale.copy_(scale)
@@ -319,14 +369,20 @@ def gelu8_fwd(x, bias, out, saved) -> None:
 def gelu8_bwd(da, saved, ws, dbias, dx, act_out) -> None:
     """From the gradient ``da`` of the activation and the 8 bits: ``dx = da gelu'(z)``, its column sums ``dbias``, and the
     activation ``act_out = gelu(z)`` again (for the weight gradient of the linear that read it).  ``dx`` may be ``da`` itself."""
-    T, F = _check_gelu8(saved, da=da, dx=dx, act_out=act_out)
-    _whole("dbias", dbias, (F,), da.dtype)
-    _same_place(da, dbias=dbias)
-    _apart(dict(dx=dx, act_out=act_out, dbias=dbias), {})
-    _apart(dict(act_out=act_out, dbias=dbias), dict(da=da))
+    key = ("gelu8'", _current(da), *_sig(da, saved.q, saved.scale, dbias, dx, act_out), ws.numel(), ws.device)
+    if _first_time(key):
+        T, F = _check_gelu8(saved, da=da, dx=dx, act_out=act_out)
+        _whole("dbias", dbias, (F,), da.dtype)
+        _same_place(da, dbias=dbias)
+        if da.is_cuda:
+            need = _cuda().gelu8_splits(T, F) * F
+            _refuse(ws.numel() < need or ws.device != da.device or ws.dtype != torch.float32,
+                    f"the workspace is for fewer rows: {ws.numel()} values on {ws.device}, the call needs {need} on {da.device}")
+        _passed(key)
+    in_place = dx.data_ptr() == da.data_ptr()
+    _pointers((act_out, dbias) if in_place else (act_out, dbias, dx), (da,))
+    _refuse(saved.q.data_ptr() % 8 != 0, "saved.q must start on an 8-byte boundary")
     if da.is_cuda:
-        need = _cuda().gelu8_splits(T, F) * F
-        _refuse(ws.numel() < need or ws.device != da.device, f"the workspace is for fewer rows: {ws.numel()} values, the call needs {need}")
         return _cuda().gelu8_bwd(da, saved, ws, dbias, dx, act_out)
     d, a, db = ref.gelu8_bwd(da, saved.q, saved.scale)
     dx.copy_(d); act_out.copy_(a); dbias.copy_(db)
