@@ -56,11 +56,11 @@ __global__ void __launch_bounds__(W * 32) fwd_mma(Args<T> a) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   bool empty;
   const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty);
-  load_window(a, h, wd, pad, empty, win);
+  load_window(a, h, wd, pad, 0.f, win);
   const size_t row0 = (size_t)b * a.S;
   stage_rows<T, HD>(sq, a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, a.S - q0, R, nullptr, 0);
   __syncthreads();
-  const float sl2 = empty ? 0.f : a.scale_log2, up = std::is_same<T, __half>::value ? 6.f : 0.f;
+  const float sl2 = a.scale_log2, up = std::is_same<T, __half>::value ? 6.f : 0.f;
   const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
   uint32_t qa[HD / 16][4];
   load_a<T, HD>(qa, sq, w * 16, lane);
@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(W * 32) fwd_mma(Args<T> a) {
         const int c = 8 * j + (e & 1), r = e >> 1;
         const float bias = far_block ? far_bias : wp[c - 8 * r];
         const bool on = keys[j >> 2] >> ((c + 2 * t) & 31) & 1u;
-        s[j][e] = on ? fmaf(s[j][e], sl2, bias) : -INFINITY;
+        s[j][e] = empty ? 0.f : fmaf(s[j][e], sl2, bias);
+        if (!on) s[j][e] = -INFINITY;
         mx[r] = fmaxf(mx[r], s[j][e]);
       }
     float base[2];
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(W * 32) fwd_mma(Args<T> a) {
     T* dst = a.ctx + ((row0 + q) * a.nh + h) * HD + 2 * t;
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<uint32_t*>(dst + 8 * j) = pack2<T>(o[j][2 * r] * f, o[j][2 * r + 1] * f);
-    if (a.lse != nullptr && t == 0) a.lse[(size_t)bh * a.S + q] = m[r] - up + lg2(l[r]);
+    if (a.lse != nullptr && t == 0) a.lse[(size_t)bh * a.Sp + q] = m[r] - up + lg2(l[r]);
   }
 }
 
@@ -157,13 +158,13 @@ __global__ void __launch_bounds__(W * 32) bwd_q_mma(Args<T> a) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   bool empty;
   const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty);
-  load_window(a, h, wd, pad, empty, win);
+  load_window(a, h, wd, pad, 0.f, win);
   const size_t row0 = (size_t)b * a.S;
   const long long H = (long long)a.nh * HD;
   stage_rows<T, HD>(sq, a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, a.S - q0, R, nullptr, 0);
   stage_rows<T, HD>(sdo, a.dctx + (row0 + q0) * H + h * HD, H, a.S - q0, R, nullptr, 0);
   __syncthreads();
-  const float sl2 = empty ? 0.f : a.scale_log2, kept = 1.f / (1.f - a.p);
+  const float sl2 = a.scale_log2, kept = 1.f / (1.f - a.p);
   const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
   const int qi = q0 + w * 16 + g;
   const bool one = len <= KB;                                      // one block of keys: delta is the sum over its registers
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(W * 32) bwd_q_mma(Args<T> a) {
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int q = qi + 8 * r;
-    lse[r] = q < a.S ? __ldg(a.lse + (size_t)bh * a.S + q) - a.grad_log2 : INFINITY;
+    lse[r] = q < a.S ? __ldg(a.lse + (size_t)bh * a.Sp + q) - a.grad_log2 : INFINITY;
     float d = 0.f;
     if (!one && q < a.S) {                                         // dctx ctx, a quad per row
       const T* c = a.ctx + ((row0 + q) * a.nh + h) * HD + t * (HD / 4);
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(W * 32) bwd_q_mma(Args<T> a) {
         const int c = 8 * j + (e & 1), r = e >> 1;
         const float bias = far_block ? far_bias : wp[c - 8 * r];
         const bool on = keys[j >> 2] >> ((c + 2 * t) & 31) & 1u;
-        s[j][e] = on ? ex2(fmaf(s[j][e], sl2, bias) - lse[r]) : 0.f;
+        s[j][e] = on ? ex2((empty ? 0.f : fmaf(s[j][e], sl2, bias)) - lse[r]) : 0.f;
         if (a.p > 0.f) {
           const uint32_t i = ((uint32_t)bh * a.S + qi + 8 * r) * (uint32_t)a.S + k0 + c + 2 * t;
           dp[j][e] = keep(seed, a.stream, i, a.p) ? dp[j][e] * kept : 0.f;
@@ -245,8 +246,8 @@ __global__ void __launch_bounds__(W * 32) bwd_q_mma(Args<T> a) {
     if (q >= a.S) continue;
     T* dst = a.dq + (row0 + q) * a.lddq + h * HD + 2 * t;
 #pragma unroll
-    for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<uint32_t*>(dst + 8 * j) = pack2<T>(dq[j][2 * r] * f, dq[j][2 * r + 1] * f);
-    if (t == 0) a.delta[(size_t)bh * a.S + q] = delta[r];
+    for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<uint32_t*>(dst + 8 * j) = empty ? 0u : pack2<T>(dq[j][2 * r] * f, dq[j][2 * r + 1] * f);
+    if (t == 0) a.delta[(size_t)bh * a.Sp + q] = delta[r];
   }
 }
 
@@ -300,13 +301,13 @@ __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   bool empty;
   const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty);
-  load_window(a, h, wd, pad, empty, win);
+  load_window(a, h, wd, pad, 0.f, win);
   for (int i = threadIdx.x; i < W * nwin; i += W * 32) sums[i] = 0.f;
   const size_t row0 = (size_t)b * a.S;
   const long long H = (long long)a.nh * HD;
   stage_rows<T, HD>(sk, a.k + (row0 + k0) * a.ldk + h * HD, a.ldk, a.S - k0, R, bits, k0);
   stage_rows<T, HD>(sv, a.v + (row0 + k0) * a.ldv + h * HD, a.ldv, a.S - k0, R, bits, k0);
-  const float sl2 = empty ? 0.f : a.scale_log2, kept = 1.f / (1.f - a.p);
+  const float sl2 = a.scale_log2, kept = 1.f / (1.f - a.p);
   const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
   const int ki = k0 + w * 16 + g;                                   // this lane's keys: ki, ki + 8
   __syncthreads();
@@ -319,8 +320,8 @@ __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
     stage_rows<T, HD>(sq, a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, a.S - q0, QB, nullptr, 0);
     stage_rows<T, HD>(sdo, a.dctx + (row0 + q0) * H + h * HD, H, a.S - q0, QB, nullptr, 0);
     for (int i = threadIdx.x; i < QB; i += W * 32) {
-      slse[i] = q0 + i < a.S ? a.lse[(size_t)bh * a.S + q0 + i] - a.grad_log2 : INFINITY;
-      sdelta[i] = q0 + i < a.S ? a.delta[(size_t)bh * a.S + q0 + i] : 0.f;
+      slse[i] = q0 + i < a.S ? a.lse[(size_t)bh * a.Sp + q0 + i] - a.grad_log2 : INFINITY;
+      sdelta[i] = q0 + i < a.S ? a.delta[(size_t)bh * a.Sp + q0 + i] : 0.f;
     }
     __syncthreads();
     float s[QB / 8][4] = {}, dp[QB / 8][4] = {};
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
       for (int e = 0; e < 4; ++e) {
         const int c = 8 * j + (e & 1), r = e >> 1;
         const float bias = far_block ? far_bias : wp[8 * r - c];
-        const float pr = on[r] ? ex2(fmaf(s[j][e], sl2, bias) - slse[c + 2 * t]) : 0.f;
+        const float pr = on[r] ? ex2((empty ? 0.f : fmaf(s[j][e], sl2, bias)) - slse[c + 2 * t]) : 0.f;
         float kf = 1.f;
         if (a.p > 0.f) {
           const uint32_t i = ((uint32_t)bh * a.S + q0 + c + 2 * t) * (uint32_t)a.S + ki + 8 * r;
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
     T* dst2 = a.dv + (row0 + k) * a.lddv + h * HD + 2 * t;
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) {
-      *reinterpret_cast<uint32_t*>(dst + 8 * j) = pack2<T>(dk[j][2 * r] * f, dk[j][2 * r + 1] * f);
+      *reinterpret_cast<uint32_t*>(dst + 8 * j) = empty ? 0u : pack2<T>(dk[j][2 * r] * f, dk[j][2 * r + 1] * f);
       *reinterpret_cast<uint32_t*>(dst2 + 8 * j) = pack2<T>(dv[j][2 * r] * a.grad_inv, dv[j][2 * r + 1] * a.grad_inv);
     }
   }
@@ -460,7 +461,11 @@ template <typename T, int HD> int run(const Args<T>& a, bool bwd, cudaStream_t s
     default: return bwd ? run_bwd<T, HD, 4>(a, st) : run_fwd<T, HD, 4>(a, st);
   }
 }
+// The tensor-core kernels beyond 64 tokens (TODO_FIGURES)
+inline bool on_tensor_cores(int S) { return S > 64; }
+
 template <typename T> int run(const Args<T>& a, int hd, bool bwd, cudaStream_t st) {
+  if (on_tensor_cores(a.S)) return bwd ? bwd_on_tensor_cores(a, hd, st) : fwd_on_tensor_cores(a, hd, st);
   if (hd == 32) return run<T, 32>(a, bwd, st);
   if (hd == 64) return run<T, 64>(a, bwd, st);
   if (hd == 128) return run<T, 128>(a, bwd, st);
@@ -475,6 +480,7 @@ struct Common {
   float p;
   const void* seed;
   unsigned stream;
+  void* status;
 };
 template <typename T> Args<T> args(const Common& c) {
   Args<T> a = {};
@@ -485,6 +491,7 @@ template <typename T> Args<T> args(const Common& c) {
   a.scale = 1.f / sqrtf((float)c.hd);
   a.scale_log2 = LOG2E * a.scale;
   a.p = c.p; a.seed = (const int*)c.seed; a.stream = c.stream;
+  a.Sp = (c.S + 127) / 128 * 128; a.status = (int*)c.status;
   return a;
 }
 
@@ -494,12 +501,15 @@ template <typename T> Args<T> args(const Common& c) {
 using namespace rb;
 
 // Key tiles of a sequence: the backward pass leaves b * tiles rows of sums by distance
-RB_API int rb_relative_tiles(int S) { return (S + 16 * rel::warps(S) - 1) / (16 * rel::warps(S)); }
+RB_API int rb_relative_tiles(int S) {
+  const int rows = rel::on_tensor_cores(S) ? 128 : 16 * rel::warps(S);
+  return (S + rows - 1) / rows;
+}
 
 RB_API int rb_relative_fwd(int dtype, const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* mask,
                            const void* table, const void* lut, int far, int nb, int b, int S, int nh, int hd, float p, const void* seed,
-                           unsigned stream, void* ctx, void* lse, cudaStream_t st) {
-  const rel::Common c{q, k, v, ldq, ldk, ldv, mask, table, lut, far, nb, b, S, nh, hd, p, seed, stream};
+                           unsigned stream, void* status, void* ctx, void* lse, cudaStream_t st) {
+  const rel::Common c{q, k, v, ldq, ldk, ldv, mask, table, lut, far, nb, b, S, nh, hd, p, seed, stream, status};
   auto go = [&](auto t) {
     using T = decltype(t);
     rel::Args<T> a = rel::args<T>(c);
@@ -513,9 +523,9 @@ RB_API int rb_relative_fwd(int dtype, const void* q, long long ldq, const void* 
 
 RB_API int rb_relative_bwd(int dtype, const void* dctx, const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
                            const void* mask, const void* table, const void* lut, int far, int nb, int b, int S, int nh, int hd, float p,
-                           const void* seed, unsigned stream, const void* ctx, const void* lse, void* delta, void* dwin, void* dq, long long lddq,
+                           const void* seed, unsigned stream, void* status, const void* ctx, const void* lse, void* delta, void* dwin, void* dq, long long lddq,
                            void* dk, long long lddk, void* dv, long long lddv, void* dtable, cudaStream_t st) {
-  const rel::Common c{q, k, v, ldq, ldk, ldv, mask, table, lut, far, nb, b, S, nh, hd, p, seed, stream};
+  const rel::Common c{q, k, v, ldq, ldk, ldv, mask, table, lut, far, nb, b, S, nh, hd, p, seed, stream, status};
   auto go = [&](auto t) {
     using T = decltype(t);
     rel::Args<T> a = rel::args<T>(c);

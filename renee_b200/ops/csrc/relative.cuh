@@ -32,7 +32,9 @@ template <typename T> struct Args {
   const int* seed;
   uint32_t stream;
   T* ctx;                        // [b S][nh HD]
-  float *lse, *delta;            // [b][nh][S]; lse in base 2, of the scaled and biased scores
+  float *lse, *delta;            // [b][nh][Sp]; lse in base 2, of the scaled and biased scores; behind S infinity and zero
+  int Sp;                        // S rounded up to 128
+  int* status;                   // where a wait that ran out is noted
   // backward
   const T* dctx;
   T *dq, *dk, *dv;
@@ -67,15 +69,14 @@ __device__ __forceinline__ int attended(const int* mask, int S, uint32_t* bits, 
   return S;
 }
 
-// win[i] = bias of distance clamp(i - pad, -wd, wd), i < 2 wd + 1 + 2 pad, times log2 e; zeros for an empty sequence.
-// With `mirror` entry i holds distance pad - i: kernels whose columns are queries read it upwards.
+// win[i] = bias of distance clamp(i - pad - wd, -wd, wd), i < 2 wd + 1 + 2 pad, times log2 e, plus a constant.
 template <typename T>
-__device__ __forceinline__ void load_window(const Args<T>& a, int h, int wd, int pad, bool empty, float* win) {
+__device__ __forceinline__ void load_window(const Args<T>& a, int h, int wd, int pad, float add, float* win) {
   const int n = 2 * wd + 1 + 2 * pad;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const int d = min(max(i - pad - wd, -wd), wd);
     const int u = min(max(__ldg(a.lut + d + a.far), 0), a.nb - 1);       // a bucket outside the table reads its nearest row
-    win[i] = empty ? 0.f : to_f(a.table[(size_t)u * a.nh + h]) * LOG2E;
+    win[i] = fmaf(to_f(a.table[(size_t)u * a.nh + h]), LOG2E, add);
   }
 }
 
@@ -89,6 +90,10 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// The kernels of relative_tc.cu, for sequences of more than 64 tokens
+template <typename T> int fwd_on_tensor_cores(const Args<T>& a, int hd, cudaStream_t st);
+template <typename T> int bwd_on_tensor_cores(const Args<T>& a, int hd, cudaStream_t st);
 
 }  // namespace rel
 }  // namespace rb

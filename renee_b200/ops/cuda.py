@@ -409,7 +409,7 @@ def bias_gelu_bwd(da, x, bias, dbias, dx_out):
 # Entry points whose argument types are set, so that they take Python's numbers as they are (wrapping each costs 0.25 us, and the
 # kernels of a small call take 5): p = address, l = long long, i = int, u = unsigned, f = float.  The stream is the last argument.
 _KINDS = {"p": _VP, "l": _LL, "i": _I, "u": _U, "f": _F}
-_RELATIVE_INPUTS = "plplplpppiiiiiifpu"
+_RELATIVE_INPUTS = "plplplpppiiiiiifpup"
 _TYPES = {
     "rb_qk_norm_rotary_fwd": "iplppppplliiiifp",
     "rb_qk_norm_rotary_bwd": "iplplpppppplpp" + "liiiifp",
@@ -464,7 +464,8 @@ def relative_tiles(S: int) -> int:
 def _relative_inputs(at, q, k, v, mask, table, buckets, nh, p, rng, stream):
     b, S = mask.shape
     return (at[0], _ld(q), at[1], _ld(k), at[2], _ld(v), mask.data_ptr(), table.data_ptr(), buckets.data_ptr(), (buckets.shape[0] - 1) // 2,
-            table.shape[0], b, S, nh, q.shape[1] // nh, p, rng.dev.data_ptr() if p > 0 else None, stream)
+            table.shape[0], b, S, nh, q.shape[1] // nh, p, rng.dev.data_ptr() if p > 0 else None, stream,
+            workspace(q.device).status.data_ptr())
 
 
 def relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):

@@ -225,11 +225,12 @@ def relative_attention_workspace(b: int, S: int, nh: int, hd: int, max_distance:
     if torch.device(device).type == "cpu":
         return RelativeWorkspace(*[torch.empty(0)] * 3)
     e = lambda n, name: guard.empty(max(n, 1), dtype=torch.float32, device=device, name=f"relative_attention.{name}")
-    lse = e(b * nh * S, "lse")
+    stats = b * nh * (-(-S // 128) * 128)         # the statistics of a sequence take whole tiles of 128 rows
+    lse = e(stats, "lse")
     if scratch is not None:
         return RelativeWorkspace(lse, scratch.delta, scratch.dwin)
     tiles = _cuda().relative_tiles(S)
-    return RelativeWorkspace(lse, e(b * nh * S, "delta"), e(b * tiles * nh * (2 * min(max_distance, S - 1) + 1), "dwin"))
+    return RelativeWorkspace(lse, e(stats, "delta"), e(b * tiles * nh * (2 * min(max_distance, S - 1) + 1), "dwin"))
 
 
 def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
@@ -277,7 +278,7 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ct
         _whole("ctx_out", ctx_out, (b * S, nh * hd), q.dtype)
         _same_place(q, ctx_out=ctx_out)
         if q.is_cuda and ws is not None:
-            _check_ws(ws, q.device, b * nh * S)
+            _check_ws(ws, q.device, b * nh * (-(-S // 128) * 128))
         _passed(key)
     at = _pointers((ctx_out,), (q, k, v, table))
     if q.is_cuda:
@@ -298,7 +299,8 @@ def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stre
         _same_place(q, dctx=dctx, ctx=ctx, dtable=dtable)
         if q.is_cuda:
             far = (buckets.numel() - 1) // 2
-            _check_ws(ws, q.device, b * nh * S, b * nh * S, b * _cuda().relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
+            stats = b * nh * (-(-S // 128) * 128)
+            _check_ws(ws, q.device, stats, stats, b * _cuda().relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
         _passed(key)
     at = _pointers((dq, dk, dv, dtable), (q, k, v, dctx, ctx, table))
     if q.is_cuda:

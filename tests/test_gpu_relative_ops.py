@@ -107,6 +107,22 @@ def test_attention_far_scores():
     torch.testing.assert_close(a.ctx.double().cpu(), want["ctx"], rtol=2.0 ** -7, atol=2.0 ** -8 * 4)
 
 
+@pytest.mark.parametrize("S", [33, 200])
+def test_attention_of_an_empty_sequence_reads_no_scores(S):
+    """Where nothing is attended, q and k do not matter, NaNs included, and have no gradient."""
+    c = attention_inputs(3, S, 2, 64, torch.bfloat16, "empty", poison=False)
+    clean = Attention(c)
+    nans = c["qk"].clone()
+    nans[S:2 * S] = float("nan")
+    dirty = Attention(dict(c, qk=nans))
+    for a in (clean, dirty):
+        a.fwd()
+        a.bwd()
+    clean.check()
+    assert torch.equal(clean.ctx, dirty.ctx) and torch.equal(clean.wide, dirty.wide) and torch.equal(clean.dtable, dirty.dtable)
+    assert not dirty.dq[S:2 * S].any() and not dirty.dk[S:2 * S].any()
+
+
 def test_attention_same_bits_again():
     c = attention_inputs(3, 200, 2, 64, torch.bfloat16, "holes")
     got = []
