@@ -2,7 +2,7 @@
 // 64 and 128, any length (formulas and conventions: relative.cuh).
 //
 // Scores are never stored: the forward pass keeps a running maximum and sum per query and leaves the logarithm of the sum, from
-// which the backward passes compute P again.  Three launches backward, all sums in a fixed order:
+// which the backward passes compute P again.  Forward: prepare (bias by distance, masks as bits), fwd.  Three launches backward, all sums in a fixed order:
 //   bwd_q   a CTA owns query rows, walks the keys: delta, dq
 //   bwd_kv  a CTA owns key rows, walks the queries: dk, dv, and dS summed by distance
 //   dtable  sums of all CTAs by distance, then by bucket
@@ -38,25 +38,69 @@ struct Carve {
   }
 };
 
+// ------------------------------------------------------------------------------------------------ windows and masks
+// CTAs 0 .. nh - 1: a head's bias by distance; the others: a sequence's mask as bits
+template <typename T>
+__global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ table, const int* __restrict__ lut, const int* __restrict__ mask,
+                                                      float* __restrict__ win, uint32_t* __restrict__ bits, int* __restrict__ lens, int far, int nb,
+                                                      int S, int nh) {
+  grid_dep_wait();
+  if ((int)blockIdx.x < nh) {
+    const int wd = min(far, S - 1), n = window_floats(wd);
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const int d = min(max(i - PAD - wd, -wd), wd);
+      const int u = min(max(__ldg(lut + d + far), 0), nb - 1);            // a bucket outside the table reads its nearest row
+      win[(size_t)blockIdx.x * n + i] = to_f(table[(size_t)u * nh + blockIdx.x]) * LOG2E;
+    }
+    return;
+  }
+  __shared__ int s_len;
+  const int b = blockIdx.x - nh, lane = threadIdx.x & 31, words = mask_words(S);
+  const int* row = mask + (size_t)b * S;
+  if (threadIdx.x == 0) s_len = 0;
+  __syncthreads();
+  int last = 0;
+#pragma unroll 4
+  for (int w = threadIdx.x >> 5; w < words; w += 8) {
+    const int s = 32 * w + lane;
+    const uint32_t m = __ballot_sync(0xffffffffu, s < S && __ldg(row + s) != 0);
+    if (lane == 0) bits[(size_t)b * words + w] = m;
+    if (m) last = 32 * w + 32 - __clz((int)m);
+  }
+  if (lane == 0 && last) atomicMax(&s_len, last);
+  __syncthreads();
+  if (threadIdx.x == 0) lens[b] = s_len;
+  if (s_len == 0)
+    for (int w = threadIdx.x; w < words; w += 256)
+      bits[(size_t)b * words + w] = S - 32 * w >= 32 ? 0xffffffffu : S > 32 * w ? (1u << (S - 32 * w)) - 1u : 0u;
+}
+
+// A CTA's copy of its head's window and its sequence's mask, in whole 16-byte pieces
+template <typename T> __device__ __forceinline__ void copy_window(const Args<T>& a, int b, int h, int wd, float* win, uint32_t* bits) {
+  const int n = window_floats(wd), words = mask_words(a.S);
+  for (int i = threadIdx.x * 4; i < n; i += blockDim.x * 4) *reinterpret_cast<float4*>(win + i) = *reinterpret_cast<const float4*>(a.win + (size_t)h * n + i);
+  for (int i = threadIdx.x * 4; i < words; i += blockDim.x * 4)
+    *reinterpret_cast<uint4*>(bits + i) = *reinterpret_cast<const uint4*>(a.bits + (size_t)b * words + i);
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int HD, int W>
 __global__ void __launch_bounds__(W * 32) fwd_mma(Args<T> a) {
   constexpr int R = W * 16, KB = 64;
   extern __shared__ __align__(16) char smem[];
-  __shared__ int s_len;
-  const int wd = window(a), pad = R + KB, qt = (a.S + R - 1) / R;
+  const int wd = window(a), qt = (a.S + R - 1) / R;
   Carve cv{smem};
   T* sq = cv.take<T>(R * (HD + 8));
   T* sk = cv.take<T>(KB * (HD + 8));
   T* sv = cv.take<T>(KB * (HD + 8));
-  float* win = cv.take<float>(2 * wd + 1 + 2 * pad);
-  uint32_t* bits = cv.take<uint32_t>((a.S + 31) / 32);
+  float* win = cv.take<float>(window_floats(wd));
+  uint32_t* bits = cv.take<uint32_t>(mask_words(a.S));
   grid_dep_wait();
   const int bh = blockIdx.x / qt, b = bh / a.nh, h = bh % a.nh, q0 = (blockIdx.x % qt) * R;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  bool empty;
-  const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty);
-  load_window(a, h, wd, pad, 0.f, win);
+  const int seen = __ldg(a.lens + b), len = seen > 0 ? seen : a.S;
+  const bool empty = seen == 0;
+  copy_window(a, b, h, wd, win, bits);
   const size_t row0 = (size_t)b * a.S;
   stage_rows<T, HD>(sq, a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, a.S - q0, R, nullptr, 0);
   __syncthreads();
@@ -77,9 +121,9 @@ __global__ void __launch_bounds__(W * 32) fwd_mma(Args<T> a) {
     // distance of column 2t of the first tile to row qi; beyond the window the block's bias is one number
     const int dlo = k0 - (q0 + R - 1), dhi = k0 + KB - 1 - q0;
     const bool far_block = dhi <= -wd || dlo >= wd;
-    const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * pad];
-    const float* wp = win + (k0 + 2 * t - qi) + wd + pad;
-    const uint32_t keys[2] = {bits[k0 >> 5], k0 + 32 < a.S ? bits[(k0 >> 5) + 1] : 0u};
+    const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+    const float* wp = win + (k0 + 2 * t - qi) + wd + PAD;
+    const uint32_t keys[2] = {bits[k0 >> 5], bits[(k0 >> 5) + 1]};
 #pragma unroll
     for (int j = 0; j < KB / 8; ++j)
 #pragma unroll
@@ -144,21 +188,20 @@ template <typename T, int HD, int W>
 __global__ void __launch_bounds__(W * 32) bwd_q_mma(Args<T> a) {
   constexpr int R = W * 16, KB = HD == 128 ? 32 : 64;
   extern __shared__ __align__(16) char smem[];
-  __shared__ int s_len;
-  const int wd = window(a), pad = R + KB, qt = (a.S + R - 1) / R;
+  const int wd = window(a), qt = (a.S + R - 1) / R;
   Carve cv{smem};
   T* sq = cv.take<T>(R * (HD + 8));
   T* sdo = cv.take<T>(R * (HD + 8));
   T* sk = cv.take<T>(KB * (HD + 8));
   T* sv = cv.take<T>(KB * (HD + 8));
-  float* win = cv.take<float>(2 * wd + 1 + 2 * pad);
-  uint32_t* bits = cv.take<uint32_t>((a.S + 31) / 32);
+  float* win = cv.take<float>(window_floats(wd));
+  uint32_t* bits = cv.take<uint32_t>(mask_words(a.S));
   grid_dep_wait();
   const int bh = blockIdx.x / qt, b = bh / a.nh, h = bh % a.nh, q0 = (blockIdx.x % qt) * R;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  bool empty;
-  const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty);
-  load_window(a, h, wd, pad, 0.f, win);
+  const int seen = __ldg(a.lens + b), len = seen > 0 ? seen : a.S;
+  const bool empty = seen == 0;
+  copy_window(a, b, h, wd, win, bits);
   const size_t row0 = (size_t)b * a.S;
   const long long H = (long long)a.nh * HD;
   stage_rows<T, HD>(sq, a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, a.S - q0, R, nullptr, 0);
@@ -204,9 +247,9 @@ __global__ void __launch_bounds__(W * 32) bwd_q_mma(Args<T> a) {
     }
     const int dlo = k0 - (q0 + R - 1), dhi = k0 + KB - 1 - q0;
     const bool far_block = dhi <= -wd || dlo >= wd;
-    const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * pad];
-    const float* wp = win + (k0 + 2 * t - qi) + wd + pad;
-    const uint32_t keys[2] = {bits[k0 >> 5], KB > 32 && k0 + 32 < a.S ? bits[(k0 >> 5) + 1] : 0u};
+    const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+    const float* wp = win + (k0 + 2 * t - qi) + wd + PAD;
+    const uint32_t keys[2] = {bits[k0 >> 5], KB > 32 ? bits[(k0 >> 5) + 1] : 0u};
 #pragma unroll
     for (int j = 0; j < KB / 8; ++j)
 #pragma unroll
@@ -247,7 +290,10 @@ __global__ void __launch_bounds__(W * 32) bwd_q_mma(Args<T> a) {
     T* dst = a.dq + (row0 + q) * a.lddq + h * HD + 2 * t;
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) *reinterpret_cast<uint32_t*>(dst + 8 * j) = empty ? 0u : pack2<T>(dq[j][2 * r] * f, dq[j][2 * r + 1] * f);
-    if (t == 0) a.delta[(size_t)bh * a.Sp + q] = delta[r];
+    if (t == 0) {
+      a.delta[(size_t)bh * a.Sp + q] = delta[r];
+      a.lse_up[(size_t)bh * a.Sp + q] = lse[r];
+    }
   }
 }
 
@@ -283,8 +329,7 @@ template <typename T, int HD, int W>
 __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
   constexpr int R = W * 16, QB = HD == 128 ? 32 : 64;
   extern __shared__ __align__(16) char smem[];
-  __shared__ int s_len;
-  const int wd = window(a), pad = R + QB, kt = (a.S + R - 1) / R, nwin = 2 * wd + 1;
+  const int wd = window(a), kt = (a.S + R - 1) / R, nwin = 2 * wd + 1;
   Carve cv{smem};
   T* sk = cv.take<T>(R * (HD + 8));
   T* sv = cv.take<T>(R * (HD + 8));
@@ -293,18 +338,19 @@ __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
   float* slse = cv.take<float>(QB);
   float* sdelta = cv.take<float>(QB);
   float* tile = cv.take<float>(W * 16 * (QB + 4));
-  float* win = cv.take<float>(nwin + 2 * pad);
+  float* win = cv.take<float>(window_floats(wd));
   float* sums = cv.take<float>(W * nwin);
-  uint32_t* bits = cv.take<uint32_t>((a.S + 31) / 32);
+  uint32_t* bits = cv.take<uint32_t>(mask_words(a.S));
   grid_dep_wait();
   const int bh = blockIdx.x / kt, b = bh / a.nh, h = bh % a.nh, ktile = blockIdx.x % kt, k0 = ktile * R;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  bool empty;
-  const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty);
-  load_window(a, h, wd, pad, 0.f, win);
+  const int seen = __ldg(a.lens + b), len = seen > 0 ? seen : a.S;
+  const bool empty = seen == 0;
+  copy_window(a, b, h, wd, win, bits);
   for (int i = threadIdx.x; i < W * nwin; i += W * 32) sums[i] = 0.f;
   const size_t row0 = (size_t)b * a.S;
   const long long H = (long long)a.nh * HD;
+  __syncthreads();
   stage_rows<T, HD>(sk, a.k + (row0 + k0) * a.ldk + h * HD, a.ldk, a.S - k0, R, bits, k0);
   stage_rows<T, HD>(sv, a.v + (row0 + k0) * a.ldv + h * HD, a.ldv, a.S - k0, R, bits, k0);
   const float sl2 = a.scale_log2, kept = 1.f / (1.f - a.p);
@@ -320,7 +366,7 @@ __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
     stage_rows<T, HD>(sq, a.q + (row0 + q0) * a.ldq + h * HD, a.ldq, a.S - q0, QB, nullptr, 0);
     stage_rows<T, HD>(sdo, a.dctx + (row0 + q0) * H + h * HD, H, a.S - q0, QB, nullptr, 0);
     for (int i = threadIdx.x; i < QB; i += W * 32) {
-      slse[i] = q0 + i < a.S ? a.lse[(size_t)bh * a.Sp + q0 + i] - a.grad_log2 : INFINITY;
+      slse[i] = q0 + i < a.S ? a.lse_up[(size_t)bh * a.Sp + q0 + i] : INFINITY;
       sdelta[i] = q0 + i < a.S ? a.delta[(size_t)bh * a.Sp + q0 + i] : 0.f;
     }
     __syncthreads();
@@ -334,8 +380,8 @@ __global__ void __launch_bounds__(W * 32) bwd_kv_mma(Args<T> a) {
     }
     const int dlo = k0 - (q0 + QB - 1), dhi = k0 + R - 1 - q0;
     const bool far_block = dhi <= -wd || dlo >= wd;
-    const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * pad];
-    const float* wp = win + (ki - q0 - 2 * t) + wd + pad;
+    const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+    const float* wp = win + (ki - q0 - 2 * t) + wd + PAD;
     // P~ (kept probabilities) in s for dv, dS in dp
 #pragma unroll
     for (int j = 0; j < QB / 8; ++j)
@@ -407,7 +453,7 @@ __global__ void __launch_bounds__(1024) dtable_kernel(const float* __restrict__ 
   for (int i = threadIdx.x; i < groups * nwin; i += blockDim.x) {
     const int gr = i / nwin, d = i - gr * nwin;
     float v = 0.f;
-#pragma unroll 4
+#pragma unroll 16
     for (int pt = gr; pt < parts; pt += groups) v += __ldcg(dwin + ((size_t)pt * nh + h) * nwin + d);
     sm[i] = v;
   }
@@ -433,11 +479,10 @@ inline int warps(int S) { return S > 32 ? 4 : S > 16 ? 2 : 1; }
 template <typename K> int set_smem(K kernel, int bytes) {
   return bytes <= 48 * 1024 ? 0 : (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
-inline int up16(int bytes) { return (bytes + 15) / 16 * 16; }
 
 template <typename T, int HD, int W> int run_fwd(const Args<T>& a, cudaStream_t st) {
   constexpr int R = 16 * W, KB = 64;
-  const int smem = (R + 2 * KB) * (HD + 8) * 2 + up16((2 * window(a) + 1 + 2 * (R + KB)) * 4) + up16((a.S + 31) / 32 * 4);
+  const int smem = (R + 2 * KB) * (HD + 8) * 2 + (window_floats(window(a)) + mask_words(a.S)) * 4;
   const int rc = set_smem(fwd_mma<T, HD, W>, smem);
   return rc ? rc : (int)launch_pdl(fwd_mma<T, HD, W>, dim3((unsigned)((a.S + R - 1) / R * a.nh * a.b)), dim3(32 * W), smem, st, a);
 }
@@ -445,7 +490,7 @@ template <typename T, int HD, int W> int run_fwd(const Args<T>& a, cudaStream_t 
 template <typename T, int HD, int W> int run_bwd(const Args<T>& a, cudaStream_t st) {
   constexpr int R = 16 * W, NB = HD == 128 ? 32 : 64;
   const int wd = window(a), nwin = 2 * wd + 1, tiles = (a.S + R - 1) / R;
-  const int base = (2 * R + 2 * NB) * (HD + 8) * 2 + up16((nwin + 2 * (R + NB)) * 4) + up16((a.S + 31) / 32 * 4);
+  const int base = (2 * R + 2 * NB) * (HD + 8) * 2 + (window_floats(wd) + mask_words(a.S)) * 4;
   const int kv = base + 2 * NB * 4 + W * 16 * (NB + 4) * 4 + up16(W * nwin * 4);
   int rc = set_smem(bwd_q_mma<T, HD, W>, base);
   if (!rc) rc = set_smem(bwd_kv_mma<T, HD, W>, kv);
@@ -475,8 +520,8 @@ template <typename T> int run(const Args<T>& a, int hd, bool bwd, cudaStream_t s
 struct Common {
   const void *q, *k, *v;
   long long ldq, ldk, ldv;
-  const void *mask, *table, *lut;
   int far, nb, b, S, nh, hd;
+  const void *win, *bits, *lens;
   float p;
   const void* seed;
   unsigned stream;
@@ -486,7 +531,7 @@ template <typename T> Args<T> args(const Common& c) {
   Args<T> a = {};
   a.q = (const T*)c.q; a.k = (const T*)c.k; a.v = (const T*)c.v;
   a.ldq = c.ldq; a.ldk = c.ldk; a.ldv = c.ldv;
-  a.mask = (const int*)c.mask; a.table = (const T*)c.table; a.lut = (const int*)c.lut;
+  a.win = (const float*)c.win; a.bits = (const uint32_t*)c.bits; a.lens = (const int*)c.lens;
   a.far = c.far; a.nb = c.nb; a.b = c.b; a.S = c.S; a.nh = c.nh;
   a.scale = 1.f / sqrtf((float)c.hd);
   a.scale_log2 = LOG2E * a.scale;
@@ -506,33 +551,39 @@ RB_API int rb_relative_tiles(int S) {
   return (S + rows - 1) / rows;
 }
 
-RB_API int rb_relative_fwd(int dtype, const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, const void* mask,
-                           const void* table, const void* lut, int far, int nb, int b, int S, int nh, int hd, float p, const void* seed,
-                           unsigned stream, void* status, void* ctx, void* lse, cudaStream_t st) {
-  const rel::Common c{q, k, v, ldq, ldk, ldv, mask, table, lut, far, nb, b, S, nh, hd, p, seed, stream, status};
+// Floats of a head's window and words of a sequence's mask in the workspace
+RB_API int rb_relative_window_floats(int far, int S) { return rel::window_floats(far < S - 1 ? far : S - 1); }
+
+RB_API int rb_relative_fwd(int dtype, const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv, int far, int nb, int b,
+                           int S, int nh, int hd, void* win, void* bits, void* lens, float p, const void* seed, unsigned stream, void* status,
+                           const void* mask, const void* table, const void* lut, void* ctx, void* lse, cudaStream_t st) {
+  const rel::Common c{q, k, v, ldq, ldk, ldv, far, nb, b, S, nh, hd, win, bits, lens, p, seed, stream, status};
   auto go = [&](auto t) {
     using T = decltype(t);
     rel::Args<T> a = rel::args<T>(c);
     a.ctx = (T*)ctx;
     a.lse = (float*)lse;
-    return rel::run<T>(a, hd, false, st);
+    const int rc = (int)launch_pdl(rel::prepare_kernel<T>, dim3(nh + b), dim3(256), 0, st, (const T*)table, (const int*)lut, (const int*)mask,
+                                   (float*)win, (uint32_t*)bits, (int*)lens, far, nb, S, nh);
+    return rc ? rc : rel::run<T>(a, hd, false, st);
   };
   if (b == 0) return 0;
   return dtype == RB_BF16 ? go(__nv_bfloat16()) : dtype == RB_F16 ? go(__half()) : -1;
 }
 
 RB_API int rb_relative_bwd(int dtype, const void* dctx, const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
-                           const void* mask, const void* table, const void* lut, int far, int nb, int b, int S, int nh, int hd, float p,
-                           const void* seed, unsigned stream, void* status, const void* ctx, const void* lse, void* delta, void* dwin, void* dq, long long lddq,
-                           void* dk, long long lddk, void* dv, long long lddv, void* dtable, cudaStream_t st) {
-  const rel::Common c{q, k, v, ldq, ldk, ldv, mask, table, lut, far, nb, b, S, nh, hd, p, seed, stream, status};
+                           int far, int nb, int b, int S, int nh, int hd, const void* win, const void* bits, const void* lens, float p,
+                           const void* seed, unsigned stream, void* status, const void* lut, const void* ctx, const void* lse, void* stats, void* dwin,
+                           void* dq, long long lddq, void* dk, long long lddk, void* dv, long long lddv, void* dtable, cudaStream_t st) {
+  const rel::Common c{q, k, v, ldq, ldk, ldv, far, nb, b, S, nh, hd, win, bits, lens, p, seed, stream, status};
   auto go = [&](auto t) {
     using T = decltype(t);
     rel::Args<T> a = rel::args<T>(c);
     a.dctx = (const T*)dctx;
     a.ctx = (T*)const_cast<void*>(ctx);
     a.lse = (float*)const_cast<void*>(lse);
-    a.delta = (float*)delta;
+    a.delta = (float*)stats;
+    a.lse_up = a.delta + (size_t)b * nh * a.Sp;
     a.dwin = (float*)dwin;
     a.dq = (T*)dq; a.dk = (T*)dk; a.dv = (T*)dv;
     a.lddq = lddq; a.lddk = lddk; a.lddv = lddv;

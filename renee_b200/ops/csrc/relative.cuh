@@ -5,10 +5,12 @@
 //   dq_i = sum_j dS_ij k_j / sqrt(HD),  dk_j = sum_i dS_ij q_i / sqrt(HD),  dv_j = sum_i P_ij keep_ij / (1 - p) dctx_i,
 //   dtable[u][h] = sum of dS_ij over all i, j with bucket(j - i) = u
 //
-// The bias depends on the distance d = j - i alone, and is constant beyond +-far: a CTA gathers its head's 2 far + 1 values once
-// into a window in shared memory (times log2 e, as all scores are in base 2) and reads win[d]; a block of keys that lies beyond
-// +-far of all its queries adds one number.  The gradient goes the same way back: dS is summed along its diagonals first, and the
-// window of sums by distance is mapped to buckets behind all CTAs (dtable_kernel), so the map may be any.
+// The bias depends on the distance d = j - i alone, and is constant beyond +-far: a launch of its own (prepare_kernel) lays out each
+// head's 2 far + 1 values as a window by distance (times log2 e, as all scores are in base 2), and the masks as bits.  A CTA copies
+// its head's window to shared memory and reads win[d]; a block of keys that lies beyond +-far of all its queries adds one number.
+// The gradient goes the same way back: dS is summed along its diagonals first, and the window of sums by distance is mapped to
+// buckets behind all CTAs (dtable_kernel), so the map may be any.  (Gathered by every CTA for itself, the window and the mask were
+// 5 us of a CTA's 12 to 18 at 512 tokens: two dependent loads per entry, and ballots.)
 // A masked key counts as absent: its K and V rows are read as zeros, whatever they hold.  A sequence without any attended key
 // attends to all of its S tokens alike (P = 1 / S): its scores are constants, so only v has a gradient there.
 #pragma once
@@ -22,17 +24,18 @@ constexpr float LOG2E = 1.4426950408889634f;
 template <typename T> struct Args {
   const T *q, *k, *v;            // rows b S + s, head h in columns h HD ..; row strides in elements
   long long ldq, ldk, ldv;
-  const int* mask;               // [b][S], 0 = masked
-  const T* table;                // [nb][nh]
-  const int* lut;                // [2 far + 1] bucket of d + far
   int far, nb, b, S, nh;
+  const float* win;              // [nh][window_floats] bias by distance, base 2
+  const uint32_t* bits;          // [b][mask_words] attended keys (an empty sequence: all)
+  const int* lens;               // [b] position behind the last attended key; 0 = nothing is attended
   float scale_log2;              // log2(e) / sqrt(HD)
   float scale;                   // 1 / sqrt(HD)
   float p;
   const int* seed;
   uint32_t stream;
   T* ctx;                        // [b S][nh HD]
-  float *lse, *delta;            // [b][nh][Sp]; lse in base 2, of the scaled and biased scores; behind S infinity and zero
+  float *lse;                    // [b][nh][Sp] in base 2, of the scaled and biased scores
+  float *delta, *lse_up;         // the same shape, from the queries' backward pass: delta, and lse - grad_log2; behind S zero and infinity
   int Sp;                        // S rounded up to 128
   int* status;                   // where a wait that ran out is noted
   // backward
@@ -46,39 +49,10 @@ template <typename T> struct Args {
 // Distances that occur within the window: beyond S - 1 there are none
 template <typename T> __host__ __device__ __forceinline__ int window(const Args<T>& a) { return a.far < a.S - 1 ? a.far : a.S - 1; }
 
-// Attended keys of sequence b as bits, and the position behind the last one.  `empty`: nothing is attended, all S count.
-// bits holds (S + 31) / 32 words; every thread of the CTA calls this.
-__device__ __forceinline__ int attended(const int* mask, int S, uint32_t* bits, int* s_len, bool& empty) {
-  const int lane = threadIdx.x & 31, words = (S + 31) / 32;
-  if (threadIdx.x == 0) *s_len = 0;
-  __syncthreads();
-  int last = 0;
-  for (int w = threadIdx.x >> 5; w < words; w += blockDim.x >> 5) {
-    const int s = 32 * w + lane;
-    const uint32_t m = __ballot_sync(0xffffffffu, s < S && __ldg(mask + s) != 0);
-    if (lane == 0) bits[w] = m;
-    if (m) last = 32 * w + 32 - __clz((int)m);
-  }
-  if (lane == 0 && last) atomicMax(s_len, last);
-  __syncthreads();
-  const int len = *s_len;
-  empty = len == 0;
-  if (!empty) return len;
-  for (int w = threadIdx.x; w < words; w += blockDim.x) bits[w] = S - 32 * w >= 32 ? 0xffffffffu : (1u << (S - 32 * w)) - 1u;
-  __syncthreads();
-  return S;
-}
-
-// win[i] = bias of distance clamp(i - pad - wd, -wd, wd), i < 2 wd + 1 + 2 pad, times log2 e, plus a constant.
-template <typename T>
-__device__ __forceinline__ void load_window(const Args<T>& a, int h, int wd, int pad, float add, float* win) {
-  const int n = 2 * wd + 1 + 2 * pad;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int d = min(max(i - pad - wd, -wd), wd);
-    const int u = min(max(__ldg(a.lut + d + a.far), 0), a.nb - 1);       // a bucket outside the table reads its nearest row
-    win[i] = fmaf(to_f(a.table[(size_t)u * a.nh + h]), LOG2E, add);
-  }
-}
+// Entry i of a head's window is the bias of distance clamp(i - PAD - wd, -wd, wd): a block that reaches beyond the window reads on
+constexpr int PAD = 192;
+__host__ __device__ __forceinline__ int window_floats(int wd) { return (2 * wd + 1 + 2 * PAD + 3) / 4 * 4; }
+__host__ __device__ __forceinline__ int mask_words(int S) { return (S + 127) / 128 * 4; }       // whole tiles of 128, zeros behind S
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -90,6 +64,8 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+inline int up16(int bytes) { return (bytes + 15) / 16 * 16; }
 
 // The kernels of relative_tc.cu, for sequences of more than 64 tokens
 template <typename T> int fwd_on_tensor_cores(const Args<T>& a, int hd, cudaStream_t st);

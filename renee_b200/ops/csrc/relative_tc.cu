@@ -19,7 +19,7 @@ namespace rel {
 
 constexpr int ROWS = 128, BLK = 64;
 
-struct alignas(64) Maps { CUtensorMap a, b, c, d; };
+struct alignas(64) Maps { CUtensorMap a, b, c, d, e; };
 
 template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
@@ -96,8 +96,8 @@ template <typename T> __device__ __forceinline__ void store_rows(char* stage, co
   }
 }
 
-constexpr int MAX_STAGES = 4;
-struct Bars { uint64_t own, full[MAX_STAGES], empty[MAX_STAGES], scores[2], done[2], end; };
+constexpr int MAX_STAGES = 3;
+struct Bars { uint64_t own, full[MAX_STAGES], empty[MAX_STAGES], scores, done, read, end; };
 
 __device__ __forceinline__ char* align1k(char* p) { return p + ((1024u - (tc::smem_u32(p) & 1023u)) & 1023u); }
 
@@ -106,8 +106,10 @@ __device__ __forceinline__ uint32_t start(Bars* bars, uint32_t* s_tmem, int warp
   if (threadIdx.x == 0) {
     tc::mbar_init(&bars->own, 1);
     tc::mbar_init(&bars->end, 1);
+    tc::mbar_init(&bars->scores, 1);
+    tc::mbar_init(&bars->done, writers);
+    tc::mbar_init(&bars->read, writers);
     for (int i = 0; i < MAX_STAGES; ++i) { tc::mbar_init(bars->full + i, 1); tc::mbar_init(bars->empty + i, 1); }
-    for (int i = 0; i < 2; ++i) { tc::mbar_init(bars->scores + i, 1); tc::mbar_init(bars->done + i, writers); }
     tc::fence_barrier_init();
   }
   if (warp == control) tc::tmem_alloc(s_tmem, cols);
@@ -115,6 +117,30 @@ __device__ __forceinline__ uint32_t start(Bars* bars, uint32_t* s_tmem, int warp
   __syncthreads();
   tc::tc_fence_after();
   return *s_tmem;
+}
+
+// The head's window and the sequence's mask, by bulk copies that count on the CTA's own barrier
+template <typename T> __device__ __forceinline__ uint32_t window_bytes(const Args<T>& a, int wd) { return (uint32_t)(window_floats(wd) + mask_words(a.S)) * 4u; }
+template <typename T> __device__ __forceinline__ void load_window(const Args<T>& a, int b, int h, int wd, float* win, uint64_t* bar) {
+  const int n = window_floats(wd), words = mask_words(a.S);
+  tc::bulk_load(win, a.win + (size_t)h * n, n * 4, bar);
+  tc::bulk_load(win + n, a.bits + (size_t)b * words, words * 4, bar);
+}
+
+// 32 scores in base 2: s scale + bias, with the bias from the window (wp, in steps of `dir`) or one number
+template <int DIR> __device__ __forceinline__ void add_bias(float (&s)[32], float scale, bool empty, float none, bool far_piece, float far_bias, const float* wp) {
+  if (empty) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[j] = none;
+  } else if (far_piece) {
+    const F2 c = f2(scale), f = f2(far_bias);
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), c, f), s[j], s[j + 1]);
+  } else {
+    const F2 c = f2(scale);
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), c, f2(wp[DIR * j], wp[DIR * (j + 1)])), s[j], s[j + 1]);
+  }
 }
 
 // A wait of a whole warp: the same answer in every lane
@@ -125,23 +151,27 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, bool& 
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// 4 warps work on the scores (a row each thread), one issues.  TMEM: two buffers of 64 columns for the scores of blocks in turn (P in
-// the first 32 of them), so that the next block's are there when a block's P is done; O from 128.
+// 4 warps work on the scores (a row each thread), one issues.  TMEM: scores 64 columns (P in the first 32 of them), O from 64: 128
+// columns, so that 4 CTAs share an SM (heads of 128: 2) and one's MMAs run under the others' exponentials.
+//
+// The reference point m of a row's exponentials is the maximum of its first block with an attended key, and stays: P may grow to
+// 2^60 (bf16; its rounding is relative) or, from 2^6, to 2^15 (fp16) without harm.  Where a block's sum shows that a row left that
+// range, the warp works the block again from a new reference, with O and the sum scaled to it.  So no block needs its maximum.
 template <typename T, int HD>
-__global__ void __launch_bounds__(160, 2) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
-  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4;
+__global__ void __launch_bounds__(160, HD == 128 ? 2 : 4) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
+  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = 2, COLS = HD == 128 ? 256 : 128;
+  constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_len;
   char* sq = align1k(smem_raw);
   char* stage = sq + TILE;                                   // [NST][K piece, V piece]
-  const int wd = window(a), pad = ROWS + BLK, qt = (a.S + ROWS - 1) / ROWS;
+  const int wd = window(a), qt = (a.S + ROWS - 1) / ROWS;
   float* win = reinterpret_cast<float*>(stage + NST * 2 * PIECE);
-  uint32_t* bits = reinterpret_cast<uint32_t*>(win + 2 * wd + 1 + 2 * pad);
+  const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
   const int bh = blockIdx.x / qt, b = bh / a.nh, h = bh % a.nh, q0 = (blockIdx.x % qt) * ROWS;
-  const uint32_t tmem = start(&bars, &s_tmem, warp, 4, 256, 4);
+  const uint32_t tmem = start(&bars, &s_tmem, warp, 4, COLS, 4);
   bool aborted = false;
   grid_dep_wait();
   const auto load_block = [&](int i) {
@@ -151,48 +181,37 @@ __global__ void __launch_bounds__(160, 2) fwd_tc(Args<T> a, const __grid_constan
     load_tile<CH>(st + PIECE, &maps.c, bars.full + i % NST, h * HD, i * BLK, b, BLK);
   };
   if (warp == 4 && tc::elect_one()) {
-    tc::mbar_expect_tx(&bars.own, TILE);
+    tc::mbar_expect_tx(&bars.own, TILE + window_bytes(a, wd));
     load_tile<CH>(sq, &maps.a, &bars.own, h * HD, q0, b, ROWS);
+    load_window(a, b, h, wd, win, &bars.own);
     load_block(0);
   }
   __syncwarp();
-  bool empty;
-  const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty), n = (len + BLK - 1) / BLK, words = (a.S + 31) / 32;
-  load_window(a, h, wd, pad, 0.f, win);
-  __syncthreads();
-    if (warp == 4) {
-    warp_wait(&bars.own, 0, aborted, a.status, tc::SITE_FULL, 0);
-    // the scores of block i, behind its copies (rows of V whose keys are masked become zeros: 0 times a NaN is one)
-    const auto scores = [&](int i) {
-      if (!warp_wait(bars.full + i % NST, (i / NST) & 1, aborted, a.status, tc::SITE_FULL, 1 + i)) return;
+  const int seen = __ldg(a.lens + b), len = seen > 0 ? seen : a.S, n = (len + BLK - 1) / BLK;
+  const bool empty = seen == 0;
+  warp_wait(&bars.own, 0, aborted, a.status, tc::SITE_FULL, 0);
+  if (warp == 4) {
+    for (int i = 0; i < n && !aborted; ++i) {
       char* st = stage + (i % NST) * 2 * PIECE;
-      const uint32_t on[2] = {bits[2 * i], 2 * i + 1 < words ? bits[2 * i + 1] : 0u};
-      if ((on[0] & on[1]) != 0xffffffffu) {
-        zero_rows<CH>(st + PIECE, on, BLK, lane);
+      if (!warp_wait(bars.full + i % NST, (i / NST) & 1, aborted, a.status, tc::SITE_FULL, 1 + i)) break;
+      if ((bits[2 * i] & bits[2 * i + 1]) != 0xffffffffu) {  // rows of V whose keys are masked: 0 times a NaN is one
+        zero_rows<CH>(st + PIECE, bits + 2 * i, BLK, lane);
         tc::fence_proxy_async();
         __syncwarp();
       }
+      // the last block's product has read P, which lies where these scores go, and its stage
+      if (i > 0 && !warp_wait(bars.empty + (i - 1) % NST, ((i - 1) / NST) & 1, aborted, a.status, tc::SITE_EMPTY, i)) break;
       tc::tc_fence_after();
       if (tc::elect_one()) {
-        mma_scores<T, HD>(tmem + (i & 1) * BLK, tc::smem_u32(sq), tc::smem_u32(st));
-        tc::umma_commit(bars.scores + (i & 1));
+        mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(st));
+        tc::umma_commit(&bars.scores);
+        if (i + NST - 1 < n) load_block(i + NST - 1);
       }
       __syncwarp();
-    };
-    if (tc::elect_one())
-      for (int i = 1; i < NST - 1 && i < n; ++i) load_block(i);
-    __syncwarp();
-    if (!aborted) scores(0);
-    for (int i = 0; i < n && !aborted; ++i) {
-      // block i - 1 is done with its stage and its buffer of scores: NST - 1 blocks ahead goes into the one, block i + 1 into the other
-      if (i > 0 && !warp_wait(bars.empty + (i - 1) % NST, ((i - 1) / NST) & 1, aborted, a.status, tc::SITE_EMPTY, i)) break;
-      if (i + NST - 1 < n && tc::elect_one()) load_block(i + NST - 1);
-      __syncwarp();
-      if (i + 1 < n) scores(i + 1);
-      if (!warp_wait(bars.done + (i & 1), (i >> 1) & 1, aborted, a.status, tc::SITE_TMEM_EMPTY, i)) break;
+      if (!warp_wait(&bars.done, i & 1, aborted, a.status, tc::SITE_TMEM_EMPTY, i)) break;
       tc::tc_fence_after();
       if (tc::elect_one()) {
-        mma_rows<T, HDP>(tmem + 128, tmem + (i & 1) * BLK, 16, tc::smem_u32(stage + (i % NST) * 2 * PIECE + PIECE), i == 0);
+        mma_rows<T, HDP>(tmem + 64, tmem, 16, tc::smem_u32(st + PIECE), i == 0);
         tc::umma_commit(bars.empty + i % NST);
         if (i + 1 == n) tc::umma_commit(&bars.end);
       }
@@ -201,74 +220,85 @@ __global__ void __launch_bounds__(160, 2) fwd_tc(Args<T> a, const __grid_constan
   } else {
     const uint32_t row_tmem = tmem + ((uint32_t)(warp * 32) << 16);
     const int q = q0 + warp * 32 + lane;
-    const float sl2 = a.scale_log2, up = std::is_same<T, __half>::value ? 6.f : 0.f;
+    const float up = FP16 ? 6.f : 0.f, limit = FP16 ? 32768.f : 1.1529215e18f;
     const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
     const uint32_t drop0 = ((uint32_t)bh * a.S + q) * (uint32_t)a.S;
     float m = -INFINITY, l = 0.f;
     for (int i = 0; i < n; ++i) {
       const int k0 = i * BLK;
-      const uint32_t buf = row_tmem + (i & 1) * BLK;
-      if (!warp_wait(bars.scores + (i & 1), (i >> 1) & 1, aborted, a.status, tc::SITE_TMEM_FULL, i)) break;
+      if (!warp_wait(&bars.scores, i & 1, aborted, a.status, tc::SITE_TMEM_FULL, i)) break;
       tc::tc_fence_after();
-      float s[2][32];
-      tmem_ld2x32(buf, buf + 32, s[0], s[1]);
-      const int dlo = k0 - (q0 + ROWS - 1), dhi = k0 + BLK - 1 - q0;
-      float mx = m;
-      if (empty) {
+      const int dlo = k0 - (q0 + warp * 32 + 31), dhi = k0 + BLK - 1 - (q0 + warp * 32);
+      const bool far_piece = dhi <= -wd || dlo >= wd;
+      const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+      const float* wp = win + (k0 - q) + wd + PAD;
+      const uint32_t on[2] = {bits[2 * i], bits[2 * i + 1]};
+      float s[2][32], sum;
+      const auto scores = [&]() {
+        tmem_ld2x32(row_tmem, row_tmem + 32, s[0], s[1]);
 #pragma unroll
-        for (int j = 0; j < BLK; ++j) s[j >> 5][j & 31] = 0.f;
-      } else if (dhi <= -wd || dlo >= wd) {
-        const float bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * pad];
+        for (int c = 0; c < 2; ++c) {
+          add_bias<1>(s[c], a.scale_log2, empty, 0.f, far_piece, far_bias, wp + 32 * c);
+          if (on[c] != 0xffffffffu) {
 #pragma unroll
-        for (int j = 0; j < BLK; ++j) s[j >> 5][j & 31] = fmaf(s[j >> 5][j & 31], sl2, bias);
-      } else {
-        const float* wp = win + (k0 - q) + wd + pad;
+            for (int j = 0; j < 32; ++j)
+              if (!(on[c] >> j & 1u)) s[c][j] = -INFINITY;
+          }
+        }
+      };
+      const auto top = [&]() {
+        float t[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
-        for (int j = 0; j < BLK; ++j) s[j >> 5][j & 31] = fmaf(s[j >> 5][j & 31], sl2, wp[j]);
+        for (int j = 4; j < BLK; ++j) t[j & 3] = fmaxf(t[j & 3], s[j >> 5][j & 31]);
+        return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+      };
+      const auto exponentials = [&]() {
+        const F2 base = f2(m == -INFINITY ? 0.f : up - m);
+        F2 l2[2] = {f2(0.f), f2(0.f)};
+#pragma unroll
+        for (int j = 0; j < BLK; j += 2) {
+          float x, y;
+          f2_get(f2(s[j >> 5][j & 31], s[j >> 5][(j & 31) + 1]) + base, x, y);
+          x = ex2(x);
+          y = ex2(y);
+          s[j >> 5][j & 31] = x;
+          s[j >> 5][(j & 31) + 1] = y;
+          l2[(j >> 1) & 1] = l2[(j >> 1) & 1] + f2(x, y);
+        }
+        float x, y;
+        f2_get(l2[0] + l2[1], x, y);
+        sum = x + y;
+      };
+      scores();
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {
+        const float t = top();
+        if (m == -INFINITY) m = t;
       }
-      const uint32_t on[2] = {bits[2 * i], 2 * i + 1 < words ? bits[2 * i + 1] : 0u};
-      if ((on[0] & on[1]) != 0xffffffffu) {
-#pragma unroll
-        for (int j = 0; j < BLK; ++j)
-          if (!(on[j >> 5] >> (j & 31) & 1u)) s[j >> 5][j & 31] = -INFINITY;
-      }
-#pragma unroll
-      for (int j = 0; j < BLK; ++j) mx = fmaxf(mx, s[j >> 5][j & 31]);
-      // The reference point follows the maximum only where it is left far behind: P up to 2^8 (fp16: 2^14) is as good as P up to 1,
-      // and O and the sum are scaled again a few times a row instead of once a block
-      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
-        const float f = m == -INFINITY ? 0.f : ex2(m - mx);
-        if (i > 0) {
-          // O is at rest behind the product of block i - 1 (the whole warp comes here)
-          if (!warp_wait(bars.empty + (i - 1) % NST, ((i - 1) / NST) & 1, aborted, a.status, tc::SITE_TMEM_FULL, i)) break;
-          tc::tc_fence_after();
+      exponentials();
+      if (__any_sync(0xffffffffu, sum > limit)) {
+        scores();
+        const float t = fmaxf(m, top()), f = m == -INFINITY ? 0.f : ex2(m - t);
+        if (i > 0) {                                         // O is at rest: these scores were issued behind the last product's commit
 #pragma unroll 1
           for (int c = 0; c < HDP; c += 16) {
-            uint32_t r[16];
-            float v[16];
-            uint32_t lo[8], hi[8];
-            tc::tmem_issue8(row_tmem + 128 + c, lo);
-            tc::tmem_issue8(row_tmem + 128 + c + 8, hi);
+            uint32_t r[16], lo[8], hi[8];
+            tc::tmem_issue8(row_tmem + 64 + c, lo);
+            tc::tmem_issue8(row_tmem + 64 + c + 8, hi);
             tc::tmem_wait8(lo);
             tc::tmem_wait8(hi);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { v[j] = __uint_as_float(lo[j]); v[8 + j] = __uint_as_float(hi[j]); }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(v[j] * f);
-            tc::tmem_st16(row_tmem + 128 + c, r);
+            for (int j = 0; j < 8; ++j) {
+              r[j] = __float_as_uint(__uint_as_float(lo[j]) * f);
+              r[8 + j] = __float_as_uint(__uint_as_float(hi[j]) * f);
+            }
+            tc::tmem_st16(row_tmem + 64 + c, r);
           }
         }
         l *= f;
-        m = mx;
+        m = t;
+        exponentials();
       }
-      const float base = m == -INFINITY ? 0.f : m - up;
-      float l2[2] = {};
-#pragma unroll
-      for (int j = 0; j < BLK; ++j) {
-        s[j >> 5][j & 31] = ex2(s[j >> 5][j & 31] - base);
-        l2[j & 1] += s[j >> 5][j & 31];
-      }
-      l += l2[0] + l2[1];
+      l += sum;
       if (a.p > 0.f) {
 #pragma unroll
         for (int j = 0; j < BLK; ++j)
@@ -279,12 +309,12 @@ __global__ void __launch_bounds__(160, 2) fwd_tc(Args<T> a, const __grid_constan
         uint32_t r[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) r[j] = pack16<T>(s[c][2 * j], s[c][2 * j + 1]);
-        tc::tmem_st16(buf + 16 * c, r);
+        tc::tmem_st16(row_tmem + 16 * c, r);
       }
       tc::tmem_wait_st();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(bars.done + (i & 1));
+      if (lane == 0) tc::mbar_arrive(&bars.done);
     }
     if (warp_wait(&bars.end, 0, aborted, a.status, tc::SITE_TMEM_FULL, n)) {
       tc::tc_fence_after();
@@ -294,16 +324,16 @@ __global__ void __launch_bounds__(160, 2) fwd_tc(Args<T> a, const __grid_constan
 #pragma unroll
       for (int c = 0; c < HD; c += 32) {
         float v[32];
-        tc::tmem_ld32(row_tmem + 128 + c, v);
+        tc::tmem_ld32(row_tmem + 64 + c, v);
         store_rows<T>(mine, v, f, out + c, (long long)a.nh * HD, a.S - q0 - warp * 32, lane);
       }
-      if (a.lse != nullptr) a.lse[(size_t)bh * a.Sp + q] = q < a.S ? (m - up) + lg2(l) : INFINITY;
+      a.lse[(size_t)bh * a.Sp + q] = q < a.S ? (m - up) + lg2(l) : INFINITY;
     }
   }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  if (warp == 4) tc::tmem_dealloc(tmem, 256);
+  if (warp == 4) tc::tmem_dealloc(tmem, COLS);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: queries
@@ -316,14 +346,14 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_len;
   __shared__ float s_sum[2][ROWS];
   char* sq = align1k(smem_raw);
   char* sdo = sq + TILE;
-  char* stage = sdo + TILE;                                  // [NST][K piece, V piece]
-  const int wd = window(a), pad = ROWS + BLK, qt = (a.S + ROWS - 1) / ROWS;
+  char* stage = sdo + TILE;                                  // [NST][K piece, V piece]; ctx in the last until delta is made
+  char* sctx = stage + (NST - 1) * 2 * PIECE;
+  const int wd = window(a), qt = (a.S + ROWS - 1) / ROWS;
   float* win = reinterpret_cast<float*>(stage + NST * 2 * PIECE);
-  uint32_t* bits = reinterpret_cast<uint32_t*>(win + 2 * wd + 1 + 2 * pad);
+  const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
   const int bh = blockIdx.x / qt, b = bh / a.nh, h = bh % a.nh, q0 = (blockIdx.x % qt) * ROWS;
   const uint32_t tmem = start(&bars, &s_tmem, warp, 8, COLS, 8);
@@ -336,43 +366,27 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
     load_tile<CH>(st + PIECE, &maps.c, bars.full + i % NST, h * HD, i * BLK, b, BLK);
   };
   if (warp == 8 && tc::elect_one()) {
-    tc::mbar_expect_tx(&bars.own, 2 * TILE);
+    tc::mbar_expect_tx(&bars.own, 3 * TILE + window_bytes(a, wd));
     load_tile<CH>(sq, &maps.a, &bars.own, h * HD, q0, b, ROWS);
     load_tile<CH>(sdo, &maps.d, &bars.own, h * HD, q0, b, ROWS);
+    load_tile<CH>(sctx, &maps.e, &bars.own, h * HD, q0, b, ROWS);
+    load_window(a, b, h, wd, win, &bars.own);
     load_block(0);
   }
   __syncwarp();
   const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, q = q0 + row;
-  const size_t H = (size_t)a.nh * HD, at = ((size_t)b * a.S + q) * H + h * HD;
-  if (warp < 8) {                                            // delta = dctx ctx: half a row each
-    float d = 0.f;
-    if (q < a.S) {
-#pragma unroll
-      for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 8) {
-        float x[8], y[8];
-        load8(a.dctx + at + c, x);
-        load8(a.ctx + at + c, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d += x[j] * y[j];
-      }
-    }
-    s_sum[half][row] = d;
-  }
-  bool empty;
-  const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty), n = (len + BLK - 1) / BLK, words = (a.S + 31) / 32;
-  load_window(a, h, wd, pad, a.grad_log2, win);
-  __syncthreads();
+  const int seen = __ldg(a.lens + b), len = seen > 0 ? seen : a.S, n = (len + BLK - 1) / BLK;
+  const bool empty = seen == 0;
+  warp_wait(&bars.own, 0, aborted, a.status, tc::SITE_FULL, 0);
   if (warp == 8) {
-    warp_wait(&bars.own, 0, aborted, a.status, tc::SITE_FULL, 0);
     if (tc::elect_one())
       for (int i = 1; i < NST - 1 && i < n; ++i) load_block(i);
     __syncwarp();
     for (int i = 0; i < n && !aborted; ++i) {
       char* st = stage + (i % NST) * 2 * PIECE;
       if (!warp_wait(bars.full + i % NST, (i / NST) & 1, aborted, a.status, tc::SITE_FULL, 1 + i)) break;
-      const uint32_t on[2] = {bits[2 * i], 2 * i + 1 < words ? bits[2 * i + 1] : 0u};
-      if ((on[0] & on[1]) != 0xffffffffu) {                  // 0 times a masked key's NaN is one
-        zero_rows<CH>(st, on, BLK, lane);
+      if ((bits[2 * i] & bits[2 * i + 1]) != 0xffffffffu) {                  // 0 times a masked key's NaN is one
+        zero_rows<CH>(st, bits + 2 * i, BLK, lane);
         tc::fence_proxy_async();
         __syncwarp();
       }
@@ -380,15 +394,15 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       if (tc::elect_one()) {
         mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(st));
         mma_scores<T, HD>(tmem + 64, tc::smem_u32(sdo), tc::smem_u32(st + PIECE));
-        tc::umma_commit(bars.scores);
+        tc::umma_commit(&bars.scores);
       }
       __syncwarp();
       if (i + NST - 1 < n) {
-        if (i > 0 && !warp_wait(bars.empty + (i - 1) % NST, ((i - 1) / NST) & 1, aborted, a.status, tc::SITE_EMPTY, i)) break;
+        if (!warp_wait(i > 0 ? bars.empty + (i - 1) % NST : &bars.read, i > 0 ? ((i - 1) / NST) & 1 : 0, aborted, a.status, tc::SITE_EMPTY, i)) break;
         if (tc::elect_one()) load_block(i + NST - 1);
         __syncwarp();
       }
-      if (!warp_wait(bars.done, i & 1, aborted, a.status, tc::SITE_TMEM_EMPTY, i)) break;
+      if (!warp_wait(&bars.done, i & 1, aborted, a.status, tc::SITE_TMEM_EMPTY, i)) break;
       tc::tc_fence_after();
       if (tc::elect_one()) {
         mma_rows<T, HDP>(tmem + 128, tmem + 128 + HDP, 16, tc::smem_u32(st), i == 0);
@@ -399,36 +413,40 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
     }
   } else {
     const uint32_t row_tmem = tmem + ((uint32_t)(quarter * 32) << 16);
-    const float sl2 = a.scale_log2, kept = 1.f / (1.f - a.p);
+    // delta = dctx ctx: half a row each
+    float d = 0.f;
+#pragma unroll
+    for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
+      float x[8], y[8];
+      const int at = (c >> 3) * ROWS * 128 + row * 128 + ((c ^ row) & 7) * 16;
+      load8(reinterpret_cast<const T*>(sdo + at), x);
+      load8(reinterpret_cast<const T*>(sctx + at), y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d += x[j] * y[j];
+    }
+    s_sum[half][row] = d;
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&bars.read);
+    const float lse = q < a.S ? __ldg(a.lse + (size_t)bh * a.Sp + q) - a.grad_log2 : INFINITY;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float delta = s_sum[0][row] + s_sum[1][row];
+    const float kept = 1.f / (1.f - a.p);
     const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
     const uint32_t drop0 = ((uint32_t)bh * a.S + q) * (uint32_t)a.S + half * 32;
-    const float delta = s_sum[0][row] + s_sum[1][row];
-    const float lse = q < a.S ? __ldg(a.lse + (size_t)bh * a.Sp + q) : INFINITY;
-    float sum[2] = {};
+    F2 sum = f2(0.f);
     for (int i = 0; i < n; ++i) {
       const int k0 = i * BLK + half * 32;                    // of this warp's columns
-      if (!warp_wait(bars.scores, i & 1, aborted, a.status, tc::SITE_TMEM_FULL, i)) break;
+      if (!warp_wait(&bars.scores, i & 1, aborted, a.status, tc::SITE_TMEM_FULL, i)) break;
       tc::tc_fence_after();
       float s[32], dp[32];
       tmem_ld2x32(row_tmem + 32 * half, row_tmem + 64 + 32 * half, s, dp);
       const int dlo = k0 - (q0 + quarter * 32 + 31), dhi = k0 + 31 - (q0 + quarter * 32);
-      if (empty) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = a.grad_log2;
-      } else if (dhi <= -wd || dlo >= wd) {
-        const float bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * pad];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = fmaf(s[j], sl2, bias);
-      } else {
-        const float* wp = win + (k0 - q) + wd + pad;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = fmaf(s[j], sl2, wp[j]);
-      }
+      add_bias<1>(s, a.scale_log2, empty, 0.f, dhi <= -wd || dlo >= wd, dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD], win + (k0 - q) + wd + PAD);
       if (a.p > 0.f) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) dp[j] = keep(seed, a.stream, drop0 + i * BLK + j, a.p) ? dp[j] * kept : 0.f;
       }
-      const uint32_t on = (k0 >> 5) < words ? bits[k0 >> 5] : 0u;
+      const uint32_t on = bits[k0 >> 5];
       if (on != 0xffffffffu) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -438,25 +456,36 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
           }
       }
       uint32_t r[16];
+      const F2 nl = f2(-lse), nd = f2(-delta);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        s[j] = ex2(s[j] - lse);
-        sum[j & 1] += s[j] * dp[j];
-        s[j] = empty ? 0.f : s[j] * (dp[j] - delta);
+      for (int j = 0; j < 32; j += 2) {
+        float x, y;
+        f2_get(f2(s[j], s[j + 1]) + nl, x, y);
+        const F2 pr = f2(ex2(x), ex2(y)), g = f2(dp[j], dp[j + 1]);
+        sum = f2_fma(pr, g, sum);
+        f2_get(pr * (g + nd), x, y);
+        r[j / 2] = pack16<T>(x, y);
       }
+      if (empty) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) r[j] = pack16<T>(s[2 * j], s[2 * j + 1]);
-      tc::tmem_st16(row_tmem + 128 + HDP + 16 * half, r);      // the last block's product has read it: its commit lies before these scores'
+        for (int j = 0; j < 16; ++j) r[j] = 0u;
+      }
+      tc::tmem_st16(row_tmem + 128 + HDP + 16 * half, r);    // the last block's product has read it: its commit lies before these scores'
       tc::tmem_wait_st();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(bars.done);
+      if (lane == 0) tc::mbar_arrive(&bars.done);
     }
     // delta for the keys' pass: the sum that was made on the way, free of ctx's rounding
+    float x, y;
+    f2_get(sum, x, y);
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    s_sum[half][row] = sum[0] + sum[1];
+    s_sum[half][row] = x + y;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (half == 0) a.delta[(size_t)bh * a.Sp + q] = q < a.S ? (s_sum[0][row] + s_sum[1][row]) * a.grad_inv : 0.f;
+    if (half == 0) {
+      a.delta[(size_t)bh * a.Sp + q] = q < a.S ? (s_sum[0][row] + s_sum[1][row]) * a.grad_inv : 0.f;
+      a.lse_up[(size_t)bh * a.Sp + q] = lse;
+    }
     if (warp_wait(&bars.end, 0, aborted, a.status, tc::SITE_TMEM_FULL, n)) {
       tc::tc_fence_after();
       const float f = a.scale * a.grad_inv;
@@ -492,15 +521,14 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_len;
   __shared__ float s_diag[8][64];
   char* sk = align1k(smem_raw);
   char* sv = sk + TILE;
   char* stage = sv + TILE;
-  const int wd = window(a), pad = ROWS + BLK, kt = (a.S + ROWS - 1) / ROWS, nwin = 2 * wd + 1, words = (a.S + 31) / 32;
+  const int wd = window(a), kt = (a.S + ROWS - 1) / ROWS, nwin = 2 * wd + 1;
   float* win = reinterpret_cast<float*>(stage + NST * STAGE_UP);
-  float* sums = win + nwin + 2 * pad;                        // [8][nwin]
-  uint32_t* bits = reinterpret_cast<uint32_t*>(sums + 8 * nwin);
+  const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
+  float* sums = win + window_floats(wd) + mask_words(a.S);   // [8][nwin]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
   const int bh = blockIdx.x / kt, b = bh / a.nh, h = bh % a.nh, ktile = blockIdx.x % kt, k0 = ktile * ROWS;
   const uint32_t tmem = start(&bars, &s_tmem, warp, 8, COLS, 8);
@@ -512,32 +540,28 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     tc::mbar_expect_tx(bar, STAGE);
     load_tile<CH>(st, &maps.a, bar, h * HD, i * BLK, b, BLK);
     load_tile<CH>(st + PIECE, &maps.d, bar, h * HD, i * BLK, b, BLK);
-    tc::bulk_load(st + 2 * PIECE, a.lse + (size_t)bh * a.Sp + i * BLK, BLK * 4, bar);
+    tc::bulk_load(st + 2 * PIECE, a.lse_up + (size_t)bh * a.Sp + i * BLK, BLK * 4, bar);
     tc::bulk_load(st + 2 * PIECE + BLK * 4, a.delta + (size_t)bh * a.Sp + i * BLK, BLK * 4, bar);
   };
   if (warp == 8 && tc::elect_one()) {
-    tc::mbar_expect_tx(&bars.own, 2 * TILE);
+    tc::mbar_expect_tx(&bars.own, 2 * TILE + window_bytes(a, wd));
+    load_window(a, b, h, wd, win, &bars.own);
     load_tile<CH>(sk, &maps.b, &bars.own, h * HD, k0, b, ROWS);
     load_tile<CH>(sv, &maps.c, &bars.own, h * HD, k0, b, ROWS);
     load_block(0);
   }
   __syncwarp();
-  bool empty;
-  const int len = attended(a.mask + (size_t)b * a.S, a.S, bits, &s_len, empty);
+  const int seen = __ldg(a.lens + b), len = seen > 0 ? seen : a.S;
+  const bool empty = seen == 0;
   const int n = k0 < len ? (a.S + BLK - 1) / BLK : 0;        // a tile without an attended key has no gradient
-  load_window(a, h, wd, pad, a.grad_log2, win);
   for (int i = threadIdx.x; i < 8 * nwin; i += blockDim.x) sums[i] = 0.f;
   __syncthreads();
+  // without a block the copies are waited for all the same: rows are staged where they land
+  warp_wait(&bars.own, 0, aborted, a.status, tc::SITE_FULL, 0);
   if (warp == 8) {
-    warp_wait(&bars.own, 0, aborted, a.status, tc::SITE_FULL, 0);
     if (n == 0) warp_wait(bars.full, 0, aborted, a.status, tc::SITE_FULL, 1);            // its copies are its own to wait for
-    uint32_t on[4], all = 0xffffffffu;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      on[w] = (k0 >> 5) + w < words ? bits[(k0 >> 5) + w] : 0u;
-      all &= on[w];
-    }
-    if (n > 0 && all != 0xffffffffu) {
+    const uint32_t* on = bits + (k0 >> 5);
+    if (n > 0 && (on[0] & on[1] & on[2] & on[3]) != 0xffffffffu) {
       zero_rows<CH>(sk, on, ROWS, lane);
       zero_rows<CH>(sv, on, ROWS, lane);
       tc::fence_proxy_async();
@@ -555,11 +579,11 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       if (tc::elect_one()) {
         mma_scores<T, HD>(tmem, tc::smem_u32(sk), tc::smem_u32(st));
         mma_scores<T, HD>(tmem + 64, tc::smem_u32(sv), tc::smem_u32(st + PIECE));
-        tc::umma_commit(bars.scores);
+        tc::umma_commit(&bars.scores);
         if (i + NST - 1 < n) load_block(i + NST - 1);
       }
       __syncwarp();
-      if (!warp_wait(bars.done, i & 1, aborted, a.status, tc::SITE_TMEM_EMPTY, i)) break;
+      if (!warp_wait(&bars.done, i & 1, aborted, a.status, tc::SITE_TMEM_EMPTY, i)) break;
       tc::tc_fence_after();
       if (tc::elect_one()) {
         mma_rows<T, HDP>(tmem + 128, tmem, 32, tc::smem_u32(st + PIECE), i == 0);
@@ -572,15 +596,15 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   } else {
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, k = k0 + row;
     const uint32_t row_tmem = tmem + ((uint32_t)(quarter * 32) << 16);
-    const float sl2 = a.scale_log2, kept = 1.f / (1.f - a.p);
+    const float kept = 1.f / (1.f - a.p);
     const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
-    const bool on = k < a.S && (bits[k >> 5] >> (k & 31) & 1u);
+    const bool on = bits[k >> 5] >> (k & 31) & 1u;
     const float not_first = lane == 0 ? 0.f : 1.f;
     float far[2] = {};
     float* mine = sums + warp * nwin;
     for (int i = 0; i < n; ++i) {
       const int q0 = i * BLK + half * 32;                    // of this warp's columns
-      if (!warp_wait(bars.scores, i & 1, aborted, a.status, tc::SITE_TMEM_FULL, i)) break;
+      if (!warp_wait(&bars.scores, i & 1, aborted, a.status, tc::SITE_TMEM_FULL, i)) break;
       tc::tc_fence_after();
       float s[32], dp[32];
       tmem_ld2x32(row_tmem + 32 * half, row_tmem + 64 + 32 * half, s, dp);
@@ -588,30 +612,30 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       const float4* del = lse + BLK / 4;
       const int dlo = k0 + quarter * 32 - (q0 + 31), dhi = k0 + quarter * 32 + 31 - q0;
       const bool far_piece = dhi <= -wd || dlo >= wd;
-      if (empty) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = a.grad_log2;
-      } else if (far_piece) {
-        const float bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * pad];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = fmaf(s[j], sl2, bias);
-      } else {
-        const float* wp = win + (k - q0) + wd + pad;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j] = fmaf(s[j], sl2, wp[-j]);
-      }
+      add_bias<-1>(s, a.scale_log2, empty, 0.f, far_piece, dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD], win + (k - q0) + wd + PAD);
       uint32_t r[16];
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {
         const float4 L = lse[j / 4], D = del[j / 4];
         const float ls[4] = {L.x, L.y, L.z, L.w}, de[4] = {D.x, D.y, D.z, D.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float pr = on ? ex2(s[j + e] - ls[e]) : 0.f;
-          float kf = 1.f;
-          if (a.p > 0.f) kf = keep(seed, a.stream, ((uint32_t)bh * a.S + q0 + j + e) * (uint32_t)a.S + k, a.p) ? kept : 0.f;
-          s[j + e] = pr * kf;
-          dp[j + e] = pr * (__fmul_rn(dp[j + e], kf) - de[e]);
+        for (int e = 0; e < 4; e += 2) {
+          float x, y;
+          f2_get(f2(s[j + e], s[j + e + 1]) + f2(-ls[e], -ls[e + 1]), x, y);
+          x = on ? ex2(x) : 0.f;
+          y = on ? ex2(y) : 0.f;
+          const F2 pr = f2(x, y);
+          F2 g = f2(dp[j + e], dp[j + e + 1]);
+          if (a.p > 0.f) {
+            const uint32_t at = ((uint32_t)bh * a.S + q0 + j + e) * (uint32_t)a.S + k;
+            const F2 kf = f2(keep(seed, a.stream, at, a.p) ? kept : 0.f, keep(seed, a.stream, at + (uint32_t)a.S, a.p) ? kept : 0.f);
+            g = g * kf;
+            f2_get(pr * kf, s[j + e], s[j + e + 1]);
+          } else {
+            s[j + e] = x;
+            s[j + e + 1] = y;
+          }
+          f2_get(pr * (g + f2(-de[e], -de[e + 1])), dp[j + e], dp[j + e + 1]);
         }
       }
       if (empty) {
@@ -627,7 +651,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       tc::tmem_wait_st();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(bars.done);
+      if (lane == 0) tc::mbar_arrive(&bars.done);
       if (far_piece) {
         float v = 0.f;
 #pragma unroll
@@ -656,8 +680,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     }
     const int rows = a.S - k0 - quarter * 32;
     T* outs[2] = {a.dv + ((size_t)b * a.S + k0 + quarter * 32) * a.lddv + h * HD, a.dk + ((size_t)b * a.S + k0 + quarter * 32) * a.lddk + h * HD};
-    // without a block the tiles' copies are waited for all the same: the rows are staged where they land
-    if (warp_wait(n == 0 ? &bars.own : &bars.end, 0, aborted, a.status, tc::SITE_TMEM_FULL, n)) {
+    if (n == 0 ? !aborted : warp_wait(&bars.end, 0, aborted, a.status, tc::SITE_TMEM_FULL, n)) {
       tc::tc_fence_after();
 #pragma unroll
       for (int o = 0; o < 2; ++o)
@@ -698,10 +721,9 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
 template <typename K> int allow_smem(K kernel, int bytes) {
   return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
-inline int up16b(int bytes) { return (bytes + 15) / 16 * 16; }
 
 template <typename T, int HD> int run_fwd_tc(const Args<T>& a, cudaStream_t st) {
-  constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = HD == 128 ? 2 : 4;
+  constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = 2;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps m;
   const uint64_t H = (uint64_t)a.nh * HD;
@@ -709,8 +731,8 @@ template <typename T, int HD> int run_fwd_tc(const Args<T>& a, cudaStream_t st) 
   if (!rc) rc = tc::make_tmap_rows(&m.b, a.k, a.b, a.S, H, a.ldk, BLK, bf);
   if (!rc) rc = tc::make_tmap_rows(&m.c, a.v, a.b, a.S, H, a.ldv, BLK, bf);
   if (rc) return rc;
-  m.d = m.c;
-  const int smem = 1024 + (ROWS + NST * 2 * BLK) * 128 * CH + up16b((2 * window(a) + 1 + 2 * (ROWS + BLK)) * 4 + (a.S + 31) / 32 * 4);
+  m.d = m.e = m.c;
+  const int smem = 1024 + (ROWS + NST * 2 * BLK) * 128 * CH + (window_floats(window(a)) + mask_words(a.S)) * 4;
   rc = allow_smem(fwd_tc<T, HD>, smem);
   if (rc) return rc;
   return (int)launch_pdl(fwd_tc<T, HD>, dim3((unsigned)((a.S + ROWS - 1) / ROWS * a.nh * a.b)), dim3(160), smem, st, a, m);
@@ -725,14 +747,16 @@ template <typename T, int HD> int run_bwd_tc(const Args<T>& a, cudaStream_t st) 
   if (!rc) rc = tc::make_tmap_rows(&q.b, a.k, a.b, a.S, H, a.ldk, BLK, bf);
   if (!rc) rc = tc::make_tmap_rows(&q.c, a.v, a.b, a.S, H, a.ldv, BLK, bf);
   if (!rc) rc = tc::make_tmap_rows(&q.d, a.dctx, a.b, a.S, H, H, ROWS, bf);
+  if (!rc) rc = tc::make_tmap_rows(&q.e, a.ctx, a.b, a.S, H, H, ROWS, bf);
   if (!rc) rc = tc::make_tmap_rows(&kv.a, a.q, a.b, a.S, H, a.ldq, BLK, bf);
   if (!rc) rc = tc::make_tmap_rows(&kv.b, a.k, a.b, a.S, H, a.ldk, ROWS, bf);
   if (!rc) rc = tc::make_tmap_rows(&kv.c, a.v, a.b, a.S, H, a.ldv, ROWS, bf);
   if (!rc) rc = tc::make_tmap_rows(&kv.d, a.dctx, a.b, a.S, H, H, BLK, bf);
   if (rc) return rc;
-  const int nwin = 2 * window(a) + 1, tail = (nwin + 2 * (ROWS + BLK)) * 4 + (a.S + 31) / 32 * 4;
-  const int smem_q = 1024 + 2 * ROWS * 128 * CH + NST * 2 * PIECE + up16b(tail);
-  const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST * STAGE_UP + up16b(tail + 8 * nwin * 4);
+  kv.e = kv.d;
+  const int nwin = 2 * window(a) + 1, tail = (window_floats(window(a)) + mask_words(a.S)) * 4;
+  const int smem_q = 1024 + 2 * ROWS * 128 * CH + NST * 2 * PIECE + tail;
+  const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST * STAGE_UP + tail + 8 * nwin * 4;
   rc = allow_smem(bwd_q_tc<T, HD>, smem_q);
   if (!rc) rc = allow_smem(bwd_kv_tc<T, HD>, smem_kv);
   const dim3 grid((unsigned)((a.S + ROWS - 1) / ROWS * a.nh * a.b));

@@ -409,12 +409,12 @@ def bias_gelu_bwd(da, x, bias, dbias, dx_out):
 # Entry points whose argument types are set, so that they take Python's numbers as they are (wrapping each costs 0.25 us, and the
 # kernels of a small call take 5): p = address, l = long long, i = int, u = unsigned, f = float.  The stream is the last argument.
 _KINDS = {"p": _VP, "l": _LL, "i": _I, "u": _U, "f": _F}
-_RELATIVE_INPUTS = "plplplpppiiiiiifpup"
+_RELATIVE_INPUTS = "plplpliiiiiipppfpup"
 _TYPES = {
     "rb_qk_norm_rotary_fwd": "iplppppplliiiifp",
     "rb_qk_norm_rotary_bwd": "iplplpppppplpp" + "liiiifp",
-    "rb_relative_fwd": "i" + _RELATIVE_INPUTS + "ppp",
-    "rb_relative_bwd": "ip" + _RELATIVE_INPUTS + "pppp" + "plplpl" + "pp",
+    "rb_relative_fwd": "i" + _RELATIVE_INPUTS + "pppppp",
+    "rb_relative_bwd": "ip" + _RELATIVE_INPUTS + "ppppp" + "plplpl" + "pp",
     "rb_gelu8_fwd": "ippppplip",
     "rb_gelu8_bwd": "ippppppplip",
 }
@@ -461,23 +461,27 @@ def relative_tiles(S: int) -> int:
     return lib().rb_relative_tiles(_I(S))
 
 
-def _relative_inputs(at, q, k, v, mask, table, buckets, nh, p, rng, stream):
+def relative_window_floats(far: int, S: int) -> int:
+    return lib().rb_relative_window_floats(_I(far), _I(S))
+
+
+def _relative_inputs(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):
     b, S = mask.shape
-    return (at[0], _ld(q), at[1], _ld(k), at[2], _ld(v), mask.data_ptr(), table.data_ptr(), buckets.data_ptr(), (buckets.shape[0] - 1) // 2,
-            table.shape[0], b, S, nh, q.shape[1] // nh, p, rng.dev.data_ptr() if p > 0 else None, stream,
+    return (at[0], _ld(q), at[1], _ld(k), at[2], _ld(v), (buckets.shape[0] - 1) // 2, table.shape[0], b, S, nh, q.shape[1] // nh,
+            ws.win.data_ptr(), ws.bits.data_ptr(), ws.lens.data_ptr(), p, rng.dev.data_ptr() if p > 0 else None, stream,
             workspace(q.device).status.data_ptr())
 
 
 def relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):
-    _call_typed("rb_relative_fwd", q.device, DT[q.dtype], *_relative_inputs(at[1:4], q, k, v, mask, table, buckets, nh, p, rng, stream), at[0],
-                None if ws is None else ws.lse.data_ptr(), launches=1 if mask.shape[0] else 0)
+    _call_typed("rb_relative_fwd", q.device, DT[q.dtype], *_relative_inputs(at[1:4], q, k, v, mask, table, buckets, nh, p, rng, stream, ws),
+                mask.data_ptr(), table.data_ptr(), buckets.data_ptr(), at[0], ws.lse.data_ptr(), launches=2 if mask.shape[0] else 0)
 
 
 def relative_attention_bwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws, dq, dk, dv):
     dq_, dk_, dv_, dtable, _, _, _, dctx, ctx, _ = at
-    _call_typed("rb_relative_bwd", q.device, DT[q.dtype], dctx, *_relative_inputs(at[4:7], q, k, v, mask, table, buckets, nh, p, rng, stream), ctx,
-                ws.lse.data_ptr(), ws.delta.data_ptr(), ws.dwin.data_ptr(), dq_, _ld(dq), dk_, _ld(dk), dv_, _ld(dv), dtable,
-                launches=3 if mask.shape[0] else 1)
+    _call_typed("rb_relative_bwd", q.device, DT[q.dtype], dctx,
+                *_relative_inputs(at[4:7], q, k, v, mask, table, buckets, nh, p, rng, stream, ws), buckets.data_ptr(), ctx, ws.lse.data_ptr(),
+                ws.stats.data_ptr(), ws.dwin.data_ptr(), dq_, _ld(dq), dk_, _ld(dk), dv_, _ld(dv), dtable, launches=3 if mask.shape[0] else 1)
 
 
 def gelu8_splits(T: int, F: int) -> int:

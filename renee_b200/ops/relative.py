@@ -212,25 +212,34 @@ def relative_buckets(num_buckets: int, max_distance: int, device=None) -> torch.
 
 
 class RelativeWorkspace:
-    """What :func:`relative_attention_fwd` leaves for its backward pass (``lse``) and the scratch of that pass."""
+    """What :func:`relative_attention_fwd` leaves for its backward pass (``lse``, the biases by distance ``win``, the masks as
+    ``bits`` and ``lens``) and the scratch of that pass (``stats``, ``dwin``)."""
 
-    def __init__(self, lse: torch.Tensor, delta: torch.Tensor, dwin: torch.Tensor):
-        self.lse, self.delta, self.dwin = lse, delta, dwin
-        self.sizes = (lse.device, lse.numel(), delta.numel(), dwin.numel())
+    def __init__(self, lse, win, bits, lens, stats, dwin):
+        self.lse, self.win, self.bits, self.lens, self.stats, self.dwin = lse, win, bits, lens, stats, dwin
+        self.sizes = (lse.device, *(t.numel() for t in (lse, win, bits, lens, stats, dwin)))
+
+
+def _relative_sizes(b: int, S: int, nh: int, far: int) -> tuple:
+    """Values of the workspace's buffers; the statistics and the bits of a sequence take whole tiles of 128 tokens."""
+    cu, up = _cuda(), -(-S // 128) * 128
+    return (b * nh * up, nh * cu.relative_window_floats(far, S), b * up // 32, b, 2 * b * nh * up,
+            b * cu.relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
 
 
 def relative_attention_workspace(b: int, S: int, nh: int, hd: int, max_distance: int, dtype, device, scratch=None) -> RelativeWorkspace:
-    """Buffers for ``b`` sequences of ``S`` tokens.  Each forward call whose backward pass is still to come needs an ``lse`` of its
-    own; ``scratch`` (another workspace of the same sizes) lends its other buffers, which live within one backward call."""
+    """Buffers for up to ``b`` sequences of ``S`` tokens.  Each forward call whose backward pass is still to come needs one of its
+    own; ``scratch`` (another workspace of the same sizes) lends the buffers that live within one backward call."""
     if torch.device(device).type == "cpu":
-        return RelativeWorkspace(*[torch.empty(0)] * 3)
-    e = lambda n, name: guard.empty(max(n, 1), dtype=torch.float32, device=device, name=f"relative_attention.{name}")
-    stats = b * nh * (-(-S // 128) * 128)         # the statistics of a sequence take whole tiles of 128 rows
-    lse = e(stats, "lse")
-    if scratch is not None:
-        return RelativeWorkspace(lse, scratch.delta, scratch.dwin)
-    tiles = _cuda().relative_tiles(S)
-    return RelativeWorkspace(lse, e(stats, "delta"), e(b * tiles * nh * (2 * min(max_distance, S - 1) + 1), "dwin"))
+        return RelativeWorkspace(*[torch.empty(0)] * 6)
+    _refuse(hd not in HEAD_DIMS or dtype not in (torch.bfloat16, torch.float16), f"no kernels for heads of {hd} in {dtype}")
+    _refuse(b < 0 or S < 1 or nh < 1 or not 0 <= max_distance <= MAX_DISTANCE, f"no workspace for {b} x {S} tokens, {nh} heads, distance {max_distance}")
+    made = []
+    for name, n, dtype in zip(("lse", "win", "bits", "lens", "stats", "dwin"), _relative_sizes(b, S, nh, max_distance),
+                              (torch.float32, torch.float32, torch.int32, torch.int32, torch.float32, torch.float32)):
+        lent = scratch is not None and name in ("stats", "dwin")
+        made.append(getattr(scratch, name) if lent else guard.empty(max(n, 4), dtype=dtype, device=device, name=f"relative_attention.{name}"))
+    return RelativeWorkspace(*made)
 
 
 def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
@@ -257,28 +266,28 @@ def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
     return b, S, hd
 
 
-def _check_ws(ws, device, *need) -> None:
+def _check_ws(ws, device, need) -> None:
     at, *have = ws.sizes
     _refuse(at != device or any(h < n for h, n in zip(have, need)),
             f"the workspace is for smaller sizes: {have} values on {at}, the call needs {list(need)} on {device}")
 
 
-def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ctx_out, ws=None) -> None:
+def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ctx_out, ws) -> None:
     """``ctx = softmax(q k^T / sqrt(hd) + table[buckets[clamp(key - query)], head])`` (dropout of the probabilities) ``v``.
 
     ``q``, ``k``, ``v`` ``[b S, nh hd]``, biases added, rows may lie apart (views of one projection); ``mask`` ``[b, S]`` int32, 0 =
     masked key: it counts as absent, whatever its row holds.  A sequence without any attended key attends to all of its tokens
     alike, as :func:`renee_b200.ops.attention_fwd` has it.  ``table`` ``[buckets, nh]`` in the activations' type, ``buckets`` from
     :func:`relative_buckets` (or any int32 map of ``2 far + 1`` distances).  ``ctx_out`` ``[b S, nh hd]``, contiguous.  ``ws``
-    receives what the backward pass needs; None where there is none."""
-    key = ("relative", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, ctx_out), None if ws is None else ws.sizes,
+    (:func:`relative_attention_workspace`) receives what the backward pass needs."""
+    key = ("relative", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, ctx_out), ws.sizes,
            *(_sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else ()))
     if _first_time(key):
         b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng)
         _whole("ctx_out", ctx_out, (b * S, nh * hd), q.dtype)
         _same_place(q, ctx_out=ctx_out)
-        if q.is_cuda and ws is not None:
-            _check_ws(ws, q.device, b * nh * (-(-S // 128) * 128))
+        if q.is_cuda:
+            _check_ws(ws, q.device, _relative_sizes(b, S, nh, (buckets.numel() - 1) // 2)[:4])
         _passed(key)
     at = _pointers((ctx_out,), (q, k, v, table))
     if q.is_cuda:
@@ -298,9 +307,7 @@ def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stre
         _whole("dtable", dtable, tuple(table.shape), q.dtype)
         _same_place(q, dctx=dctx, ctx=ctx, dtable=dtable)
         if q.is_cuda:
-            far = (buckets.numel() - 1) // 2
-            stats = b * nh * (-(-S // 128) * 128)
-            _check_ws(ws, q.device, stats, stats, b * _cuda().relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
+            _check_ws(ws, q.device, _relative_sizes(b, S, nh, (buckets.numel() - 1) // 2))
         _passed(key)
     at = _pointers((dq, dk, dv, dtable), (q, k, v, dctx, ctx, table))
     if q.is_cuda:

@@ -135,7 +135,8 @@ def test_gelu8_edges():
 def _attention_call(**change):
     c = attention_inputs(2, 8, 2, 32, torch.float32)
     q, k, v = views(c)
-    a = dict(q=q, k=k, v=v, mask=c["mask"], table=c["table"], buckets=c["buckets"], nh=2, p=0.0, rng=None, stream=0, ctx_out=torch.empty(16, 64))
+    a = dict(q=q, k=k, v=v, mask=c["mask"], table=c["table"], buckets=c["buckets"], nh=2, p=0.0, rng=None, stream=0, ctx_out=torch.empty(16, 64),
+             ws=ops.relative_attention_workspace(2, 8, 2, 32, 9, torch.float32, "cpu"))
     a.update(change)
     ops.relative_attention_fwd(**a)
 
