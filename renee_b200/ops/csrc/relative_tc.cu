@@ -10,10 +10,12 @@
 // the first products and, as it stands, the MN-major B operand of the second ones).  A thread reads its row of scores from TMEM,
 // works on it, and writes 16-bit P or dS back to TMEM, where they are the A operand of the second product: scores never pass through
 // shared memory, and a row's maximum and sum need no shuffle.
-// CTAs stay (3 or 2 per SM) and take every gridDim.x-th tile.  One warp issues all copies and MMAs and runs ahead: a block's scores
-// are issued as soon as the last block's have been read into registers, so that the MMAs run under the exponentials; copies run one
-// to two blocks ahead, into the next tile's too.  MMAs with different accumulators are not taken to run in order: what one
-// reads is overwritten only behind a commit that covers it.
+// CTAs stay (2 per SM; heads of 128: 1) and take every gridDim.x-th tile.  Ten warps: 0-7 work on the scores (warp w and w + 4 share 32
+// rows and take 32 columns each), 8 issues copies (one to three blocks ahead, into the next tile's too), 9 issues MMAs from one
+// thread.  A block's scores are issued as soon as their place is free, so that the MMAs run under the exponentials.  MMAs with
+// different accumulators are not taken to run in order: what one reads is overwritten only behind a commit that covers it.
+// (One warp for copies, MMAs and the zeros for masked rows was what bounded all three kernels: 1000 clocks a block, whatever the
+// others did.)
 #include "relative.cuh"
 #include "tc.cuh"
 
@@ -96,53 +98,85 @@ template <typename T> __device__ __forceinline__ void store_row(T* out, const fl
   }
 }
 
-// own: the tile's rows and window; full / empty: the stages of blocks; scores: a block's first products; read: they are in
-// registers; done: P or dS is in TMEM; end: the tile's accumulators are complete; taken: they have been read
-constexpr int MAX_STAGES = 3;
-struct Bars { uint64_t own, full[MAX_STAGES], empty[MAX_STAGES], scores, read, done, end, taken; };
+// own: a tile's rows and window (tiles in turn); raw: copies that are not complete before masked rows are zeros; full / empty: the
+// stages of blocks; scores: a block's first products (blocks in turn); read: they are in registers; done: P or dS is in TMEM (blocks
+// in turn); freed: nothing reads a tile's rows any more; end: its accumulators are complete; taken: they have been read (tiles in
+// turn).  A barrier that somebody may come late to is doubled: its next phase cannot then pass him by.
+constexpr int MAX_STAGES = 4, WORKERS = 8;
+struct Bars { uint64_t own[2], raw[MAX_STAGES], full[MAX_STAGES], empty[MAX_STAGES], scores[2], read, done[2], freed, end, taken[2]; };
 
 __device__ __forceinline__ char* align1k(char* p) { return p + ((1024u - (tc::smem_u32(p) & 1023u)) & 1023u); }
 
-// What every kernel starts with: barriers, TMEM (`more`: 32 columns of their own beside the first ones).  `workers`: warps that work
-// on the scores; the one behind them issues
-template <int COLS, bool MORE> __device__ __forceinline__ void start(Bars* bars, uint32_t* s_tmem, int warp, int workers) {
+// What every kernel starts with: barriers, TMEM.  free_by: arrivals that say a tile's rows are free
+template <int COLS> __device__ __forceinline__ void start(Bars* bars, uint32_t* s_tmem, int warp, int free_by) {
   if (threadIdx.x == 0) {
-    tc::mbar_init(&bars->own, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(bars->own + i, 1);
+      tc::mbar_init(bars->scores + i, 1);
+      tc::mbar_init(bars->done + i, WORKERS);
+      tc::mbar_init(bars->taken + i, WORKERS);
+    }
+    for (int i = 0; i < MAX_STAGES; ++i) {
+      tc::mbar_init(bars->raw + i, 1);
+      tc::mbar_init(bars->full + i, 1);
+      tc::mbar_init(bars->empty + i, 1);
+    }
+    tc::mbar_init(&bars->read, WORKERS);
+    tc::mbar_init(&bars->freed, free_by);
     tc::mbar_init(&bars->end, 1);
-    tc::mbar_init(&bars->scores, 1);
-    tc::mbar_init(&bars->done, workers);
-    tc::mbar_init(&bars->read, workers);
-    tc::mbar_init(&bars->taken, workers);
-    for (int i = 0; i < MAX_STAGES; ++i) { tc::mbar_init(bars->full + i, 1); tc::mbar_init(bars->empty + i, 1); }
     tc::fence_barrier_init();
   }
-  if (warp == workers) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(s_tmem)), "n"(COLS) : "memory");
-    if (MORE) asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(s_tmem + 1)), "n"(32) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == WORKERS) tc::tmem_alloc(s_tmem, COLS);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
 }
-template <int COLS, bool MORE> __device__ __forceinline__ void finish(const uint32_t* s_tmem, int warp, int workers) {
+template <int COLS> __device__ __forceinline__ void finish(const uint32_t* s_tmem, int warp) {
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  if (warp == workers) {
-    tc::tmem_dealloc(s_tmem[0], COLS);
-    if (MORE) tc::tmem_dealloc(s_tmem[1], 32);
-  }
+  if (warp == WORKERS) tc::tmem_dealloc(*s_tmem, COLS);
 }
 
-// A wait of a whole warp: the same answer in every lane
+// Waits, bounded by the SM's clock (1.5 s at 2 GHz).  Once one has run out, all later ones return at once; whoever goes on then works
+// on what is there, so that he comes to all meetings, and the status word says that the results are void.
+constexpr long long WAIT_CLOCKS = 3000000000LL;
 struct Waiter {
   bool aborted;
   int* status;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t phase, int site) {
-    tc::mbar_wait(bar, phase & 1, aborted, status, site, (int)phase);
-    aborted = __any_sync(0xffffffffu, aborted);
-    return !aborted;
+  __device__ __forceinline__ void note(int site, uint32_t phase) {
+    aborted = true;
+    if (status != nullptr && atomicCAS(status, 0, 1000 + site) == 0) {
+      status[1] = (int)blockIdx.x;
+      status[2] = site;
+      status[3] = (int)phase;
+    }
+  }
+  // one thread
+  __device__ __forceinline__ bool one(uint64_t* bar, uint32_t phase, int site) {
+    if (aborted) return false;
+    if (tc::mbar_try_wait(bar, phase & 1)) return true;
+    const long long t0 = clock64();
+    do {
+#pragma unroll 1
+      for (int i = 0; i < 64; ++i)
+        if (tc::mbar_try_wait(bar, phase & 1)) return true;
+    } while (clock64() - t0 < WAIT_CLOCKS);
+    note(site, phase);
+    return false;
+  }
+  // a whole warp, with the same answer in every lane
+  __device__ __forceinline__ bool all(uint64_t* bar, uint32_t phase, int site) {
+    if (aborted) return false;
+    if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, phase & 1))) return true;
+    const long long t0 = clock64();
+    do {
+#pragma unroll 1
+      for (int i = 0; i < 64; ++i)
+        if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, phase & 1))) return true;
+    } while (__any_sync(0xffffffffu, clock64() - t0 < WAIT_CLOCKS));
+    note(site, phase);
+    return false;
   }
 };
 // One arrival for a warp whose TMEM accesses before it are complete
@@ -152,7 +186,7 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) tc::mbar_arrive(bar);
 }
 
-// The head's window and the sequence's mask, by bulk copies that count on the CTA's own barrier
+// The head's window and the sequence's mask, by bulk copies
 template <typename T> __device__ __forceinline__ uint32_t window_bytes(const Args<T>& a, int wd) { return (uint32_t)(window_floats(wd) + mask_words(a.S)) * 4u; }
 template <typename T> __device__ __forceinline__ void load_window(const Args<T>& a, int b, int h, int wd, float* win, uint64_t* bar) {
   const int n = window_floats(wd), words = mask_words(a.S);
@@ -160,23 +194,32 @@ template <typename T> __device__ __forceinline__ void load_window(const Args<T>&
   tc::bulk_load(win + n, a.bits + (size_t)b * words, words * 4, bar);
 }
 
-// 32 scores in base 2: s scale + bias, with the bias from the window (wp, in steps of DIR) or one number
-template <int DIR> __device__ __forceinline__ void add_bias(float (&s)[32], float scale, bool empty, bool far_piece, float far_bias, const float* wp) {
-  const F2 c = f2(scale);
+// 32 exponents in base 2: s scale + bias + c.  The bias comes from the window (wp), or is one number (far_piece; an empty sequence's
+// scores are zeros whatever q and k hold)
+__device__ __forceinline__ void exponents(float (&s)[32], float scale, bool empty, bool far_piece, float far_bias, const float* wp, float c) {
+  const F2 k = f2(scale);
   if (empty) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) s[j] = 0.f;
+    for (int j = 0; j < 32; ++j) s[j] = c;
   } else if (far_piece) {
-    const F2 f = f2(far_bias);
+    const F2 f = f2(far_bias + c);
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), c, f), s[j], s[j + 1]);
+    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), k, f), s[j], s[j + 1]);
   } else {
+    const F2 f = f2(c);
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), c, f2(wp[DIR * j], wp[DIR * (j + 1)])), s[j], s[j + 1]);
+    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), k, f2(wp[j], wp[j + 1])) + f, s[j], s[j + 1]);
+  }
+}
+__device__ __forceinline__ void mask_columns(float (&s)[32], uint32_t on) {
+  if (on != 0xffffffffu) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (!(on >> j & 1u)) s[j] = -INFINITY;
   }
 }
 
-// Where a tile lies: tile t of `per` tiles a (sequence, head)
+// Where a tile of queries lies: tile t of `per` tiles a (sequence, head)
 struct Place {
   int bh, b, h, row0;
   template <typename T> __device__ __forceinline__ Place(const Args<T>& a, int t, int per) {
@@ -186,197 +229,227 @@ struct Place {
     row0 = (t - bh * per) * ROWS;
   }
 };
-template <typename T> __device__ __forceinline__ int key_blocks(const Args<T>& a, int t, int per) {
-  const int seen = __ldg(a.lens + t / per / a.nh);
+template <typename T> __device__ __forceinline__ int key_blocks(const Args<T>& a, int b) {
+  const int seen = __ldg(a.lens + b);
   return ((seen > 0 ? seen : a.S) + BLK - 1) / BLK;
 }
 
-// The issuing warp of fwd and bwd_q, whose order of work is the same.
-//   own(t, k): copies of tile t, the CTA's k-th;  load(t, i, s): block i of tile t into stage s;  scores(s), rows(s, first): the products
-//   fix(k, i, s): zeros where a NaN would reach a product (the whole warp)
-template <int NST, typename T, typename Own, typename Load, typename Fix, typename Scores, typename Rows>
-__device__ __forceinline__ void issue_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, Own own, Load load, Fix fix,
-                                                  Scores scores, Rows rows) {
-  int lt = blockIdx.x, li = 0, ln = lt < tiles ? key_blocks(a, lt, per) : 0;       // the next block to load
-  unsigned loaded = 0;
-  const auto load_next = [&]() {
-    if (lt >= tiles) return;
-    if (tc::elect_one()) load(lt, li, loaded % NST);
+// The copying warp of fwd and bwd_q.  own(at, k, bar): a tile's copies, the CTA's k-th; load(at, i, s, bar): block i into stage s;
+// masked: the half of the stage (K or V) whose masked rows become zeros, because 0 times a NaN is one
+template <int NST, int CH, int PIECE, typename T, typename Own, typename Load>
+__device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, char* stage, int masked, int lane,
+                                                 Own own, Load load) {
+  unsigned g = 0, k = 0, turns = 0;                            // turns: bit s = phase of raw[s]
+  uint2 on_last = make_uint2(0xffffffffu, 0xffffffffu);        // attended keys of the block before, if it has to be mended
+  const auto mend = [&](unsigned x) {                          // block x
+    if ((on_last.x & on_last.y) == 0xffffffffu) return;
+    const int s = x % NST;
+    wait.all(bars.raw + s, turns >> s & 1u, tc::SITE_FULL);
+    turns ^= 1u << s;
+    char* tile = stage + s * 2 * PIECE + masked * PIECE;
+    for (int r = lane >> 3; r < BLK; r += 4)
+      if (!((r < 32 ? on_last.x : on_last.y) >> (r & 31) & 1u))
+#pragma unroll
+        for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(tile + c * BLK * 128 + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    tc::fence_proxy_async();
     __syncwarp();
-    ++loaded;
-    if (++li == ln) {
-      li = 0;
-      lt += gridDim.x;
-      if (lt < tiles) ln = key_blocks(a, lt, per);
-    }
+    if (lane == 0) tc::mbar_arrive(bars.full + s);
   };
-  for (int s = 0; s < NST; ++s) load_next();
-  unsigned g = 0, k = 0;                                       // blocks and tiles begun
-  // the second product of block g - 1: first / last of its tile, the CTA's j-th
-  const auto second = [&](bool first, bool last, unsigned j) {
-    if (!wait(&bars.done, g - 1, tc::SITE_TMEM_EMPTY)) return;
-    if (first && j > 0 && !wait(&bars.taken, j - 1, tc::SITE_TMEM_EMPTY)) return;
-    tc::tc_fence_after();
-    if (tc::elect_one()) {
-      rows((g - 1) % NST, first);
-      tc::umma_commit(bars.empty + (g - 1) % NST);
-      if (last) tc::umma_commit(&bars.end);
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++k) {
+    const Place at(a, t, per);
+    const int n = key_blocks(a, at.b);
+    const uint2* bits = reinterpret_cast<const uint2*>(a.bits + (size_t)at.b * mask_words(a.S));
+    for (int i = 0; i < n; ++i, ++g) {
+      const uint2 on = __ldg(bits + i);
+      const int s = g % NST;
+      if (NST == 2 && g > 0) {                                 // the product that frees this stage is issued behind the scores of block g - 1
+        mend(g - 1);
+        on_last = make_uint2(0xffffffffu, 0xffffffffu);
+      }
+      if (g >= NST) wait.all(bars.empty + s, g / NST - 1, tc::SITE_EMPTY);
+      if (wait.aborted) return;
+      if (tc::elect_one()) load(at, i, s, (on.x & on.y) == 0xffffffffu ? bars.full + s : bars.raw + s);
+      __syncwarp();
+      if (i == 0) {                                            // the first block first: it may be on its way while the last tile's rows are read
+        if (g > 0) mend(g - 1);                                // the last tile ends behind it
+        on_last = make_uint2(0xffffffffu, 0xffffffffu);
+        if (k > 0) wait.all(&bars.freed, k - 1, tc::SITE_EMPTY);
+        if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
+        if (wait.aborted) return;
+        if (tc::elect_one()) own(at, k, bars.own + (k & 1));
+        __syncwarp();
+      } else {
+        mend(g - 1);
+      }
+      on_last = on;
     }
-    __syncwarp();
+  }
+  if (g > 0) mend(g - 1);
+}
+
+// The MMA thread of fwd and bwd_q.  scores(g, s), rows(g, s, first): the products of block g, in stage s.
+// TURNS: scores have two buffers, which P shares: one is free when the product before last is complete.  Otherwise they have one,
+// free as soon as the scores are in registers, and dS has two places of its own.
+template <int NST, bool TURNS, typename T, typename Scores, typename Rows>
+__device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, Scores scores, Rows rows) {
+  unsigned g = 0, k = 0;
+  // the second product of block x: first / last of its tile, the CTA's j-th
+  const auto second = [&](unsigned x, bool first, bool last, unsigned j) {
+    wait.one(bars.done + (x & 1), x >> 1, tc::SITE_TMEM_EMPTY);
+    if (first && j > 0) wait.one(bars.taken + ((j - 1) & 1), (j - 1) >> 1, tc::SITE_TMEM_EMPTY);
+    if (wait.aborted) return;
+    tc::tc_fence_after();
+    rows(x, x % NST, first);
+    tc::umma_commit(bars.empty + x % NST);
+    if (last) tc::umma_commit(&bars.end);
   };
   int n_last = 0;
   for (int t = blockIdx.x; t < tiles && !wait.aborted; t += gridDim.x, ++k) {
-    const int n = key_blocks(a, t, per);
+    const int n = key_blocks(a, t / per / a.nh);
     for (int i = 0; i < n && !wait.aborted; ++i, ++g) {
-      if (g > 0 && !wait(&bars.read, g - 1, tc::SITE_TMEM_EMPTY)) break;
-      if (i == 0) {                                            // the last tile's scores have been read: its rows' place is free
-        if (tc::elect_one()) own(t, k);
-        __syncwarp();
-        if (g > 0) second(n_last == 1, true, k - 1);
-        if (!wait(&bars.own, k, tc::SITE_FULL)) break;
+      if (TURNS) {
+        if (g > 1) wait.one(bars.empty + (g - 2) % NST, (g - 2) / NST, tc::SITE_EMPTY);
+      } else {
+        if (g > 0) wait.one(&bars.read, g - 1, tc::SITE_TMEM_EMPTY);
       }
-      if (!wait(bars.full + g % NST, g / NST, tc::SITE_FULL)) break;
-      fix(k, i, g % NST);
+      if (i == 0 && g > 0) second(g - 1, n_last == 1, true, k - 1);      // the last tile's end before this one's rows are waited for
+      if (i == 0) wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
+      wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
+      if (wait.aborted) return;
       tc::tc_fence_after();
-      if (tc::elect_one()) {
-        scores(g % NST);
-        tc::umma_commit(&bars.scores);
-      }
-      __syncwarp();
-      if (i > 0) second(i == 1, false, k);
-      if (g > 0) {
-        if (!wait(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_EMPTY)) break;
-        load_next();
-      }
+      scores(g, g % NST);
+      tc::umma_commit(bars.scores + (g & 1));
+      if (TURNS && i + 1 == n) tc::umma_commit(&bars.freed);
+      if (i > 0) second(g - 1, i == 1, false, k);
     }
     n_last = n;
   }
-  if (g > 0 && !wait.aborted) second(n_last == 1, true, k - 1);
+  if (g > 0) second(g - 1, n_last == 1, true, k - 1);
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// 4 warps work on the scores (a row each thread).  TMEM: scores 64 columns, O behind them, P (32 columns) apart, so that the next
-// scores need not wait for P's product: 160 columns, 3 CTAs an SM (heads of 128: 2).
+// TMEM: two buffers of 64 columns for the scores of blocks in turn (P in columns 0-15 and 32-47, each warp's over its own), O from
+// 128.  The next block's scores are there when a block's P is written, so the warps never wait for a product.
 //
 // The reference point m of a row's exponentials is the maximum of its first block with an attended key, and stays: P may grow to
 // 2^60 (bf16; its rounding is relative) or, from 2^6, to 2^15 (fp16) without harm.  Where a block's sum shows that a row left that
-// range, the warp works the block again from a new reference, with O and the sum scaled to it.  So no other block needs its maximum.
+// range, both warps of the rows work the block again from a new reference, with O and the sums scaled to it.  So no other block needs
+// its maximum, and the two warps meet once a block, to hear whether the other one left the range.
 template <typename T, int HD>
-__global__ void __launch_bounds__(160, HD == 128 ? 2 : 3) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
-  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 3;
-  constexpr int COLS = HD == 128 ? 256 : 128;
-  constexpr bool FP16 = std::is_same<T, __half>::value, MORE = HD != 128;
+__global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
+  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4, COLS = 256;
+  constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
-  __shared__ uint32_t s_tmem[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_row[2][2][ROWS];                        // [maxima, sums][half][row]
   char* sq = align1k(smem_raw);
   char* stage = sq + TILE;                                   // [NST][K piece, V piece]
   const int wd = window(a), per = (a.S + ROWS - 1) / ROWS, tiles = per * a.nh * a.b, wfloats = window_floats(wd) + mask_words(a.S);
   float* windows = reinterpret_cast<float*>(stage + NST * 2 * PIECE);           // [2][window, mask]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
-  start<COLS, MORE>(&bars, s_tmem, warp, 4);
-  const uint32_t tmem = s_tmem[0], p_cols = MORE ? s_tmem[1] : tmem + 64 + HDP;
+  start<COLS>(&bars, &s_tmem, warp, 1);
+  const uint32_t tmem = s_tmem;
   Waiter wait{false, a.status};
   grid_dep_wait();
-  if (warp == 4) {
-    issue_query_tiles<NST>(
-        a, bars, wait, tiles, per,
-        [&](int t, unsigned k) {
-          const Place at(a, t, per);
-          tc::mbar_expect_tx(&bars.own, TILE + window_bytes(a, wd));
-          load_tile<CH>(sq, &maps.a, &bars.own, at.h * HD, at.row0, at.b, ROWS);
-          load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, &bars.own);
+  if (warp == WORKERS) {
+    copy_query_tiles<NST, CH, PIECE>(
+        a, bars, wait, tiles, per, stage, 1, lane,
+        [&](const Place& at, unsigned k, uint64_t* bar) {
+          tc::mbar_expect_tx(bar, TILE + window_bytes(a, wd));
+          load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
+          load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, bar);
         },
-        [&](int t, int i, int s) {
-          const Place at(a, t, per);
-          tc::mbar_expect_tx(bars.full + s, 2 * PIECE);
-          load_tile<CH>(stage + s * 2 * PIECE, &maps.b, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
-          load_tile<CH>(stage + s * 2 * PIECE + PIECE, &maps.c, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
-        },
-        [&](unsigned k, int i, int s) {                      // rows of V whose keys are masked: 0 times a NaN is one
-          const uint32_t* on = reinterpret_cast<const uint32_t*>(windows + (k & 1) * wfloats + window_floats(wd)) + 2 * i;
-          if ((on[0] & on[1]) != 0xffffffffu) {
-            zero_rows<CH>(stage + s * 2 * PIECE + PIECE, on, BLK, lane);
-            tc::fence_proxy_async();
-            __syncwarp();
-          }
-        },
-        [&](int s) { mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE)); },
-        [&](int s, bool first) { mma_rows<T, HDP>(tmem + 64, p_cols, 16, tc::smem_u32(stage + s * 2 * PIECE + PIECE), first); });
+        [&](const Place& at, int i, int s, uint64_t* bar) {
+          tc::mbar_expect_tx(bar, 2 * PIECE);
+          load_tile<CH>(stage + s * 2 * PIECE, &maps.b, bar, at.h * HD, i * BLK, at.b, BLK);
+          load_tile<CH>(stage + s * 2 * PIECE + PIECE, &maps.c, bar, at.h * HD, i * BLK, at.b, BLK);
+        });
+  } else if (warp > WORKERS) {
+    if (tc::elect_one())
+      multiply_query_tiles<NST, true>(
+          a, bars, wait, tiles, per,
+          [&](unsigned g, int s) { mma_scores<T, HD>(tmem + (g & 1) * BLK, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE)); },
+          [&](unsigned g, int s, bool first) {
+            mma_rows<T, HDP>(tmem + 128, tmem + (g & 1) * BLK, 32, tc::smem_u32(stage + s * 2 * PIECE + PIECE), first);
+          });
   } else {
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16, row_s = tmem + lanes, row_o = row_s + 64, row_p = p_cols + lanes;
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_o = tmem + lanes + 128;
     const float up = FP16 ? 6.f : 0.f, limit = FP16 ? 32768.f : 1.1529215e18f;
     const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
-    for (int t = blockIdx.x; t < tiles && !wait.aborted; t += gridDim.x, ++k) {
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++k) {
       const Place at(a, t, per);
       const int seen = __ldg(a.lens + at.b), n = ((seen > 0 ? seen : a.S) + BLK - 1) / BLK;
       const bool empty = seen == 0;
-      const int q_warp = at.row0 + warp * 32, q = q_warp + lane;
+      const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
       const float* win = windows + (k & 1) * wfloats;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
       const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S;
       float m = -INFINITY, l = 0.f;
-      if (!wait(&bars.own, k, tc::SITE_FULL)) break;
+      wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       for (int i = 0; i < n; ++i, ++g) {
-        const int k0 = i * BLK, dlo = k0 - (q_warp + 31), dhi = k0 + BLK - 1 - q_warp;
+        const int k0 = i * BLK + 32 * half, dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;     // of this warp's columns
         const bool far_piece = dhi <= -wd || dlo >= wd;
         const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
         const float* wp = win + (k0 - q) + wd + PAD;
-        if (!wait(&bars.scores, g, tc::SITE_TMEM_FULL)) break;
+        const uint32_t on = bits[k0 >> 5];
+        const uint32_t row_s = tmem + lanes + (g & 1) * BLK + 32 * half;
+        wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
         tc::tc_fence_after();
-        float s[2][32], sum;
-        const auto bias_and_mask = [&]() {
+        float s[32], sum;
+        tc::tmem_ld32(row_s, s);
+        if (__any_sync(0xffffffffu, m == -INFINITY)) {       // the same answer in both warps of the rows
+          float x = m;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            add_bias<1>(s[c], a.scale_log2, empty, far_piece, far_bias, wp + 32 * c);
-            const uint32_t on = bits[2 * i + c];
-            if (on != 0xffffffffu) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (!(on >> j & 1u)) s[c][j] = -INFINITY;
-            }
+          for (int j = 0; j < 32; ++j) {
+            const float v = empty ? 0.f : fmaf(s[j], a.scale_log2, far_piece ? far_bias : wp[j]);
+            if (on >> j & 1u) x = fmaxf(x, v);
           }
-        };
-        const auto top = [&]() {
-          float x[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
-#pragma unroll
-          for (int j = 4; j < BLK; ++j) x[j & 3] = fmaxf(x[j & 3], s[j >> 5][j & 31]);
-          return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        };
-        // P in place of the scores; returns its sum
-        const auto exponentials = [&](float (&v)[32]) {
-          const F2 base = f2(m == -INFINITY ? 0.f : up - m);
-          F2 l2 = f2(0.f);
+          s_row[0][half][row] = x;
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+          x = fmaxf(s_row[0][0][row], s_row[0][1][row]);
+          if (m == -INFINITY) m = x;
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        }
+        const auto exponentials = [&]() {
+          F2 l2[2] = {f2(0.f), f2(0.f)};
+          exponents(s, a.scale_log2, empty, far_piece, far_bias, wp, m == -INFINITY ? 0.f : up - m);
+          mask_columns(s, on);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            float x, y;
-            f2_get(f2(v[j], v[j + 1]) + base, x, y);
-            v[j] = ex2(x);
-            v[j + 1] = ex2(y);
-            l2 = l2 + f2(v[j], v[j + 1]);
+            s[j] = ex2(s[j]);
+            s[j + 1] = ex2(s[j + 1]);
+            l2[(j >> 1) & 1] = l2[(j >> 1) & 1] + f2(s[j], s[j + 1]);
           }
           float x, y;
-          f2_get(l2, x, y);
-          return x + y;
+          f2_get(l2[0] + l2[1], x, y);
+          sum = x + y;
         };
-        tmem_ld2x32(row_s, row_s + 32, s[0], s[1]);
-        bias_and_mask();
-        if (__any_sync(0xffffffffu, m == -INFINITY)) {
-          const float x = top();
-          if (m == -INFINITY) m = x;
-        }
-        sum = exponentials(s[0]);
-        sum += exponentials(s[1]);
-        if (__any_sync(0xffffffffu, sum > limit)) {
-          tmem_ld2x32(row_s, row_s + 32, s[0], s[1]);
-          bias_and_mask();
-          const float x = fmaxf(m, top()), f = m == -INFINITY ? 0.f : ex2(m - x);
-          if (i > 0) {                                       // O is at rest behind the last block's product
-            if (!wait(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_TMEM_FULL)) break;
+        exponentials();
+        uint32_t out_of_range = sum > limit;
+        asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+                     : "+r"(out_of_range) : "r"(1 + quarter) : "memory");
+        if (out_of_range) {
+          tc::tmem_ld32(row_s, s);
+          float x = m;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float v = empty ? 0.f : fmaf(s[j], a.scale_log2, far_piece ? far_bias : wp[j]);
+            if (on >> j & 1u) x = fmaxf(x, v);
+          }
+          s_row[0][half][row] = x;
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+          x = fmaxf(s_row[0][0][row], s_row[0][1][row]);
+          const float f = m == -INFINITY ? 0.f : ex2(m - x);
+          l *= f;
+          m = x;
+          if (i > 0) {                                       // O is at rest behind the last block's product; half of it each
+            wait.all(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_TMEM_FULL);
             tc::tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HDP; c += 16) {
+            for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
               uint32_t r[16], lo[8], hi[8];
               tc::tmem_issue8(row_o + c, lo);
               tc::tmem_issue8(row_o + c + 8, hi);
@@ -390,60 +463,54 @@ __global__ void __launch_bounds__(160, HD == 128 ? 2 : 3) fwd_tc(Args<T> a, cons
               tc::tmem_st16(row_o + c, r);
             }
           }
-          l *= f;
-          m = x;
-          sum = exponentials(s[0]);
-          sum += exponentials(s[1]);
+          exponentials();
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
         }
-        warp_arrive(&bars.read, lane);
         l += sum;
         if (a.p > 0.f) {
 #pragma unroll
-          for (int j = 0; j < BLK; ++j)
-            if (!keep(seed, a.stream, drop0 + k0 + j, a.p)) s[j >> 5][j & 31] = 0.f;
+          for (int j = 0; j < 32; ++j)
+            if (!keep(seed, a.stream, drop0 + k0 + j, a.p)) s[j] = 0.f;
         }
-        // the last block's product has read P
-        if (g > 0 && !wait(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_TMEM_FULL)) break;
+        uint32_t r[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t r[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = pack16<T>(s[c][2 * j], s[c][2 * j + 1]);
-          tc::tmem_st16(row_p + 16 * c, r);
-        }
+        for (int j = 0; j < 16; ++j) r[j] = pack16<T>(s[2 * j], s[2 * j + 1]);
+        tc::tmem_st16(row_s, r);
         tc::tmem_wait_st();
-        warp_arrive(&bars.done, lane);
+        warp_arrive(bars.done + (g & 1), lane);
       }
-      if (!wait(&bars.end, k, tc::SITE_TMEM_FULL)) break;
+      s_row[1][half][row] = l;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+      l = s_row[1][0][row] + s_row[1][1][row];
+      wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
       const float f = 1.f / (1.f - a.p) / l;
       T* out = a.ctx + (((size_t)at.b * a.S + q) * a.nh + at.h) * HD;
 #pragma unroll
-      for (int c = 0; c < HD; c += 32) {
+      for (int c = 0; c < CH; ++c) {
         float v[32];
-        tc::tmem_ld32(row_o + c, v);
-        if (c + 32 >= HD) warp_arrive(&bars.taken, lane);
-        if (q < a.S) store_row<T>(out + c, v, f);
+        tc::tmem_ld32(row_o + half * 32 + 64 * c, v);
+        if (c == CH - 1) warp_arrive(bars.taken + (k & 1), lane);
+        if (q < a.S && half * 32 + 64 * c < HD) store_row<T>(out + half * 32 + 64 * c, v, f);
       }
-      a.lse[(size_t)at.bh * a.Sp + q] = q < a.S ? (m - up) + lg2(l) : INFINITY;
+      if (half == 0) a.lse[(size_t)at.bh * a.Sp + q] = q < a.S ? (m - up) + lg2(l) : INFINITY;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
     }
   }
-  finish<COLS, MORE>(s_tmem, warp, 4);
+  finish<COLS>(&s_tmem, warp);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: queries
-// 8 warps work on the scores: warp w and w + 4 share 32 rows and take 32 columns each.  TMEM: scores 64 columns, dP 64, dQ from 128,
-// dS (32) behind it.  delta for these rows is dctx ctx; the keys' pass gets the sum of P dP that is made on the way, which is free of
+// TMEM: scores 64 columns, dP 64, dQ from 128, behind it two places of 32 for the dS of blocks in turn.  delta for these rows is dctx ctx; the keys' pass gets the sum of P dP that is made on the way, which is free of
 // ctx's rounding (dtable's error at 32 x 512 tokens in fp16: 3.9e-4 with dctx ctx in both, 2.2e-4 so).
 template <typename T, int HD>
-__global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 3;
   constexpr int COLS = HD == 128 ? 512 : 256;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
-  __shared__ uint32_t s_tmem[1];
+  __shared__ uint32_t s_tmem;
   __shared__ float s_sum[2][2][ROWS];
-  __shared__ int s_abort;
   char* sq = align1k(smem_raw);
   char* sdo = sq + TILE;
   char* sctx = sdo + TILE;
@@ -451,41 +518,34 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   const int wd = window(a), per = (a.S + ROWS - 1) / ROWS, tiles = per * a.nh * a.b, wfloats = window_floats(wd) + mask_words(a.S);
   float* windows = reinterpret_cast<float*>(stage + NST * 2 * PIECE);           // [2][window, mask]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) s_abort = 0;
-  start<COLS, false>(&bars, s_tmem, warp, 8);
-  const uint32_t tmem = s_tmem[0], ds_cols = tmem + 128 + HDP;
+  start<COLS>(&bars, &s_tmem, warp, WORKERS);
+  const uint32_t tmem = s_tmem, ds_cols = tmem + 128 + HDP;
   Waiter wait{false, a.status};
   grid_dep_wait();
-  if (warp == 8) {
-    issue_query_tiles<NST>(
-        a, bars, wait, tiles, per,
-        [&](int t, unsigned k) {
-          const Place at(a, t, per);
-          tc::mbar_expect_tx(&bars.own, 3 * TILE + window_bytes(a, wd));
-          load_tile<CH>(sq, &maps.a, &bars.own, at.h * HD, at.row0, at.b, ROWS);
-          load_tile<CH>(sdo, &maps.d, &bars.own, at.h * HD, at.row0, at.b, ROWS);
-          load_tile<CH>(sctx, &maps.e, &bars.own, at.h * HD, at.row0, at.b, ROWS);
-          load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, &bars.own);
+  if (warp == WORKERS) {
+    copy_query_tiles<NST, CH, PIECE>(
+        a, bars, wait, tiles, per, stage, 0, lane,
+        [&](const Place& at, unsigned k, uint64_t* bar) {
+          tc::mbar_expect_tx(bar, 3 * TILE + window_bytes(a, wd));
+          load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
+          load_tile<CH>(sdo, &maps.d, bar, at.h * HD, at.row0, at.b, ROWS);
+          load_tile<CH>(sctx, &maps.e, bar, at.h * HD, at.row0, at.b, ROWS);
+          load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, bar);
         },
-        [&](int t, int i, int s) {
-          const Place at(a, t, per);
-          tc::mbar_expect_tx(bars.full + s, 2 * PIECE);
-          load_tile<CH>(stage + s * 2 * PIECE, &maps.b, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
-          load_tile<CH>(stage + s * 2 * PIECE + PIECE, &maps.c, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
-        },
-        [&](unsigned k, int i, int s) {                      // rows of K whose keys are masked: 0 times a NaN is one
-          const uint32_t* on = reinterpret_cast<const uint32_t*>(windows + (k & 1) * wfloats + window_floats(wd)) + 2 * i;
-          if ((on[0] & on[1]) != 0xffffffffu) {
-            zero_rows<CH>(stage + s * 2 * PIECE, on, BLK, lane);
-            tc::fence_proxy_async();
-            __syncwarp();
-          }
-        },
-        [&](int s) {
-          mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE));
-          mma_scores<T, HD>(tmem + 64, tc::smem_u32(sdo), tc::smem_u32(stage + s * 2 * PIECE + PIECE));
-        },
-        [&](int s, bool first) { mma_rows<T, HDP>(tmem + 128, ds_cols, 16, tc::smem_u32(stage + s * 2 * PIECE), first); });
+        [&](const Place& at, int i, int s, uint64_t* bar) {
+          tc::mbar_expect_tx(bar, 2 * PIECE);
+          load_tile<CH>(stage + s * 2 * PIECE, &maps.b, bar, at.h * HD, i * BLK, at.b, BLK);
+          load_tile<CH>(stage + s * 2 * PIECE + PIECE, &maps.c, bar, at.h * HD, i * BLK, at.b, BLK);
+        });
+  } else if (warp > WORKERS) {
+    if (tc::elect_one())
+      multiply_query_tiles<NST, false>(
+          a, bars, wait, tiles, per,
+          [&](unsigned, int s) {
+            mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE));
+            mma_scores<T, HD>(tmem + 64, tc::smem_u32(sdo), tc::smem_u32(stage + s * 2 * PIECE + PIECE));
+          },
+          [&](unsigned g, int s, bool first) { mma_rows<T, HDP>(tmem + 128, ds_cols + (g & 1) * 32, 16, tc::smem_u32(stage + s * 2 * PIECE), first); });
   } else {
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_s = tmem + lanes + 32 * half, row_dq = tmem + lanes + 128, row_ds = ds_cols + lanes + 16 * half;
@@ -501,7 +561,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       const float* win = windows + (k & 1) * wfloats;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
       const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S + half * 32;
-      wait(&bars.own, k, tc::SITE_FULL);
+      wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       float d = 0.f;                                         // delta = dctx ctx: half a row each
 #pragma unroll
       for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
@@ -514,17 +574,18 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       }
       s_sum[0][half][row] = d;
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const F2 nl = f2(-lse), nd = f2(-(s_sum[0][0][row] + s_sum[0][1][row]));
+      const F2 nd = f2(-(s_sum[0][0][row] + s_sum[0][1][row]));
       F2 sum = f2(0.f);
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + half * 32;                  // of this warp's columns
         const int dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;
-        if (!wait(&bars.scores, g, tc::SITE_TMEM_FULL)) break;
+        wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
         tc::tc_fence_after();
         float s[32], dp[32];
         tmem_ld2x32(row_s, row_s + 64, s, dp);
         warp_arrive(&bars.read, lane);
-        add_bias<1>(s, a.scale_log2, empty, dhi <= -wd || dlo >= wd, dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD], win + (k0 - q) + wd + PAD);
+        if (i + 1 == n && lane == 0) tc::mbar_arrive(&bars.freed);
+        exponents(s, a.scale_log2, empty, dhi <= -wd || dlo >= wd, dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD], win + (k0 - q) + wd + PAD, -lse);
         if (a.p > 0.f) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) dp[j] = keep(seed, a.stream, drop0 + i * BLK + j, a.p) ? dp[j] * kept : 0.f;
@@ -541,9 +602,8 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
         uint32_t r[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
+          const F2 pr = f2(ex2(s[j]), ex2(s[j + 1])), v = f2(dp[j], dp[j + 1]);
           float x, y;
-          f2_get(f2(s[j], s[j + 1]) + nl, x, y);
-          const F2 pr = f2(ex2(x), ex2(y)), v = f2(dp[j], dp[j + 1]);
           sum = f2_fma(pr, v, sum);
           f2_get(pr * (v + nd), x, y);
           r[j / 2] = pack16<T>(x, y);
@@ -552,30 +612,26 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 #pragma unroll
           for (int j = 0; j < 16; ++j) r[j] = 0u;
         }
-        // the last block's product has read dS
-        if (g > 0 && !wait(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_TMEM_FULL)) break;
-        tc::tmem_st16(row_ds, r);
+        tc::tmem_st16(row_ds + (g & 1) * 32, r);             // the product before last has read it: it was issued before these scores
         tc::tmem_wait_st();
-        warp_arrive(&bars.done, lane);
+        warp_arrive(bars.done + (g & 1), lane);
       }
       float x, y;
       f2_get(sum, x, y);
       s_sum[1][half][row] = x + y;
-      if (wait.aborted) s_abort = 1;                         // a warp that gave up still comes to the meetings; all leave behind one
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (*(volatile int*)&s_abort) break;
       if (half == 0) {                                       // negative, as the keys' pass adds them; behind S nothing is left of P
         a.delta[(size_t)at.bh * a.Sp + q] = q < a.S ? -(s_sum[1][0][row] + s_sum[1][1][row]) * a.grad_inv : 0.f;
         a.lse_up[(size_t)at.bh * a.Sp + q] = -lse;
       }
-      if (!wait(&bars.end, k, tc::SITE_TMEM_FULL)) continue;
+      wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
       T* out = a.dq + ((size_t)at.b * a.S + q) * a.lddq + at.h * HD;
       const float f = a.scale * a.grad_inv;
       float v[HDP / 64][32];
 #pragma unroll
       for (int c = 0; c < HDP / 64; ++c) tc::tmem_ld32(row_dq + half * 32 + 64 * c, v[c]);
-      warp_arrive(&bars.taken, lane);
+      warp_arrive(bars.taken + (k & 1), lane);
 #pragma unroll
       for (int c = 0; c < HDP / 64; ++c) {
         if (empty) {
@@ -586,7 +642,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       }
     }
   }
-  finish<COLS, false>(s_tmem, warp, 8);
+  finish<COLS>(&s_tmem, warp);
 }
 
 // ------------------------------------------------------------------------------------------------ backward: keys
@@ -597,15 +653,14 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 // running sum handed to the next lane collects it: one shuffle and one add per column.  Lane 31 drops a finished diagonal each
 // step, the last 32 are in the lanes at the end; the warp then adds all 63 to its window of sums.  This runs under the products.
 template <typename T, int HD>
-__global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH;
   constexpr int STAGE = 2 * PIECE + 2 * BLK * 4;             // Q piece, dO piece, -lse, -delta
   constexpr int STAGE_UP = (STAGE + 1023) / 1024 * 1024, NST = HD == 128 ? 2 : 3, COLS = HD == 128 ? 512 : 256;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
-  __shared__ uint32_t s_tmem[1];
+  __shared__ uint32_t s_tmem;
   __shared__ float s_diag[8][64];
-  __shared__ int s_abort;
   __shared__ float s_none[32];                               // the window of a masked key
   char* sk = align1k(smem_raw);
   char* sv = sk + TILE;
@@ -615,95 +670,99 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   float* windows = reinterpret_cast<float*>(stage + NST * STAGE_UP);            // [2][window, mask]
   float* sums = windows + 2 * wfloats;                       // [8][nwin]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) s_abort = 0;
-  start<COLS, false>(&bars, s_tmem, warp, 8);
-  const uint32_t tmem = s_tmem[0];
+  start<COLS>(&bars, &s_tmem, warp, WORKERS);
+  const uint32_t tmem = s_tmem;
   Waiter wait{false, a.status};
   grid_dep_wait();
+  // tiles in order of their place in the sequence: the last ones, of which few have an attended key, are spread over all CTAs
+  const auto place = [&](int t) {
+    const int bhs = a.nh * a.b, part = t / bhs;
+    return Place(a, (t - part * bhs) * per + part, per);
+  };
   // a tile without an attended key has no gradient and no blocks
   const auto blocks = [&](int t) {
-    const Place at(a, t, per);
+    const Place at = place(t);
     const int seen = __ldg(a.lens + at.b);
     return at.row0 < (seen > 0 ? seen : a.S) ? nq : 0;
   };
-  if (warp == 8) {
-    int lt = blockIdx.x, li = 0;
-    while (lt < tiles && blocks(lt) == 0) lt += gridDim.x;
-    unsigned loaded = 0;
-    const auto load_next = [&]() {
-      if (lt >= tiles) return;
-      if (tc::elect_one()) {
-        const Place at(a, lt, per);
-        char* st = stage + (loaded % NST) * STAGE_UP;
-        uint64_t* bar = bars.full + loaded % NST;
-        tc::mbar_expect_tx(bar, STAGE);
-        load_tile<CH>(st, &maps.a, bar, at.h * HD, li * BLK, at.b, BLK);
-        load_tile<CH>(st + PIECE, &maps.d, bar, at.h * HD, li * BLK, at.b, BLK);
-        tc::bulk_load(st + 2 * PIECE, a.lse_up + (size_t)at.bh * a.Sp + li * BLK, BLK * 4, bar);
-        tc::bulk_load(st + 2 * PIECE + BLK * 4, a.delta + (size_t)at.bh * a.Sp + li * BLK, BLK * 4, bar);
+  if (warp == WORKERS) {
+    unsigned g = 0, k = 0, turn = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      if (blocks(t) == 0) continue;
+      const Place at = place(t);
+      const uint4 on = __ldg(reinterpret_cast<const uint4*>(a.bits + (size_t)at.b * mask_words(a.S)) + at.row0 / ROWS);
+      const bool whole = (on.x & on.y & on.z & on.w) == 0xffffffffu;
+      for (int i = 0; i < nq; ++i, ++g) {
+        const int s = g % NST;
+        if (g >= NST) wait.all(bars.empty + s, g / NST - 1, tc::SITE_EMPTY);
+        if (wait.aborted) break;
+        if (tc::elect_one()) {
+          char* st = stage + s * STAGE_UP;
+          tc::mbar_expect_tx(bars.full + s, STAGE);
+          load_tile<CH>(st, &maps.a, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
+          load_tile<CH>(st + PIECE, &maps.d, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
+          tc::bulk_load(st + 2 * PIECE, a.lse_up + (size_t)at.bh * a.Sp + i * BLK, BLK * 4, bars.full + s);
+          tc::bulk_load(st + 2 * PIECE + BLK * 4, a.delta + (size_t)at.bh * a.Sp + i * BLK, BLK * 4, bars.full + s);
+        }
+        __syncwarp();
+        if (i > 0) continue;
+        if (k > 0) wait.all(&bars.freed, k - 1, tc::SITE_EMPTY);
+        if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
+        if (wait.aborted) break;
+        uint64_t* bar = whole ? bars.own + (k & 1) : bars.raw;
+        if (tc::elect_one()) {
+          tc::mbar_expect_tx(bar, 2 * TILE + window_bytes(a, wd));
+          load_tile<CH>(sk, &maps.b, bar, at.h * HD, at.row0, at.b, ROWS);
+          load_tile<CH>(sv, &maps.c, bar, at.h * HD, at.row0, at.b, ROWS);
+          load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, bar);
+        }
+        __syncwarp();
+        if (!whole) {
+          wait.all(bars.raw, turn++, tc::SITE_FULL);
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(windows + (k & 1) * wfloats + window_floats(wd)) + (at.row0 >> 5);
+          zero_rows<CH>(sk, w, ROWS, lane);
+          zero_rows<CH>(sv, w, ROWS, lane);
+          tc::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(bars.own + (k & 1));
+        }
       }
-      __syncwarp();
-      ++loaded;
-      if (++li == nq) {
-        li = 0;
-        do lt += gridDim.x; while (lt < tiles && blocks(lt) == 0);
-      }
-    };
-    for (int s = 0; s < NST; ++s) load_next();
-    unsigned g = 0, k = 0;
-    const auto second = [&](bool first, bool last, unsigned j) {
-      if (!wait(&bars.done, g - 1, tc::SITE_TMEM_EMPTY)) return;
-      if (first && j > 0 && !wait(&bars.taken, j - 1, tc::SITE_TMEM_EMPTY)) return;
-      tc::tc_fence_after();
-      if (tc::elect_one()) {
-        char* st = stage + ((g - 1) % NST) * STAGE_UP;
+      if (wait.aborted) break;
+      ++k;
+    }
+  } else if (warp > WORKERS) {
+    if (tc::elect_one()) {
+      unsigned g = 0, k = 0;
+      // the second products of block x, and the wait for them: the next scores go where P~ and dS are
+      const auto second = [&](unsigned x, bool first, bool last, unsigned j) {
+        wait.one(bars.done + (x & 1), x >> 1, tc::SITE_TMEM_EMPTY);
+        if (first && j > 0) wait.one(bars.taken + ((j - 1) & 1), (j - 1) >> 1, tc::SITE_TMEM_EMPTY);
+        if (wait.aborted) return;
+        tc::tc_fence_after();
+        char* st = stage + (x % NST) * STAGE_UP;
         mma_rows<T, HDP>(tmem + 128, tmem, 32, tc::smem_u32(st + PIECE), first);
         mma_rows<T, HDP>(tmem + 128 + HDP, tmem + 64, 32, tc::smem_u32(st), first);
-        tc::umma_commit(bars.empty + (g - 1) % NST);
+        tc::umma_commit(bars.empty + x % NST);
         if (last) tc::umma_commit(&bars.end);
-      }
-      __syncwarp();
-      if (!wait(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_EMPTY)) return;
-      load_next();
-    };
-    for (int t = blockIdx.x; t < tiles && !wait.aborted; t += gridDim.x) {
-      if (blocks(t) == 0) continue;
-      for (int i = 0; i < nq && !wait.aborted; ++i, ++g) {
-        if (i == 0) {
-          if (k > 0 && !wait(&bars.read, k - 1, tc::SITE_TMEM_EMPTY)) break;      // reported once a tile here
-          if (tc::elect_one()) {
-            const Place at(a, t, per);
-            tc::mbar_expect_tx(&bars.own, 2 * TILE + window_bytes(a, wd));
-            load_tile<CH>(sk, &maps.b, &bars.own, at.h * HD, at.row0, at.b, ROWS);
-            load_tile<CH>(sv, &maps.c, &bars.own, at.h * HD, at.row0, at.b, ROWS);
-            load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, &bars.own);
-          }
-          __syncwarp();
-        }
-        if (g > 0) second(nq == 1 || i == 1, i == 0, i == 0 ? k - 1 : k);
-        if (i == 0) {
-          if (!wait(&bars.own, k, tc::SITE_FULL)) break;
-          const uint32_t* on = reinterpret_cast<const uint32_t*>(windows + (k & 1) * wfloats + window_floats(wd)) + (Place(a, t, per).row0 >> 5);
-          if ((on[0] & on[1] & on[2] & on[3]) != 0xffffffffu) {
-            zero_rows<CH>(sk, on, ROWS, lane);
-            zero_rows<CH>(sv, on, ROWS, lane);
-            tc::fence_proxy_async();
-            __syncwarp();
-          }
-        }
-        if (!wait(bars.full + g % NST, g / NST, tc::SITE_FULL)) break;
-        tc::tc_fence_after();
-        if (tc::elect_one()) {
+        wait.one(bars.empty + x % NST, x / NST, tc::SITE_EMPTY);
+      };
+      for (int t = blockIdx.x; t < tiles && !wait.aborted; t += gridDim.x) {
+        if (blocks(t) == 0) continue;
+        for (int i = 0; i < nq && !wait.aborted; ++i, ++g) {
+          if (g > 0) second(g - 1, nq == 1 || i == 1, i == 0, i == 0 ? k - 1 : k);
+          if (i == 0) wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
+          wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
+          if (wait.aborted) break;
+          tc::tc_fence_after();
           const char* st = stage + (g % NST) * STAGE_UP;
           mma_scores<T, HD>(tmem, tc::smem_u32(sk), tc::smem_u32(st));
           mma_scores<T, HD>(tmem + 64, tc::smem_u32(sv), tc::smem_u32(st + PIECE));
-          tc::umma_commit(&bars.scores);
+          tc::umma_commit(bars.scores + (g & 1));
         }
-        __syncwarp();
+        ++k;
       }
-      ++k;
+      if (g > 0 && !wait.aborted) second(g - 1, nq == 1, true, k - 1);
     }
-    if (g > 0 && !wait.aborted) second(nq == 1, true, k - 1);
   } else {
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_s = tmem + lanes + 32 * half, row_acc = tmem + lanes + 128 + 32 * half;
@@ -715,11 +774,11 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     asm volatile("bar.sync 1, 256;" ::: "memory");
     unsigned g = 0, k = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const Place at(a, t, per);
+      const Place at = place(t);
       const int k_warp = at.row0 + quarter * 32, key = k_warp + lane, n = blocks(t);
       T* const out_v = a.dv + ((size_t)at.b * a.S + key) * a.lddv + at.h * HD;
       T* const out_k = a.dk + ((size_t)at.b * a.S + key) * a.lddk + at.h * HD;
-      float* const out_w = a.dwin + ((size_t)(at.b * per + t % per) * a.nh + at.h) * nwin;
+      float* const out_w = a.dwin + ((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin;
       if (n == 0) {
         float v[32] = {};
         if (key < a.S)
@@ -732,7 +791,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         continue;
       }
       const bool empty = __ldg(a.lens + at.b) == 0;
-      wait(&bars.own, k, tc::SITE_FULL);
+      wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       const float* win = windows + (k & 1) * wfloats;
       const bool on = reinterpret_cast<const uint32_t*>(win + window_floats(wd))[key >> 5] >> (key & 31) & 1u;
       float far[2] = {};
@@ -740,15 +799,20 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         const int q0 = i * BLK + half * 32;                  // of this warp's columns
         const int dlo = k_warp - (q0 + 31), dhi = k_warp + 31 - q0;
         const bool far_piece = dhi <= -wd || dlo >= wd;
-        if (!wait(&bars.scores, g, tc::SITE_TMEM_FULL)) break;
+        wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
         tc::tc_fence_after();
         float s[32], dp[32];
         tmem_ld2x32(row_s, row_s + 64, s, dp);
-        if (i + 1 == n) warp_arrive(&bars.read, lane);
+        if (i + 1 == n) warp_arrive(&bars.freed, lane);
         const float4* lse = reinterpret_cast<const float4*>(stage + (g % NST) * STAGE_UP + 2 * PIECE + half * 128);
         const float4* del = lse + BLK / 4;
-        add_bias<-1>(s, a.scale_log2, empty, far_piece, !on ? -INFINITY : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD],
-                     on ? win + (key - q0) + wd + PAD : s_none + 31);
+        const float far_bias = !on ? -INFINITY : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+        const float* wp = on ? win + (key - q0) + wd + PAD : s_none + 31;
+        const F2 scale = f2(empty ? 0.f : a.scale_log2);
+        if (empty) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) s[j] = 0.f;
+        }
         uint32_t r[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
@@ -758,7 +822,8 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           for (int e = 0; e < 2; ++e) {
             const int c = j + 2 * e;
             float x, y;
-            f2_get(f2(s[c], s[c + 1]) + ls[e], x, y);
+            f2_get(far_piece || empty ? f2_fma(f2(s[c], s[c + 1]), scale, ls[e] + f2(empty ? 0.f : far_bias))
+                                      : f2_fma(f2(s[c], s[c + 1]), scale, f2(wp[-c], wp[-c - 1])) + ls[e], x, y);
             const F2 pr = f2(ex2(x), ex2(y));
             F2 v = f2(dp[c], dp[c + 1]);
             if (a.p > 0.f) {
@@ -782,7 +847,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         for (int j = 0; j < 16; ++j) r[j] = pack16<T>(dp[2 * j], dp[2 * j + 1]);
         tc::tmem_st16(row_s + 64, r);
         tc::tmem_wait_st();
-        warp_arrive(&bars.done, lane);
+        warp_arrive(bars.done + (g & 1), lane);
         if (far_piece) {
           float v = 0.f;
 #pragma unroll
@@ -816,9 +881,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         mine[0] += far[0];
         mine[2 * wd] += far[1];
       }
-      if (wait.aborted) s_abort = 1;                         // a warp that gave up still comes to the meetings; all leave behind one
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const bool leave = *(volatile int*)&s_abort != 0;
       for (int i = threadIdx.x; i < nwin; i += 256) {
         float v = 0.f;
 #pragma unroll
@@ -829,8 +892,7 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         out_w[i] = v * a.grad_inv;
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (leave) break;
-      if (!wait(&bars.end, k++, tc::SITE_TMEM_FULL)) continue;
+      wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
 #pragma unroll
       for (int o = 0; o < 2; ++o)
@@ -838,16 +900,17 @@ __global__ void __launch_bounds__(288, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         for (int c = 0; c < CH; ++c) {
           float v[32];
           tc::tmem_ld32(row_acc + o * HDP + 64 * c, v);
-          if (o == 1 && c == CH - 1) warp_arrive(&bars.taken, lane);
+          if (o == 1 && c == CH - 1) warp_arrive(bars.taken + (k & 1), lane);
           if (o == 1 && empty) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.f;
           }
           if (key < a.S && 32 * half + 64 * c < HD) store_row<T>((o ? out_k : out_v) + 32 * half + 64 * c, v, o ? a.scale * a.grad_inv : a.grad_inv);
         }
+      ++k;
     }
   }
-  finish<COLS, false>(s_tmem, warp, 8);
+  finish<COLS>(&s_tmem, warp);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -856,7 +919,7 @@ template <typename K> int allow_smem(K kernel, int bytes) {
 }
 
 template <typename T, int HD> int run_fwd_tc(const Args<T>& a, cudaStream_t st) {
-  constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = HD == 128 ? 2 : 3;
+  constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = HD == 128 ? 2 : 4;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps m;
   const uint64_t H = (uint64_t)a.nh * HD;
@@ -868,8 +931,8 @@ template <typename T, int HD> int run_fwd_tc(const Args<T>& a, cudaStream_t st) 
   const int smem = 1024 + (ROWS + NST * 2 * BLK) * 128 * CH + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
   rc = allow_smem(fwd_tc<T, HD>, smem);
   if (rc) return rc;
-  const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * (HD == 128 ? 2 : 3);
-  return (int)launch_pdl(fwd_tc<T, HD>, dim3(tiles < most ? tiles : most), dim3(160), smem, st, a, m);
+  const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * 2;
+  return (int)launch_pdl(fwd_tc<T, HD>, dim3(tiles < most ? tiles : most), dim3(320), smem, st, a, m);
 }
 
 template <typename T, int HD> int run_bwd_tc(const Args<T>& a, cudaStream_t st) {
@@ -895,8 +958,8 @@ template <typename T, int HD> int run_bwd_tc(const Args<T>& a, cudaStream_t st) 
   if (!rc) rc = allow_smem(bwd_kv_tc<T, HD>, smem_kv);
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * (HD == 128 ? 1 : 2);
   const dim3 grid(tiles < most ? tiles : most);
-  if (!rc) rc = (int)launch_pdl(bwd_q_tc<T, HD>, grid, dim3(288), smem_q, st, a, q);
-  if (!rc) rc = (int)launch_pdl(bwd_kv_tc<T, HD>, grid, dim3(288), smem_kv, st, a, kv);
+  if (!rc) rc = (int)launch_pdl(bwd_q_tc<T, HD>, grid, dim3(320), smem_q, st, a, q);
+  if (!rc) rc = (int)launch_pdl(bwd_kv_tc<T, HD>, grid, dim3(320), smem_kv, st, a, kv);
   return rc;
 }
 
