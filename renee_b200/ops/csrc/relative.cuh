@@ -50,7 +50,7 @@ template <typename T> struct Args {
 template <typename T> __host__ __device__ __forceinline__ int window(const Args<T>& a) { return a.far < a.S - 1 ? a.far : a.S - 1; }
 
 // Entry i of a head's window is the bias of distance clamp(i - PAD - wd, -wd, wd): a block that reaches beyond the window reads on
-constexpr int PAD = 192;
+constexpr int PAD = 128;
 __host__ __device__ __forceinline__ int window_floats(int wd) { return (2 * wd + 1 + 2 * PAD + 3) / 4 * 4; }
 __host__ __device__ __forceinline__ int mask_words(int S) { return (S + 127) / 128 * 4; }       // whole tiles of 128, zeros behind S
 

@@ -481,7 +481,8 @@ def relative_attention_bwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream
     dq_, dk_, dv_, dtable, _, _, _, dctx, ctx, _ = at
     _call_typed("rb_relative_bwd", q.device, DT[q.dtype], dctx,
                 *_relative_inputs(at[4:7], q, k, v, mask, table, buckets, nh, p, rng, stream, ws), buckets.data_ptr(), ctx, ws.lse.data_ptr(),
-                ws.stats.data_ptr(), ws.dwin.data_ptr(), dq_, _ld(dq), dk_, _ld(dk), dv_, _ld(dv), dtable, launches=3 if mask.shape[0] else 1)
+                ws.stats.data_ptr(), ws.dwin.data_ptr(), dq_, _ld(dq), dk_, _ld(dk), dv_, _ld(dv), dtable,
+                launches=1 + (0 if not mask.shape[0] else 2 if mask.shape[1] > 64 else 1))
 
 
 def gelu8_splits(T: int, F: int) -> int:

@@ -23,7 +23,7 @@ from . import reference as ref
 from ..utils import guard
 
 HEAD_DIMS = (32, 64, 128)
-MAX_DISTANCE = 1024               # of the bucket map: the window of sums by distance lives in shared memory
+MAX_DISTANCE = 512                # of the bucket map: the window of sums by distance lives in shared memory
 GELU8_BLOCK = 128                 # neighbouring values of a row that share a scale
 
 
