@@ -39,7 +39,7 @@ template <int HD> __device__ __forceinline__ float head_sum(float v) {
 
 // Every lane of a warp takes part in the shuffles; lanes behind the last head hold zeros.
 template <typename T, int HD>
-__global__ void __launch_bounds__(THREADS) fwd_kernel(const T* __restrict__ x, const T* __restrict__ gq, const T* __restrict__ gk,
+__global__ void __launch_bounds__(THREADS, 4) fwd_kernel(const T* __restrict__ x, const T* __restrict__ gq, const T* __restrict__ gk,
                                                       T* __restrict__ y, unsigned total, size_t ldx, size_t ldy, Args a) {
   constexpr int CH = HD / 16;
   grid_dep_wait();
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(const T* __restrict__ x, c
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(THREADS) bwd_kernel(const T* dy, const T* __restrict__ x, const T* __restrict__ gq,
+__global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const T* dy, const T* __restrict__ x, const T* __restrict__ gq,
                                                       const T* __restrict__ gk, T* dx, float* __restrict__ part_out,
                                                       unsigned total, size_t lddy, size_t ldx, size_t lddx, Args a) {
   constexpr int CH = HD / 16;
@@ -90,6 +90,18 @@ __global__ void __launch_bounds__(THREADS) bwd_kernel(const T* dy, const T* __re
   float g1[8], g2[8], d1[8] = {}, d2[8] = {};
   load8(&(part ? gk : gq)[c], g1);
   load8(&(part ? gk : gq)[HD / 2 + c], g2);
+  // the next item's values are on their way while one is worked on (the compiler may not move loads over the stores: dx may be dy)
+  struct Item { Raw8<T> x1, x2, y1, y2; };
+  const auto fetch = [&](unsigned i, Item& it) {
+    const unsigned t = i / per, h = (i - t * per) / CH;
+    const size_t col = (size_t)part * a.nh * HD + (size_t)h * HD + c;
+    it.x1 = load_raw8(x + t * ldx + col);
+    it.x2 = load_raw8(x + t * ldx + col + HD / 2);
+    it.y1 = load_raw8(dy + t * lddy + col);
+    it.y2 = load_raw8(dy + t * lddy + col + HD / 2);
+  };
+  Item next = {};
+  if (blockIdx.x * THREADS + threadIdx.x < total) fetch(blockIdx.x * THREADS + threadIdx.x, next);
   for (unsigned base = blockIdx.x * THREADS; base < total; base += gridDim.x * THREADS) {
     const unsigned i = base + threadIdx.x;
     const bool on = i < total;
@@ -97,14 +109,15 @@ __global__ void __launch_bounds__(THREADS) bwd_kernel(const T* dy, const T* __re
     const size_t col = (size_t)part * a.nh * HD + (size_t)h * HD + c;
     float x1[8] = {}, x2[8] = {}, y1[8] = {}, y2[8] = {}, cs[8] = {}, sn[8] = {};
     if (on) {
-      load8(x + t * ldx + col, x1);
-      load8(x + t * ldx + col + HD / 2, x2);
-      load8(dy + t * lddy + col, y1);
-      load8(dy + t * lddy + col + HD / 2, y2);
       const float* tab = a.table + (size_t)position(a, t) * HD + c;
       load8(tab, cs);
       load8(tab + HD / 2, sn);
+      unpack8(next.x1, x1);
+      unpack8(next.x2, x2);
+      unpack8(next.y1, y1);
+      unpack8(next.y2, y2);
     }
+    if (i + gridDim.x * THREADS < total) fetch(i + gridDim.x * THREADS, next);
     float s = 0.f, m = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -168,8 +181,7 @@ int bwd(const void* dy, const void* x, const void* gq, const void* gk, void* dx,
                              (T*)dx, part, total, (size_t)lddy, (size_t)ldx, (size_t)lddx, a);
     if (rc) return rc;
   }
-  int rc = sum_partials<T>(part, (T*)dgq, blocks, HD, 2 * HD, st);
-  return rc ? rc : sum_partials<T>(part + HD, (T*)dgk, blocks, HD, 2 * HD, st);
+  return sum_partials<T>(part, (T*)dgq, (T*)dgk, blocks, 2 * HD, HD, st);
 }
 
 template <typename F> int by_type(int dtype, F&& f) {
@@ -186,11 +198,12 @@ template <typename F> int by_type(int dtype, F&& f) {
 
 using namespace rb;
 
-// CTAs per half (queries, keys) of either pass: at most 4 per SM in all, at least one item per thread.
-RB_API int rb_qk_norm_rotary_blocks(long long T, int nh, int hd) {
-  const long long total = T * nh * (hd / 16), need = (total + rot::THREADS - 1) / rot::THREADS;
-  return (int)(need < 2 * sm_count() ? need : 2 * sm_count());
+// CTAs per half (queries, keys): one wave, which is 2 per SM in all backward and 4 forward; at least one item per thread
+static int rotary_blocks(long long total, int most) {
+  const long long need = (total + rot::THREADS - 1) / rot::THREADS;
+  return (int)(need < most ? need : most);
 }
+RB_API int rb_qk_norm_rotary_blocks(long long T, int nh, int hd) { return rotary_blocks(T * nh * (hd / 16), sm_count()); }
 
 RB_API int rb_qk_norm_rotary_fwd(int dtype, const void* x, long long ldx, const void* gq, const void* gk, const void* table,
                                  const void* positions, void* y, long long ldy, long long T, int n_pos, int S, int nh, int hd, float eps,
@@ -198,7 +211,7 @@ RB_API int rb_qk_norm_rotary_fwd(int dtype, const void* x, long long ldx, const 
   const rot::Args a{(const float*)table, (const int*)positions, n_pos, S, nh, eps};
   const unsigned total = (unsigned)(T * nh * (hd / 16));
   if (total == 0) return 0;
-  const int blocks = rb_qk_norm_rotary_blocks(T, nh, hd) * 2;
+  const int blocks = rotary_blocks(total, 2 * sm_count());
   return rot::by_type(dtype, [&](auto t) {
     using E = decltype(t);
     if (hd == 32) return rot::fwd<E, 32>(x, gq, gk, y, total, ldx, ldy, a, blocks, st);

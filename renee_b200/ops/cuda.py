@@ -454,7 +454,7 @@ def qk_norm_rotary_bwd(at, dy, x, table, S, nh, hd, eps, ws, dx, positions):
     T = x.shape[0]
     _call_typed("rb_qk_norm_rotary_bwd", x.device, DT[x.dtype], dy.data_ptr(), _ld(dy), x_, _ld(x), gq, gk, table_,
                 None if positions is None else positions.data_ptr(), ws.data_ptr(), dx_, _ld(dx), dgq, dgk, T, table.shape[0], S, nh, hd, eps,
-                launches=3 if T else 2)
+                launches=2 if T else 1)
 
 
 def relative_tiles(S: int) -> int:

@@ -351,7 +351,7 @@ def _check_gelu8(saved, **like_x):
         _whole(name, t, (T, F), x.dtype)
     _whole("saved.q", saved.q, (T, F), torch.int8)
     _whole("saved.scale", saved.scale, (T, -(-F // GELU8_BLOCK)), torch.float32)
-    _refuse(T >= 2 ** 30 or T * F >= 2 ** 38, f"{T} rows of {F} are too many for one call")
+    _refuse(T >= 2 ** 30 or F >= 2 ** 30, f"{T} rows of {F} are too many for one call")
     _same_place(x, **{"saved.q": saved.q, "saved.scale": saved.scale}, **like_x)
     return T, F
 
