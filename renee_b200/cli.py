@@ -55,6 +55,13 @@ def build_parser() -> argparse.ArgumentParser:
     # ---- extensions
     p.add_argument("--pooling", choices=["mean", "cls"], default="mean")
     p.add_argument("--encoder-dtype", choices=["bf16", "fp16"], default="bf16")
+    p.add_argument("--rotary", action="store_true", default=False,
+                   help="norms of queries and keys for each head, rotated by position (new parameters: train from scratch or fine-tune)")
+    p.add_argument("--relative-buckets", type=int, default=0, metavar="N",
+                   help="learned bias of the attention scores by N buckets of distance (0: none)")
+    p.add_argument("--relative-max-distance", type=int, default=128, metavar="N")
+    p.add_argument("--gelu8", action="store_true", default=False,
+                   help="the feed-forward blocks keep their pre-activations in 8 bits between the passes")
     p.add_argument("--encoder-weights", type=str, default="", help="state_dict (.pt) with HF DistilBERT keys")
     p.add_argument("--synthetic-labels", type=int, default=0, help="generate a synthetic workload with this many labels")
     p.add_argument("--synthetic-train", type=int, default=4096)
@@ -103,11 +110,23 @@ def _load_data(args, rank: int):
     return trn, tst, labels.shape[1], tlabels, filt, inv_prop, dataset_name
 
 
+def _encoder_config(args):
+    """The architecture of ``--tf`` with the relative positions and the 8-bit feed-forward blocks that were asked for.  A relative
+    encoder may read texts beyond the position table of its preset: the table grows to ``--maxlen``."""
+    import dataclasses
+    from .models.encoder import config_from_name
+    cfg = config_from_name(args.tf)
+    relative = args.rotary or args.relative_buckets > 0
+    return dataclasses.replace(cfg, rotary=args.rotary, relative_buckets=args.relative_buckets, gelu8=args.gelu8,
+                               relative_max_distance=args.relative_max_distance,
+                               max_position_embeddings=max(cfg.max_position_embeddings, args.maxlen if relative else 0))
+
+
 def start(local_device: int, ngpus_per_node: int, args) -> None:
     """Per-process entry (the reference's ``start``, main.py:20-186)."""
     from .data.collate import GlobalBatchSampler, PrefetchLoader, XCCollator
     from .evaluate import FullPredictor, PrecEvaluator
-    from .models.encoder import config_from_name, strip_ngame_prefix
+    from .models.encoder import strip_ngame_prefix
     from .parallel.dist import env_world, init_distributed, shutdown
     from .train import TrainConfig, XCTrainer, seed_everything
     from .utils.sharding import shard_labels
@@ -140,7 +159,7 @@ def start(local_device: int, ngpus_per_node: int, args) -> None:
                                 XCCollator(sharding, tst, rank, args.accum, xfcz, False, False),
                                 pin=ctx.device.type == "cuda")
 
-    enc_cfg = config_from_name(args.tf)
+    enc_cfg = _encoder_config(args)
     cfg = TrainConfig.from_args(args)
     cfg.out_dir = os.path.join(args.results_dir, dataset_name, args.expname)
     comm = None
@@ -172,7 +191,7 @@ def start(local_device: int, ngpus_per_node: int, args) -> None:
         init_sd = convert_bert_state_dict(init_sd, roberta="roberta" in args.tf.lower())   # BERT / RoBERTa / MiniLM keys
     if init_sd is not None:
         if args.default_impl:
-            trainer.model.embed[0].transformer.load_state_dict(init_sd, strict=True)
+            trainer.model.embed[0].transformer.load_state_dict(init_sd, strict=not (args.rotary or args.relative_buckets))
         else:
             trainer.encoder.load_encoder_state_dict(init_sd, strict=True)
 

@@ -12,7 +12,9 @@ attention mask.  This module is an own implementation of the same architecture s
 
 Architecture (checked against transformers' DistilBERT): word + learned position embeddings →
 LayerNorm(eps 1e-12) → dropout; each block ``h = LN(x + drop(out_lin(attn(x))))`` then
-``LN(h + drop(lin2(gelu(lin1(h)))))``; exact-erf GELU; no token types, no pooler.
+``LN(h + drop(lin2(gelu(lin1(h)))))``; exact-erf GELU; no token types, no pooler.  Without a counterpart in the reference,
+an encoder may also know relative positions: queries and keys normalised for each head and rotated by their position
+(``rotary``), and a bias of the scores by buckets of the distance (``relative_buckets``).
 """
 from __future__ import annotations
 
@@ -38,6 +40,12 @@ class EncoderConfig:
     initializer_range: float = 0.02
     pad_token_id: int = 0
     attn_output_dropout: float = 0.0   # BERT/RoBERTa drop the attention output projection; DistilBERT does not
+    rotary: bool = False               # RMS norm of every head's queries and keys (learned gains), rotated by position
+    rotary_base: float = 10000.0
+    rotary_eps: float = 1e-6
+    relative_buckets: int = 0          # learned bias of the scores by buckets of key - query, one table per layer; 0 = none
+    relative_max_distance: int = 128
+    gelu8: bool = False                # engine only: the FFN keeps its pre-activation in 8 bits and makes its activation again
 
     @property
     def hidden_size(self) -> int:  # HF alias used by the reference (main.py:149,152)
@@ -95,6 +103,14 @@ class Embeddings(nn.Module):
         return self.dropout(self.LayerNorm(x))
 
 
+class HeadGain(nn.Module):
+    """The learned gain of a head's norm (its parameter only; :mod:`renee_b200.ops` computes the norm)."""
+
+    def __init__(self, hd: int):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(hd))
+
+
 class SelfAttention(nn.Module):
     def __init__(self, cfg: EncoderConfig):
         super().__init__()
@@ -105,6 +121,18 @@ class SelfAttention(nn.Module):
         self.k_lin = nn.Linear(cfg.dim, cfg.dim)
         self.v_lin = nn.Linear(cfg.dim, cfg.dim)
         self.out_lin = nn.Linear(cfg.dim, cfg.dim)
+        self.rotary, self.rotary_base, self.rotary_eps = cfg.rotary, cfg.rotary_base, cfg.rotary_eps
+        if cfg.rotary:
+            self.q_norm, self.k_norm = (HeadGain(cfg.dim // cfg.n_heads) for _ in range(2))
+        self.relative_max_distance = cfg.relative_max_distance if cfg.relative_buckets else 0
+        if cfg.relative_buckets:
+            self.relative_bias = nn.Embedding(cfg.relative_buckets, cfg.n_heads)
+
+    def _bias(self, S: int, device) -> torch.Tensor:
+        from ..ops import relative_buckets
+        far, at = self.relative_max_distance, torch.arange(S, device=device)
+        bucket = relative_buckets(self.relative_bias.num_embeddings, far, device).long()
+        return self.relative_bias(bucket[(at[None, :] - at[:, None]).clamp(-far, far) + far]).permute(2, 0, 1)
 
     def forward(self, x: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
         b, S, _ = x.shape
@@ -113,8 +141,16 @@ class SelfAttention(nn.Module):
         def split(t):
             return t.view(b, S, self.n_heads, hd).transpose(1, 2)
 
-        q, k, v = split(self.q_lin(x)), split(self.k_lin(x)), split(self.v_lin(x))
+        q, k, v = self.q_lin(x), self.k_lin(x), split(self.v_lin(x))
+        if self.rotary:
+            from ..ops import reference, rotary_table
+            table = rotary_table(S, hd, self.rotary_base, x.device).to(x.dtype)
+            q, k = reference.qk_norm_rotary_fwd(torch.cat([q, k], -1).view(b * S, 2 * self.dim), self.q_norm.weight, self.k_norm.weight, table, S,
+                                                self.n_heads, self.rotary_eps).view(b, S, 2 * self.dim).chunk(2, -1)
+        q, k = split(q), split(k)
         scores = torch.matmul(q, k.transpose(-1, -2)) / math.sqrt(hd)
+        if self.relative_max_distance:
+            scores = scores + self._bias(S, x.device).to(scores.dtype)
         scores = scores.masked_fill(mask[:, None, None, :] == 0, torch.finfo(scores.dtype).min)
         w = F.dropout(torch.softmax(scores, dim=-1), self.p, self.training)
         ctx = torch.matmul(w, v).transpose(1, 2).reshape(b, S, self.dim)

@@ -24,7 +24,10 @@ so this engine is built for CUDA-graph capture instead:
 * with CLS pooling on that path the last layer goes on with first tokens only behind its attention (``_first_tokens``), as do
   their gradients up to it: training steps of 256 x 32 tokens 2.58 -> 2.46 ms, 128 x 128 4.60 -> 4.26, 512 x 32 with 1.3 M
   labels 7.83 -> 7.54; evaluation of 256 x 32 tokens 695 -> 664 us;
-* dropout masks are recomputed from a counter-based RNG in the backward pass.
+* dropout masks are recomputed from a counter-based RNG in the backward pass;
+* encoders with relative positions (``EncoderConfig.rotary``, ``relative_buckets``) or an FFN that keeps 8 bits (``gelu8``) take the
+  kernels of :mod:`renee_b200.ops.relative`, with library GEMMs over all tokens (the packed rows and fused epilogues of the own
+  GEMMs do not know them).
 
 State-dict keys are those of HF DistilBERT (see :mod:`renee_b200.models.encoder`).
 """
@@ -100,6 +103,10 @@ class FlatEncoder:
                       (p + "ffn.lin1.weight", (Fd, H)), (p + "ffn.lin1.bias", (Fd,)),
                       (p + "ffn.lin2.weight", (H, Fd)), (p + "ffn.lin2.bias", (H,)),
                       (p + "output_layer_norm.weight", (H,)), (p + "output_layer_norm.bias", (H,))]
+            if cfg.rotary:
+                names += [(p + "attention.q_norm.weight", (H // cfg.n_heads,)), (p + "attention.k_norm.weight", (H // cfg.n_heads,))]
+            if cfg.relative_buckets:
+                names += [(p + "attention.relative_bias.weight", (cfg.relative_buckets, cfg.n_heads))]
         self.encoder_param_names = [n for n, _ in names]
         if self.bottleneck_dims > 0:
             names.append(("__bottleneck__.transformer_weight", (self.bottleneck_dims, H)))
@@ -109,8 +116,8 @@ class FlatEncoder:
         # contiguous range whose gradients are final as soon as the backward pass leaves the layer, while every
         # vector-shaped gradient (LayerNorm, biases: converted by one launch at the end of the pass) sits in the
         # tail of the buffer — which is what lets the gradient reduction start layer by layer under the backward pass
-        ln_w = [(n, s) for n, s in decay if n.endswith("layer_norm.weight")]
-        decay = [(n, s) for n, s in decay if not n.endswith("layer_norm.weight") and not n.startswith("__bottleneck__")] \
+        ln_w = [(n, s) for n, s in decay if n.endswith("_norm.weight")]
+        decay = [(n, s) for n, s in decay if not n.endswith("_norm.weight") and not n.startswith("__bottleneck__")] \
             + ln_w + [(n, s) for n, s in decay if n.startswith("__bottleneck__")]
         self.slots: dict[str, _Slot] = {}
         off = 0
@@ -128,6 +135,16 @@ class FlatEncoder:
         if H % ALIGN != 0:
             raise ValueError(f"hidden size must be a multiple of {ALIGN}")
         dev = self.device
+        self.relative = cfg.rotary or cfg.relative_buckets > 0
+        if self.relative:
+            if dev.type != "cpu" and act_dtype == torch.float32:
+                raise ValueError("relative positions need 16-bit activations on a GPU")
+            hd = H // cfg.n_heads
+            self._rotary_table = ops.rotary_table(cfg.max_position_embeddings, hd, cfg.rotary_base, dev) if cfg.rotary else None
+            # rotation without a bias: one bucket whose bias is and stays zero
+            self._buckets = ops.relative_buckets(cfg.relative_buckets, cfg.relative_max_distance, dev) if cfg.relative_buckets else \
+                torch.zeros(1, dtype=torch.int32, device=dev)
+            self._no_bias = None if cfg.relative_buckets else guard.zeros(1, cfg.n_heads, dtype=act_dtype, device=dev, name="encoder.no_bias")
         self.p32 = guard.zeros(off, dtype=torch.float32, device=dev, name="encoder.p32")
         if act_dtype == torch.float32:
             self.p16 = self.p32
@@ -162,7 +179,7 @@ class FlatEncoder:
             # RENEE_B200_OWN_GEMM: 1 = the own tcgen05 GEMMs with fused epilogues always, 0 = library GEMMs + separate
             # element-wise kernels, auto (default) = own from OWN_GEMM_MIN_TOKENS tokens per step and GPU upwards
             self._own_mode = os.environ.get("RENEE_B200_OWN_GEMM", "auto")
-            self._own_supported = cu.enc_gemm_supported(self.p16, H, Fd)
+            self._own_supported = cu.enc_gemm_supported(self.p16, H, Fd) and not (self.relative or cfg.gelu8)
             self.own_gemm = self._own_supported and self._own_mode != "auto"
             if self._own_supported and self.device.type == "cuda" and os.environ.get("RENEE_B200_WGRAD_STREAM", "1") != "0":
                 # weight gradients are off the critical path of the backward pass (nothing reads them before the
@@ -186,7 +203,7 @@ class FlatEncoder:
         g = torch.Generator(device="cpu").manual_seed(int(seed))
         std = self.cfg.initializer_range
         for n, s in self.slots.items():
-            if n.endswith("LayerNorm.weight") or n.endswith("layer_norm.weight"):
+            if n.endswith("LayerNorm.weight") or n.endswith("_norm.weight"):
                 t = torch.ones(s.shape)
             elif n.endswith("bias"):
                 t = torch.zeros(s.shape)
@@ -208,7 +225,9 @@ class FlatEncoder:
         return {n: self.view(self.p32, n).detach().clone() for n in self.encoder_param_names}
 
     def load_encoder_state_dict(self, sd: dict, strict: bool = True) -> None:
-        missing = [n for n in self.encoder_param_names if n not in sd]
+        # weights of an encoder without relative positions can be loaded: its new parameters keep their first values
+        new = ("attention.q_norm.weight", "attention.k_norm.weight", "attention.relative_bias.weight")
+        missing = [n for n in self.encoder_param_names if n not in sd and not n.endswith(new)]
         if strict and missing:
             raise KeyError(f"missing encoder keys: {missing[:4]} ...")
         for n in self.encoder_param_names:
@@ -229,13 +248,20 @@ class FlatEncoder:
         e = lambda *shape, dtype=dt: guard.empty(*shape, dtype=dtype, device=dev, name=f"encoder.act{guard.registered()}")
         layers = []
         # long sequences: one softmax-gradient scratch serves every layer (it lives within one attention backward)
-        att_ds = ops.attention_ds(b, S, nh, dev, dt)
+        att_ds = None if self.relative else ops.attention_ds(b, S, nh, dev, dt)
+        att = None
+        ffn = dict(f1=e(T, Fd), a1=e(T, Fd)) if cfg.gelu8 else None      # 8 bits: one pre-activation and activation for all layers
         for _ in range(cfg.n_layers):
+            if self.relative:      # the backward scratch, too, lives within one call
+                att = ops.relative_attention_workspace(b, S, nh, H // nh, cfg.relative_max_distance if cfg.relative_buckets else 0, dt, dev, scratch=att)
+            else:
+                att = ops.attention_workspace(b, S, nh, dev, dt, ds=att_ds)
             layers.append(dict(qkv=e(T, 3 * H), ctx=e(T, H), ao=e(T, H), pre1=e(T, H), h1=e(T, H),
                                mean1=e(T, dtype=torch.float32), rstd1=e(T, dtype=torch.float32),
-                               f1=e(T, Fd), a1=e(T, Fd), f2=e(T, H), pre2=e(T, H), h2=e(T, H),
-                               mean2=e(T, dtype=torch.float32), rstd2=e(T, dtype=torch.float32),
-                               att=ops.attention_workspace(b, S, nh, dev, dt, ds=att_ds)))
+                               **(ffn or dict(f1=e(T, Fd), a1=e(T, Fd))), f2=e(T, H), pre2=e(T, H), h2=e(T, H),
+                               mean2=e(T, dtype=torch.float32), rstd2=e(T, dtype=torch.float32), att=att,
+                               **(dict(qk=e(T, 2 * H)) if cfg.rotary else {}),
+                               **(dict(f8=ops.gelu8_saved(T, Fd, dev)) if cfg.gelu8 else {})))
         self._acts = dict(h0=e(T, H), mean0=e(T, dtype=torch.float32), rstd0=e(T, dtype=torch.float32),
                           layers=layers, pooled=e(b, H, dtype=torch.float32),
                           dh=e(T, H), dctx=e(T, H), att_ds=att_ds,
@@ -315,10 +341,14 @@ class FlatEncoder:
             pre = f"transformer.layer.{l}."
             sb = 8 * (l + 1)
             qkv = L["qkv"][:T]
-            torch.mm(h, self._qkv(P, l, "weight").t(), out=qkv)
             ctx = L["ctx"][:T]
-            ops.attention_fwd(qkv, self._qkv(P, l, "bias"), attention_mask, cfg.n_heads, pa, rng, sb + _S_PROBS,
-                              ctx, L["att"])
+            if self.relative:
+                torch.addmm(self._qkv(P, l, "bias"), h, self._qkv(P, l, "weight").t(), out=qkv)
+                self._relative_attention(l, L, qkv, attention_mask, pa, rng, sb + _S_PROBS, ctx)
+            else:
+                torch.mm(h, self._qkv(P, l, "weight").t(), out=qkv)
+                ops.attention_fwd(qkv, self._qkv(P, l, "bias"), attention_mask, cfg.n_heads, pa, rng, sb + _S_PROBS,
+                                  ctx, L["att"])
             ao = L["ao"][:T]
             torch.mm(ctx, self.view(P, pre + "attention.out_lin.weight").t(), out=ao)
             h1 = L["h1"][:T]
@@ -330,7 +360,10 @@ class FlatEncoder:
             f1 = L["f1"][:T]
             torch.mm(h1, self.view(P, pre + "ffn.lin1.weight").t(), out=f1)
             a1 = L["a1"][:T]
-            ops.bias_gelu_fwd(f1, self.view(P, pre + "ffn.lin1.bias"), a1)
+            if cfg.gelu8:
+                ops.gelu8_fwd(f1, self.view(P, pre + "ffn.lin1.bias"), a1, L["f8"][:T])
+            else:
+                ops.bias_gelu_fwd(f1, self.view(P, pre + "ffn.lin1.bias"), a1)
             f2 = L["f2"][:T]
             torch.mm(a1, self.view(P, pre + "ffn.lin2.weight").t(), out=f2)
             h2 = L["h2"][:T]
@@ -351,6 +384,38 @@ class FlatEncoder:
             torch.mm(pooled, self.bottleneck_weight().t(), out=emb)   # fp32, master weights
             return emb
         return pooled
+
+    def _relative_parts(self, l: int, L: dict, qkv):
+        """(queries, keys, values, table) of a layer with relative positions: views of its buffers."""
+        H = self.cfg.dim
+        qk = L["qk"][:qkv.shape[0]] if self.cfg.rotary else qkv
+        table = self._no_bias if self._no_bias is not None else self.view(self.p16, f"transformer.layer.{l}.attention.relative_bias.weight")
+        return qk[:, :H], qk[:, H:2 * H], qkv[:, 2 * H:], table
+
+    def _rotary_args(self, l: int, x):
+        pre, cfg = f"transformer.layer.{l}.attention.", self.cfg
+        return (x, self.view(self.p16, pre + "q_norm.weight"), self.view(self.p16, pre + "k_norm.weight"), self._rotary_table)
+
+    def _relative_attention(self, l: int, L: dict, qkv, mask, p: float, rng, stream: int, ctx) -> None:
+        """Attention of a layer with relative positions; ``qkv`` holds the biased projections."""
+        cfg, H = self.cfg, self.cfg.dim
+        if cfg.rotary:
+            ops.qk_norm_rotary_fwd(*self._rotary_args(l, qkv[:, :2 * H]), mask.shape[1], cfg.n_heads, cfg.rotary_eps, L["qk"][:qkv.shape[0]])
+        q, k, v, table = self._relative_parts(l, L, qkv)
+        ops.relative_attention_fwd(q, k, v, mask, table, self._buckets, cfg.n_heads, p, rng, stream, ctx, L["att"])
+
+    def _relative_attention_bwd(self, l: int, L: dict, dctx, qkv, mask, p: float, rng, stream: int, buf: dict, dqkv, dbqkv) -> None:
+        cfg, H, T = self.cfg, self.cfg.dim, qkv.shape[0]
+        q, k, v, table = self._relative_parts(l, L, qkv)
+        dqk = buf["dqk"][:T] if cfg.rotary else dqkv
+        dtable = buf["dtable"] if self._no_bias is not None else self.view(self.g, f"transformer.layer.{l}.attention.relative_bias.weight")
+        ops.relative_attention_bwd(dctx, q, k, v, mask, table, self._buckets, cfg.n_heads, p, rng, stream, L["ctx"][:T], L["att"],
+                                   dqk[:, :H], dqk[:, H:2 * H], dqkv[:, 2 * H:], dtable)
+        if cfg.rotary:
+            pre = f"transformer.layer.{l}.attention."
+            ops.qk_norm_rotary_bwd(dqk, *self._rotary_args(l, qkv[:, :2 * H]), mask.shape[1], cfg.n_heads, cfg.rotary_eps, buf["rotary"],
+                                   dqkv[:, :2 * H], self.view(self.g, pre + "q_norm.weight"), self.view(self.g, pre + "k_norm.weight"))
+        ops.colsum(dqkv, dbqkv)
 
     def _forward_layers_fused(self, h, attention_mask, T, pd, pa, po, rng, packed, first):
         """The transformer blocks on the own GEMMs: 4 GEMMs, 1 attention and 2 LayerNorm launches per layer.  With a
@@ -473,12 +538,17 @@ class FlatEncoder:
                 pd, rng, sb + _S_FFN,
                 self.view(G, pre + "output_layer_norm.weight"), self.view(G, pre + "output_layer_norm.bias"),
                 self.view(G, pre + "ffn.lin2.bias"), buf["dh_b"][:T], L["f2"][:T])
-            torch.mm(d_f2.t(), L["a1"][:T], out=self.view(G, pre + "ffn.lin2.weight"))
             da1 = buf["da1"][:T]
-            torch.mm(d_f2, self.view(P, pre + "ffn.lin2.weight"), out=da1)
             df1 = buf["df1"][:T]
-            ops.bias_gelu_bwd(da1, L["f1"][:T], self.view(P, pre + "ffn.lin1.bias"),
-                              self.view(G, pre + "ffn.lin1.bias"), df1)
+            if cfg.gelu8:          # makes the activation again, which the weight gradient reads
+                torch.mm(d_f2, self.view(P, pre + "ffn.lin2.weight"), out=da1)
+                ops.gelu8_bwd(da1, L["f8"][:T], buf["gelu8"], self.view(G, pre + "ffn.lin1.bias"), df1, L["a1"][:T])
+                torch.mm(d_f2.t(), L["a1"][:T], out=self.view(G, pre + "ffn.lin2.weight"))
+            else:
+                torch.mm(d_f2.t(), L["a1"][:T], out=self.view(G, pre + "ffn.lin2.weight"))
+                torch.mm(d_f2, self.view(P, pre + "ffn.lin2.weight"), out=da1)
+                ops.bias_gelu_bwd(da1, L["f1"][:T], self.view(P, pre + "ffn.lin1.bias"),
+                                  self.view(G, pre + "ffn.lin1.bias"), df1)
             torch.mm(df1.t(), L["h1"][:T], out=self.view(G, pre + "ffn.lin1.weight"))
             # dh1 = d_pre2 (residual) + df1 @ W1
             dh1 = d_pre2.addmm_(df1, self.view(P, pre + "ffn.lin1.weight"))      # in place: no copy of the addend
@@ -492,8 +562,11 @@ class FlatEncoder:
             dctx = A["dctx"][:T]
             torch.mm(d_ao, self.view(P, pre + "attention.out_lin.weight"), out=dctx)
             dqkv = buf["dqkv"][:T]
-            ops.attention_bwd(dctx, L["qkv"][:T], self._qkv(P, l, "bias"), mask, cfg.n_heads, pa, rng,
-                              sb + _S_PROBS, L["att"], dqkv, self._qkv(G, l, "bias"))
+            if self.relative:
+                self._relative_attention_bwd(l, L, dctx, L["qkv"][:T], mask, pa, rng, sb + _S_PROBS, buf, dqkv, self._qkv(G, l, "bias"))
+            else:
+                ops.attention_bwd(dctx, L["qkv"][:T], self._qkv(P, l, "bias"), mask, cfg.n_heads, pa, rng,
+                                  sb + _S_PROBS, L["att"], dqkv, self._qkv(G, l, "bias"))
             torch.mm(dqkv.t(), h_in, out=self._qkv(G, l, "weight"))
             d_pre1.addmm_(dqkv, self._qkv(P, l, "weight"))                       # d_pre1 is dh
             if on_layer_done is not None:
@@ -517,12 +590,19 @@ class FlatEncoder:
             return
         (b, S), H, Fd = self._acts_key, self.cfg.dim, self.cfg.hidden_dim
         widths = (("dpre2", H), ("dpre1", H), ("df1", Fd), ("dqkv", 3 * H)) if self.own_gemm else \
-            (("dh_b", H), ("dqkv", 3 * H), ("df1", Fd), ("da1", Fd))
+            (("dh_b", H), ("dqkv", 3 * H), ("df1", Fd), ("da1", Fd), *((("dqk", 2 * H),) if self.cfg.rotary else ()))
         sets = 2 if self.own_gemm else 1
         sizes = [b * S * n for _, n in widths] * sets
         flat = guard.empty(sum(sizes), dtype=self.act_dtype, device=self.device, name="encoder.activations.bwd").split(sizes)
         self._acts[which] = [{k: flat[len(widths) * i + j].view(b * S, n) for j, (k, n) in enumerate(widths)}
                              for i in range(sets)]
+        cfg, lib = self.cfg, self._acts["lib"][0] if which == "lib" else {}
+        if which == "lib" and cfg.rotary:
+            lib["rotary"] = ops.qk_norm_rotary_workspace(b * S, cfg.n_heads, H // cfg.n_heads, self.device)
+        if which == "lib" and self.relative and self._no_bias is not None:
+            lib["dtable"] = torch.empty_like(self._no_bias)
+        if which == "lib" and cfg.gelu8:
+            lib["gelu8"] = ops.gelu8_workspace(b * S, Fd, self.device)
         if self.own_gemm and self._wgrad_group is None:
             from ..ops import cuda as cu
             self._wgrad_group = cu.WgradGroup([(3 * H, H), (H, H), (Fd, H), (H, Fd), (3 * H, H)], self.device)

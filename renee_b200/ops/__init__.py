@@ -144,6 +144,12 @@ def bias_gelu_bwd(da, x, bias, dbias, dx_out):
     dx_out.copy_(ref.bias_gelu_bwd(da, x, bias, dbias))
 
 
+def colsum(x, out):
+    if _is_cuda(x):
+        return _cuda().colsum(x, out)
+    ref.colsum(x, out)
+
+
 def pool_fwd(h, mask, mode, out, **packed):
     if _is_cuda(h):
         return _cuda().pool_fwd(h, mask, mode, out, **packed)

@@ -138,45 +138,20 @@ template <int COLS> __device__ __forceinline__ void finish(const uint32_t* s_tme
   if (warp == WORKERS) tc::tmem_dealloc(*s_tmem, COLS);
 }
 
-// Waits, bounded by the SM's clock (1.5 s at 2 GHz).  Once one has run out, all later ones return at once; whoever goes on then works
-// on what is there, so that he comes to all meetings, and the status word says that the results are void.
-constexpr long long WAIT_CLOCKS = 3000000000LL;
+// Bounded waits (tc.cuh).  Once one has run out, all later ones return at once; whoever goes on then works on what is there, so that he
+// comes to all meetings, and the status word says that the results are void.
 struct Waiter {
   bool aborted;
   int* status;
-  __device__ __forceinline__ void note(int site, uint32_t phase) {
-    aborted = true;
-    if (status != nullptr && atomicCAS(status, 0, 1000 + site) == 0) {
-      status[1] = (int)blockIdx.x;
-      status[2] = site;
-      status[3] = (int)phase;
-    }
-  }
   // one thread
   __device__ __forceinline__ bool one(uint64_t* bar, uint32_t phase, int site) {
-    if (aborted) return false;
-    if (tc::mbar_try_wait(bar, phase & 1)) return true;
-    const long long t0 = clock64();
-    do {
-#pragma unroll 1
-      for (int i = 0; i < 64; ++i)
-        if (tc::mbar_try_wait(bar, phase & 1)) return true;
-    } while (clock64() - t0 < WAIT_CLOCKS);
-    note(site, phase);
-    return false;
+    return tc::mbar_wait(bar, phase & 1, aborted, status, site, (int)phase);
   }
   // a whole warp, with the same answer in every lane
   __device__ __forceinline__ bool all(uint64_t* bar, uint32_t phase, int site) {
-    if (aborted) return false;
-    if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, phase & 1))) return true;
-    const long long t0 = clock64();
-    do {
-#pragma unroll 1
-      for (int i = 0; i < 64; ++i)
-        if (__all_sync(0xffffffffu, tc::mbar_try_wait(bar, phase & 1))) return true;
-    } while (__any_sync(0xffffffffu, clock64() - t0 < WAIT_CLOCKS));
-    note(site, phase);
-    return false;
+    tc::mbar_wait(bar, phase & 1, aborted, status, site, (int)phase);
+    aborted = __any_sync(0xffffffffu, aborted);
+    return !aborted;
   }
 };
 // One arrival for a warp whose TMEM accesses before it are complete
