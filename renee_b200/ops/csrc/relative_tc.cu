@@ -103,7 +103,7 @@ template <typename T> __device__ __forceinline__ void store_row(T* out, const fl
 // in turn); freed: nothing reads a tile's rows any more; end: its accumulators are complete; taken: they have been read (tiles in
 // turn).  A barrier that somebody may come late to is doubled: its next phase cannot then pass him by.
 constexpr int MAX_STAGES = 4, WORKERS = 8;
-struct Bars { uint64_t own[2], raw[MAX_STAGES], full[MAX_STAGES], empty[MAX_STAGES], scores[2], read, done[2], freed, end, taken[2]; };
+struct Bars { uint64_t own[2], raw[MAX_STAGES], full[MAX_STAGES], empty[MAX_STAGES], scores[3], read, done[3], freed, end, taken[2]; };
 
 __device__ __forceinline__ char* align1k(char* p) { return p + ((1024u - (tc::smem_u32(p) & 1023u)) & 1023u); }
 
@@ -112,9 +112,11 @@ template <int COLS> __device__ __forceinline__ void start(Bars* bars, uint32_t* 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(bars->own + i, 1);
+      tc::mbar_init(bars->taken + i, WORKERS);
+    }
+    for (int i = 0; i < 3; ++i) {
       tc::mbar_init(bars->scores + i, 1);
       tc::mbar_init(bars->done + i, WORKERS);
-      tc::mbar_init(bars->taken + i, WORKERS);
     }
     for (int i = 0; i < MAX_STAGES; ++i) {
       tc::mbar_init(bars->raw + i, 1);
@@ -263,48 +265,55 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
 }
 
 // The MMA thread of fwd and bwd_q.  scores(g, s), rows(g, s, first): the products of block g, in stage s.
-// TURNS: scores have two buffers, which P shares: one is free when the product before last is complete.  Otherwise they have one,
-// free as soon as the scores are in registers, and dS has two places of its own.
-template <int NST, bool TURNS, typename T, typename Scores, typename Rows>
+// TURNS > 0: scores have that many buffers, which P shares: one is free when the product TURNS blocks back is complete, and scores are
+// issued TURNS - 1 blocks before the second product waits for its P.  TURNS = 0: scores have one buffer, free as soon as they are in
+// registers, and dS has two places of its own.
+template <int NST, int TURNS, typename T, typename Scores, typename Rows>
 __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, Scores scores, Rows rows) {
-  unsigned g = 0, k = 0;
-  // the second product of block x: first / last of its tile, the CTA's j-th
-  const auto second = [&](unsigned x, bool first, bool last, unsigned j) {
-    wait.one(bars.done + (x & 1), x >> 1, tc::SITE_TMEM_EMPTY);
-    if (first && j > 0) wait.one(bars.taken + ((j - 1) & 1), (j - 1) >> 1, tc::SITE_TMEM_EMPTY);
+  constexpr unsigned SLOTS = TURNS ? TURNS : 2, AHEAD = TURNS ? TURNS - 1 : 1;
+  unsigned g = 0, k = 0, x = 0;                                // blocks begun, tiles begun, second products issued
+  unsigned jx = 0, ix = 0, nx = 0, n_last = 0;                 // block x: the ix-th of nx of the CTA's jx-th tile
+  const auto second = [&]() {
+    wait.one(bars.done + x % SLOTS, x / SLOTS, tc::SITE_TMEM_EMPTY);
+    if (ix == 0 && jx > 0) wait.one(bars.taken + ((jx - 1) & 1), (jx - 1) >> 1, tc::SITE_TMEM_EMPTY);
     if (wait.aborted) return;
     tc::tc_fence_after();
-    rows(x, x % NST, first);
+    rows(x, x % NST, ix == 0);
     tc::umma_commit(bars.empty + x % NST);
-    if (last) tc::umma_commit(&bars.end);
+    ++x;
+    if (++ix == nx) {
+      tc::umma_commit(&bars.end);
+      ix = 0;
+      ++jx;
+    }
   };
-  int n_last = 0;
   for (int t = blockIdx.x; t < tiles && !wait.aborted; t += gridDim.x, ++k) {
-    const int n = key_blocks(a, t / per / a.nh);
-    for (int i = 0; i < n && !wait.aborted; ++i, ++g) {
+    const unsigned n = key_blocks(a, t / per / a.nh);
+    nx = n_last;
+    while (x < g && !wait.aborted) second();                   // the last tile's end before this one's rows are waited for
+    nx = n_last = n;
+    for (unsigned i = 0; i < n && !wait.aborted; ++i, ++g) {
       if (TURNS) {
-        if (g > 1) wait.one(bars.empty + (g - 2) % NST, (g - 2) / NST, tc::SITE_EMPTY);
+        if (g >= SLOTS) wait.one(bars.empty + (g - SLOTS) % NST, (g - SLOTS) / NST, tc::SITE_EMPTY);
       } else {
         if (g > 0) wait.one(&bars.read, g - 1, tc::SITE_TMEM_EMPTY);
       }
-      if (i == 0 && g > 0) second(g - 1, n_last == 1, true, k - 1);      // the last tile's end before this one's rows are waited for
       if (i == 0) wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
       if (wait.aborted) return;
       tc::tc_fence_after();
       scores(g, g % NST);
-      tc::umma_commit(bars.scores + (g & 1));
+      tc::umma_commit(bars.scores + g % SLOTS);
       if (TURNS && i + 1 == n) tc::umma_commit(&bars.freed);
-      if (i > 0) second(g - 1, i == 1, false, k);
+      if (g >= x + AHEAD) second();
     }
-    n_last = n;
   }
-  if (g > 0) second(g - 1, n_last == 1, true, k - 1);
+  while (x < g && !wait.aborted) second();
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// TMEM: two buffers of 64 columns for the scores of blocks in turn (P in columns 0-15 and 32-47, each warp's over its own), O from
-// 128.  The next block's scores are there when a block's P is written, so the warps never wait for a product.
+// TMEM: three buffers of 64 columns (heads of 128: two) for the scores of blocks in turn (P in columns 0-15 and 32-47, each warp's over
+// its own), O behind them.  The next blocks' scores are there when a block's P is written, so the warps seldom wait for a product.
 //
 // The reference point m of a row's exponentials is the maximum of its first block with an attended key, and stays: P may grow to
 // 2^60 (bf16; its rounding is relative) or, from 2^6, to 2^15 (fp16) without harm.  Where a block's sum shows that a row left that
@@ -312,7 +321,7 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
 // its maximum, and the two warps meet once a block, to hear whether the other one left the range.
 template <typename T, int HD>
 __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
-  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4, COLS = 256;
+  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4, COLS = 256, TURNS = HD == 128 ? 2 : 3, O_COL = TURNS * BLK;
   constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
@@ -342,15 +351,15 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
         });
   } else if (warp > WORKERS) {
     if (tc::elect_one())
-      multiply_query_tiles<NST, true>(
+      multiply_query_tiles<NST, TURNS>(
           a, bars, wait, tiles, per,
-          [&](unsigned g, int s) { mma_scores<T, HD>(tmem + (g & 1) * BLK, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE)); },
+          [&](unsigned g, int s) { mma_scores<T, HD>(tmem + (g % TURNS) * BLK, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE)); },
           [&](unsigned g, int s, bool first) {
-            mma_rows<T, HDP>(tmem + 128, tmem + (g & 1) * BLK, 32, tc::smem_u32(stage + s * 2 * PIECE + PIECE), first);
+            mma_rows<T, HDP>(tmem + O_COL, tmem + (g % TURNS) * BLK, 32, tc::smem_u32(stage + s * 2 * PIECE + PIECE), first);
           });
   } else {
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_o = tmem + lanes + 128;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_o = tmem + lanes + O_COL;
     const float up = FP16 ? 6.f : 0.f, limit = FP16 ? 32768.f : 1.1529215e18f;
     const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
@@ -370,8 +379,8 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
         const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
         const float* wp = win + (k0 - q) + wd + PAD;
         const uint32_t on = bits[k0 >> 5];
-        const uint32_t row_s = tmem + lanes + (g & 1) * BLK + 32 * half;
-        wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
+        const uint32_t row_s = tmem + lanes + (g % TURNS) * BLK + 32 * half;
+        wait.all(bars.scores + g % TURNS, g / TURNS, tc::SITE_TMEM_FULL);
         tc::tc_fence_after();
         float s[32], sum;
         tc::tmem_ld32(row_s, s);
@@ -452,7 +461,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
         for (int j = 0; j < 16; ++j) r[j] = pack16<T>(s[2 * j], s[2 * j + 1]);
         tc::tmem_st16(row_s, r);
         tc::tmem_wait_st();
-        warp_arrive(bars.done + (g & 1), lane);
+        warp_arrive(bars.done + g % TURNS, lane);
       }
       s_row[1][half][row] = l;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
@@ -514,7 +523,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
         });
   } else if (warp > WORKERS) {
     if (tc::elect_one())
-      multiply_query_tiles<NST, false>(
+      multiply_query_tiles<NST, 0>(
           a, bars, wait, tiles, per,
           [&](unsigned, int s) {
             mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE));
