@@ -24,6 +24,15 @@ namespace rel {
 
 constexpr int ROWS = 128, BLK = 64;
 
+// Two values per instruction
+struct V2 { float2 v; };
+__device__ __forceinline__ V2 v2(float a, float b) { return V2{make_float2(a, b)}; }
+__device__ __forceinline__ V2 v2(float a) { return v2(a, a); }
+__device__ __forceinline__ void v2_get(V2 x, float& a, float& b) { a = x.v.x; b = x.v.y; }
+__device__ __forceinline__ V2 operator+(V2 a, V2 b) { return V2{__fadd2_rn(a.v, b.v)}; }
+__device__ __forceinline__ V2 operator*(V2 a, V2 b) { return V2{__fmul2_rn(a.v, b.v)}; }
+__device__ __forceinline__ V2 v2_fma(V2 a, V2 b, V2 c) { return V2{__ffma2_rn(a.v, b.v, c.v)}; }
+
 struct alignas(64) Maps { CUtensorMap a, b, c, d, e; };
 
 template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -174,18 +183,18 @@ template <typename T> __device__ __forceinline__ void load_window(const Args<T>&
 // 32 exponents in base 2: s scale + bias + c.  The bias comes from the window (wp), or is one number (far_piece; an empty sequence's
 // scores are zeros whatever q and k hold)
 __device__ __forceinline__ void exponents(float (&s)[32], float scale, bool empty, bool far_piece, float far_bias, const float* wp, float c) {
-  const F2 k = f2(scale);
+  const V2 k = v2(scale);
   if (empty) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) s[j] = c;
   } else if (far_piece) {
-    const F2 f = f2(far_bias + c);
+    const V2 f = v2(far_bias + c);
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), k, f), s[j], s[j + 1]);
+    for (int j = 0; j < 32; j += 2) v2_get(v2_fma(v2(s[j], s[j + 1]), k, f), s[j], s[j + 1]);
   } else {
-    const F2 f = f2(c);
+    const V2 f = v2(c);
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) f2_get(f2_fma(f2(s[j], s[j + 1]), k, f2(wp[j], wp[j + 1])) + f, s[j], s[j + 1]);
+    for (int j = 0; j < 32; j += 2) v2_get(v2_fma(v2(s[j], s[j + 1]), k, v2(wp[j], wp[j + 1])) + f, s[j], s[j + 1]);
   }
 }
 __device__ __forceinline__ void mask_columns(float (&s)[32], uint32_t on) {
@@ -398,17 +407,17 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
           asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
         }
         const auto exponentials = [&]() {
-          F2 l2[2] = {f2(0.f), f2(0.f)};
+          V2 l2[2] = {v2(0.f), v2(0.f)};
           exponents(s, a.scale_log2, empty, far_piece, far_bias, wp, m == -INFINITY ? 0.f : up - m);
           mask_columns(s, on);
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             s[j] = ex2(s[j]);
             s[j + 1] = ex2(s[j + 1]);
-            l2[(j >> 1) & 1] = l2[(j >> 1) & 1] + f2(s[j], s[j + 1]);
+            l2[(j >> 1) & 1] = l2[(j >> 1) & 1] + v2(s[j], s[j + 1]);
           }
           float x, y;
-          f2_get(l2[0] + l2[1], x, y);
+          v2_get(l2[0] + l2[1], x, y);
           sum = x + y;
         };
         exponentials();
@@ -558,8 +567,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       }
       s_sum[0][half][row] = d;
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const F2 nd = f2(-(s_sum[0][0][row] + s_sum[0][1][row]));
-      F2 sum = f2(0.f);
+      const V2 nd = v2(-(s_sum[0][0][row] + s_sum[0][1][row]));
+      V2 sum = v2(0.f);
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + half * 32;                  // of this warp's columns
         const int dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;
@@ -586,10 +595,10 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
         uint32_t r[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-          const F2 pr = f2(ex2(s[j]), ex2(s[j + 1])), v = f2(dp[j], dp[j + 1]);
+          const V2 pr = v2(ex2(s[j]), ex2(s[j + 1])), v = v2(dp[j], dp[j + 1]);
           float x, y;
-          sum = f2_fma(pr, v, sum);
-          f2_get(pr * (v + nd), x, y);
+          sum = v2_fma(pr, v, sum);
+          v2_get(pr * (v + nd), x, y);
           r[j / 2] = pack16<T>(x, y);
         }
         if (empty) {
@@ -601,7 +610,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
         warp_arrive(bars.done + (g & 1), lane);
       }
       float x, y;
-      f2_get(sum, x, y);
+      v2_get(sum, x, y);
       s_sum[1][half][row] = x + y;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (half == 0) {                                       // negative, as the keys' pass adds them; behind S nothing is left of P
@@ -792,7 +801,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         const float4* del = lse + BLK / 4;
         const float far_bias = !on ? -INFINITY : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
         const float* wp = on ? win + (key - q0) + wd + PAD : s_none + 31;
-        const F2 scale = f2(empty ? 0.f : a.scale_log2);
+        const V2 scale = v2(empty ? 0.f : a.scale_log2);
         if (empty) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) s[j] = 0.f;
@@ -801,25 +810,25 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
           const float4 L = lse[j / 4], D = del[j / 4];
-          const F2 ls[2] = {f2(L.x, L.y), f2(L.z, L.w)}, de[2] = {f2(D.x, D.y), f2(D.z, D.w)};
+          const V2 ls[2] = {v2(L.x, L.y), v2(L.z, L.w)}, de[2] = {v2(D.x, D.y), v2(D.z, D.w)};
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int c = j + 2 * e;
             float x, y;
-            f2_get(far_piece || empty ? f2_fma(f2(s[c], s[c + 1]), scale, ls[e] + f2(empty ? 0.f : far_bias))
-                                      : f2_fma(f2(s[c], s[c + 1]), scale, f2(wp[-c], wp[-c - 1])) + ls[e], x, y);
-            const F2 pr = f2(ex2(x), ex2(y));
-            F2 v = f2(dp[c], dp[c + 1]);
+            v2_get(far_piece || empty ? v2_fma(v2(s[c], s[c + 1]), scale, ls[e] + v2(empty ? 0.f : far_bias))
+                                      : v2_fma(v2(s[c], s[c + 1]), scale, v2(wp[-c], wp[-c - 1])) + ls[e], x, y);
+            const V2 pr = v2(ex2(x), ex2(y));
+            V2 v = v2(dp[c], dp[c + 1]);
             if (a.p > 0.f) {
               const uint32_t at0 = ((uint32_t)at.bh * a.S + q0 + c) * (uint32_t)a.S + key;
-              const F2 kf = f2(keep(seed, a.stream, at0, a.p) ? kept : 0.f, keep(seed, a.stream, at0 + (uint32_t)a.S, a.p) ? kept : 0.f);
+              const V2 kf = v2(keep(seed, a.stream, at0, a.p) ? kept : 0.f, keep(seed, a.stream, at0 + (uint32_t)a.S, a.p) ? kept : 0.f);
               v = v * kf;
-              f2_get(pr * kf, x, y);
+              v2_get(pr * kf, x, y);
             } else {
-              f2_get(pr, x, y);
+              v2_get(pr, x, y);
             }
             r[c / 2] = pack16<T>(x, y);
-            f2_get(pr * (v + de[e]), dp[c], dp[c + 1]);
+            v2_get(pr * (v + de[e]), dp[c], dp[c + 1]);
           }
         }
         tc::tmem_st16(row_s, r);
