@@ -180,21 +180,20 @@ template <typename T> __device__ __forceinline__ void load_window(const Args<T>&
   tc::bulk_load(win + n, a.bits + (size_t)b * words, words * 4, bar);
 }
 
-// 32 exponents in base 2: s scale + bias + c.  The bias comes from the window (wp), or is one number (far_piece; an empty sequence's
-// scores are zeros whatever q and k hold)
-__device__ __forceinline__ void exponents(float (&s)[32], float scale, bool empty, bool far_piece, float far_bias, const float* wp, float c) {
-  const V2 k = v2(scale);
-  if (empty) {
+// How a warp works a piece of 32 columns: beyond the window (its bias is one number) or within it, and with or without masked columns
+// (with: also an empty sequence and a row's first block).  Each way has a body of its own, from the scores' load to the store of what
+// the products read: where the ways met again before that, the registers of all 32 scores were copied (keys' pass of 32 x 512 x 16
+// heads 159 -> 134 us).
+template <bool FAR_, bool MASK_> struct Way { static constexpr bool FAR = FAR_, MASK = MASK_; };
+
+// 32 exponents in base 2: s scale + bias + c; an empty sequence's scores are zeros whatever q and k hold
+template <typename W> __device__ __forceinline__ void exponents(float (&s)[32], float scale, bool empty, float far_bias, const float* wp, float c) {
+  const V2 k = v2(scale), f = v2(W::FAR ? far_bias + c : c);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) s[j] = c;
-  } else if (far_piece) {
-    const V2 f = v2(far_bias + c);
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) v2_get(v2_fma(v2(s[j], s[j + 1]), k, f), s[j], s[j + 1]);
-  } else {
-    const V2 f = v2(c);
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) v2_get(v2_fma(v2(s[j], s[j + 1]), k, v2(wp[j], wp[j + 1])) + f, s[j], s[j + 1]);
+  for (int j = 0; j < 32; j += 2) {
+    if (W::MASK && empty) s[j] = s[j + 1] = 0.f;
+    if constexpr (W::FAR) v2_get(v2_fma(v2(s[j], s[j + 1]), k, f), s[j], s[j + 1]);
+    else v2_get(v2_fma(v2(s[j], s[j + 1]), k, v2(wp[j], wp[j + 1])) + f, s[j], s[j + 1]);
   }
 }
 __device__ __forceinline__ void mask_columns(float (&s)[32], uint32_t on) {
@@ -328,7 +327,7 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
 // 2^60 (bf16; its rounding is relative) or, from 2^6, to 2^15 (fp16) without harm.  Where a block's sum shows that a row left that
 // range, both warps of the rows work the block again from a new reference, with O and the sums scaled to it.  So no other block needs
 // its maximum, and the two warps meet once a block, to hear whether the other one left the range.
-template <typename T, int HD>
+template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4, COLS = 256, TURNS = HD == 128 ? 2 : 3, O_COL = TURNS * BLK;
   constexpr bool FP16 = std::is_same<T, __half>::value;
@@ -370,7 +369,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_o = tmem + lanes + O_COL;
     const float up = FP16 ? 6.f : 0.f, limit = FP16 ? 32768.f : 1.1529215e18f;
-    const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
+    const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++k) {
       const Place at(a, t, per);
@@ -384,16 +383,12 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
       wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + 32 * half, dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;     // of this warp's columns
-        const bool far_piece = dhi <= -wd || dlo >= wd;
-        const float far_bias = dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+        const bool far_piece = empty || dhi <= -wd || dlo >= wd;
+        const float far_bias = empty ? 0.f : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
         const float* wp = win + (k0 - q) + wd + PAD;
         const uint32_t on = bits[k0 >> 5];
         const uint32_t row_s = tmem + lanes + (g % TURNS) * BLK + 32 * half;
-        wait.all(bars.scores + g % TURNS, g / TURNS, tc::SITE_TMEM_FULL);
-        tc::tc_fence_after();
-        float s[32], sum;
-        tc::tmem_ld32(row_s, s);
-        if (__any_sync(0xffffffffu, m == -INFINITY)) {       // the same answer in both warps of the rows
+        const auto top = [&](const float (&s)[32]) {         // of the scores, or m
           float x = m;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
@@ -402,74 +397,83 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
           }
           s_row[0][half][row] = x;
           asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-          x = fmaxf(s_row[0][0][row], s_row[0][1][row]);
-          if (m == -INFINITY) m = x;
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-        }
-        const auto exponentials = [&]() {
+          return fmaxf(s_row[0][0][row], s_row[0][1][row]);
+        };
+        const auto piece = [&](auto way, bool again) {
+          using W = decltype(way);
+          float s[32];
+          tc::tmem_ld32(row_s, s);
+          if constexpr (W::MASK) {
+            if (again) {                                     // a new reference; O is at rest behind the last block's product, half of it each
+              const float x = top(s), f = m == -INFINITY ? 0.f : ex2(m - x);
+              l *= f;
+              m = x;
+              if (i > 0) {
+                wait.all(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_TMEM_FULL);
+                tc::tc_fence_after();
+#pragma unroll 1
+                for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
+                  uint32_t r[16], lo[8], hi[8];
+                  tc::tmem_issue8(row_o + c, lo);
+                  tc::tmem_issue8(row_o + c + 8, hi);
+                  tc::tmem_wait8(lo);
+                  tc::tmem_wait8(hi);
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) {
+                    r[j] = __float_as_uint(__uint_as_float(lo[j]) * f);
+                    r[8 + j] = __float_as_uint(__uint_as_float(hi[j]) * f);
+                  }
+                  tc::tmem_st16(row_o + c, r);
+                }
+              }
+              asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+            } else if (__any_sync(0xffffffffu, m == -INFINITY)) {          // the same answer in both warps of the rows
+              const float x = top(s);
+              if (m == -INFINITY) m = x;
+              asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+            }
+          }
+          exponents<W>(s, a.scale_log2, empty, far_bias, wp, m == -INFINITY ? 0.f : up - m);
+          if constexpr (W::MASK) mask_columns(s, on);
           V2 l2[2] = {v2(0.f), v2(0.f)};
-          exponents(s, a.scale_log2, empty, far_piece, far_bias, wp, m == -INFINITY ? 0.f : up - m);
-          mask_columns(s, on);
+          uint32_t r[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             s[j] = ex2(s[j]);
             s[j + 1] = ex2(s[j + 1]);
             l2[(j >> 1) & 1] = l2[(j >> 1) & 1] + v2(s[j], s[j + 1]);
+            if (DROP) {
+              if (!keep(seed, a.stream, drop0 + k0 + j, a.p)) s[j] = 0.f;
+              if (!keep(seed, a.stream, drop0 + k0 + j + 1, a.p)) s[j + 1] = 0.f;
+            }
+            r[j / 2] = pack16<T>(s[j], s[j + 1]);
           }
           float x, y;
           v2_get(l2[0] + l2[1], x, y);
-          sum = x + y;
+          uint32_t out_of_range = 0;
+          if (!again) {
+            out_of_range = x + y > limit;
+            asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+                         : "+r"(out_of_range) : "r"(1 + quarter) : "memory");
+          }
+          if (!out_of_range) {
+            l += x + y;
+            tc::tmem_st16(row_s, r);
+            tc::tmem_wait_st();
+          }
+          return out_of_range != 0;
         };
-        exponentials();
-        uint32_t out_of_range = sum > limit;
-        asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
-                     : "+r"(out_of_range) : "r"(1 + quarter) : "memory");
-        if (out_of_range) {
-          tc::tmem_ld32(row_s, s);
-          float x = m;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float v = empty ? 0.f : fmaf(s[j], a.scale_log2, far_piece ? far_bias : wp[j]);
-            if (on >> j & 1u) x = fmaxf(x, v);
-          }
-          s_row[0][half][row] = x;
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-          x = fmaxf(s_row[0][0][row], s_row[0][1][row]);
-          const float f = m == -INFINITY ? 0.f : ex2(m - x);
-          l *= f;
-          m = x;
-          if (i > 0) {                                       // O is at rest behind the last block's product; half of it each
-            wait.all(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_TMEM_FULL);
-            tc::tc_fence_after();
-#pragma unroll 1
-            for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
-              uint32_t r[16], lo[8], hi[8];
-              tc::tmem_issue8(row_o + c, lo);
-              tc::tmem_issue8(row_o + c + 8, hi);
-              tc::tmem_wait8(lo);
-              tc::tmem_wait8(hi);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                r[j] = __float_as_uint(__uint_as_float(lo[j]) * f);
-                r[8 + j] = __float_as_uint(__uint_as_float(hi[j]) * f);
-              }
-              tc::tmem_st16(row_o + c, r);
-            }
-          }
-          exponentials();
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        wait.all(bars.scores + g % TURNS, g / TURNS, tc::SITE_TMEM_FULL);
+        tc::tc_fence_after();
+        bool more;
+        if (i == 0 || on != 0xffffffffu || empty || __any_sync(0xffffffffu, m == -INFINITY))
+          more = far_piece ? piece(Way<true, true>(), false) : piece(Way<false, true>(), false);
+        else
+          more = far_piece ? piece(Way<true, false>(), false) : piece(Way<false, false>(), false);
+        if (more) {
+          if (far_piece) piece(Way<true, true>(), true);
+          else piece(Way<false, true>(), true);
         }
-        l += sum;
-        if (a.p > 0.f) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (!keep(seed, a.stream, drop0 + k0 + j, a.p)) s[j] = 0.f;
-        }
-        uint32_t r[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = pack16<T>(s[2 * j], s[2 * j + 1]);
-        tc::tmem_st16(row_s, r);
-        tc::tmem_wait_st();
         warp_arrive(bars.done + g % TURNS, lane);
       }
       s_row[1][half][row] = l;
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
 // ------------------------------------------------------------------------------------------------ backward: queries
 // TMEM: scores 64 columns, dP 64, dQ from 128, behind it two places of 32 for the dS of blocks in turn.  delta for these rows is dctx ctx; the keys' pass gets the sum of P dP that is made on the way, which is free of
 // ctx's rounding (dtable's error at 32 x 512 tokens in fp16: 3.9e-4 with dctx ctx in both, 2.2e-4 so).
-template <typename T, int HD>
+template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 3;
   constexpr int COLS = HD == 128 ? 512 : 256;
@@ -543,7 +547,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_s = tmem + lanes + 32 * half, row_dq = tmem + lanes + 128, row_ds = ds_cols + lanes + 16 * half;
     const float kept = 1.f / (1.f - a.p);
-    const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
+    const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++k) {
       const Place at(a, t, per);
@@ -572,41 +576,46 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + half * 32;                  // of this warp's columns
         const int dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;
+        const bool far_piece = empty || dhi <= -wd || dlo >= wd;
+        const float far_bias = empty ? 0.f : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+        const uint32_t on = bits[k0 >> 5];
+        const auto piece = [&](auto way) {
+          using W = decltype(way);
+          float s[32], dp[32];
+          tmem_ld2x32(row_s, row_s + 64, s, dp);
+          warp_arrive(&bars.read, lane);
+          if (i + 1 == n && lane == 0) tc::mbar_arrive(&bars.freed);
+          exponents<W>(s, a.scale_log2, empty, far_bias, win + (k0 - q) + wd + PAD, -lse);
+          if constexpr (W::MASK) mask_columns(s, on);
+          uint32_t r[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            if (DROP) {
+              dp[j] = keep(seed, a.stream, drop0 + i * BLK + j, a.p) ? dp[j] * kept : 0.f;
+              dp[j + 1] = keep(seed, a.stream, drop0 + i * BLK + j + 1, a.p) ? dp[j + 1] * kept : 0.f;
+            }
+            if constexpr (W::MASK) {                         // a masked key's V may hold anything
+              if (!(on >> j & 1u)) dp[j] = 0.f;
+              if (!(on >> j & 2u)) dp[j + 1] = 0.f;
+            }
+            const V2 pr = v2(ex2(s[j]), ex2(s[j + 1])), v = v2(dp[j], dp[j + 1]);
+            float x, y;
+            sum = v2_fma(pr, v, sum);
+            v2_get(pr * (v + nd), x, y);
+            r[j / 2] = W::MASK && empty ? 0u : pack16<T>(x, y);
+          }
+          tc::tmem_st16(row_ds + (g & 1) * 32, r);           // the product before last has read it: it was issued before these scores
+          tc::tmem_wait_st();
+        };
         wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
         tc::tc_fence_after();
-        float s[32], dp[32];
-        tmem_ld2x32(row_s, row_s + 64, s, dp);
-        warp_arrive(&bars.read, lane);
-        if (i + 1 == n && lane == 0) tc::mbar_arrive(&bars.freed);
-        exponents(s, a.scale_log2, empty, dhi <= -wd || dlo >= wd, dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD], win + (k0 - q) + wd + PAD, -lse);
-        if (a.p > 0.f) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) dp[j] = keep(seed, a.stream, drop0 + i * BLK + j, a.p) ? dp[j] * kept : 0.f;
+        if (on != 0xffffffffu || empty) {
+          if (far_piece) piece(Way<true, true>());
+          else piece(Way<false, true>());
+        } else {
+          if (far_piece) piece(Way<true, false>());
+          else piece(Way<false, false>());
         }
-        const uint32_t on = bits[k0 >> 5];
-        if (on != 0xffffffffu) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (!(on >> j & 1u)) {
-              s[j] = -INFINITY;
-              dp[j] = 0.f;
-            }
-        }
-        uint32_t r[16];
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const V2 pr = v2(ex2(s[j]), ex2(s[j + 1])), v = v2(dp[j], dp[j + 1]);
-          float x, y;
-          sum = v2_fma(pr, v, sum);
-          v2_get(pr * (v + nd), x, y);
-          r[j / 2] = pack16<T>(x, y);
-        }
-        if (empty) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = 0u;
-        }
-        tc::tmem_st16(row_ds + (g & 1) * 32, r);             // the product before last has read it: it was issued before these scores
-        tc::tmem_wait_st();
         warp_arrive(bars.done + (g & 1), lane);
       }
       float x, y;
@@ -645,7 +654,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 // The sums by distance: a diagonal of a warp's 32 x 32 piece of dS (row = lane, column = step) moves on by one lane each step, so a
 // running sum handed to the next lane collects it: one shuffle and one add per column.  Lane 31 drops a finished diagonal each
 // step, the last 32 are in the lanes at the end; the warp then adds all 63 to its window of sums.  This runs under the products.
-template <typename T, int HD>
+template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH;
   constexpr int STAGE = 2 * PIECE + 2 * BLK * 4;             // Q piece, dO piece, -lse, -delta
@@ -760,7 +769,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_s = tmem + lanes + 32 * half, row_acc = tmem + lanes + 128 + 32 * half;
     const float kept = 1.f / (1.f - a.p), not_first = lane == 0 ? 0.f : 1.f;
-    const uint32_t seed = a.p > 0.f ? (uint32_t)__ldg(a.seed) : 0u;
+    const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
     float* mine = sums + warp * nwin;
     for (int i = lane; i < nwin; i += 32) mine[i] = 0.f;
     if (warp == 0) s_none[lane] = -INFINITY;
@@ -792,80 +801,82 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         const int q0 = i * BLK + half * 32;                  // of this warp's columns
         const int dlo = k_warp - (q0 + 31), dhi = k_warp + 31 - q0;
         const bool far_piece = dhi <= -wd || dlo >= wd;
-        wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
-        tc::tc_fence_after();
-        float s[32], dp[32];
-        tmem_ld2x32(row_s, row_s + 64, s, dp);
-        if (i + 1 == n) warp_arrive(&bars.freed, lane);
-        const float4* lse = reinterpret_cast<const float4*>(stage + (g % NST) * STAGE_UP + 2 * PIECE + half * 128);
-        const float4* del = lse + BLK / 4;
         const float far_bias = !on ? -INFINITY : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
         const float* wp = on ? win + (key - q0) + wd + PAD : s_none + 31;
-        const V2 scale = v2(empty ? 0.f : a.scale_log2);
-        if (empty) {
+        const float4* lse = reinterpret_cast<const float4*>(stage + (g % NST) * STAGE_UP + 2 * PIECE + half * 128);
+        const float4* del = lse + BLK / 4;
+        const auto piece = [&](auto way) {                   // MASK: an empty sequence, whose scores are zeros and which has no dS
+          using W = decltype(way);
+          float s[32], dp[32];
+          tmem_ld2x32(row_s, row_s + 64, s, dp);
+          if (i + 1 == n) warp_arrive(&bars.freed, lane);
+          const V2 scale = v2(a.scale_log2), fb = v2(far_bias);
+          uint32_t r[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) s[j] = 0.f;
-        }
-        uint32_t r[16];
+          for (int j = 0; j < 32; j += 4) {
+            const float4 L = lse[j / 4], D = del[j / 4];
+            const V2 ls[2] = {v2(L.x, L.y), v2(L.z, L.w)}, de[2] = {v2(D.x, D.y), v2(D.z, D.w)};
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 L = lse[j / 4], D = del[j / 4];
-          const V2 ls[2] = {v2(L.x, L.y), v2(L.z, L.w)}, de[2] = {v2(D.x, D.y), v2(D.z, D.w)};
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = j + 2 * e;
-            float x, y;
-            v2_get(far_piece || empty ? v2_fma(v2(s[c], s[c + 1]), scale, ls[e] + v2(empty ? 0.f : far_bias))
-                                      : v2_fma(v2(s[c], s[c + 1]), scale, v2(wp[-c], wp[-c - 1])) + ls[e], x, y);
-            const V2 pr = v2(ex2(x), ex2(y));
-            V2 v = v2(dp[c], dp[c + 1]);
-            if (a.p > 0.f) {
-              const uint32_t at0 = ((uint32_t)at.bh * a.S + q0 + c) * (uint32_t)a.S + key;
-              const V2 kf = v2(keep(seed, a.stream, at0, a.p) ? kept : 0.f, keep(seed, a.stream, at0 + (uint32_t)a.S, a.p) ? kept : 0.f);
-              v = v * kf;
-              v2_get(pr * kf, x, y);
-            } else {
-              v2_get(pr, x, y);
+            for (int e = 0; e < 2; ++e) {
+              const int c = j + 2 * e;
+              float x, y;
+              if constexpr (W::MASK) v2_get(ls[e], x, y);
+              else if constexpr (W::FAR) v2_get(v2_fma(v2(s[c], s[c + 1]), scale, ls[e] + fb), x, y);
+              else v2_get(v2_fma(v2(s[c], s[c + 1]), scale, v2(wp[-c], wp[-c - 1])) + ls[e], x, y);
+              const V2 pr = v2(ex2(x), ex2(y));
+              V2 v = v2(dp[c], dp[c + 1]);
+              if (DROP) {
+                const uint32_t at0 = ((uint32_t)at.bh * a.S + q0 + c) * (uint32_t)a.S + key;
+                const V2 kf = v2(keep(seed, a.stream, at0, a.p) ? kept : 0.f, keep(seed, a.stream, at0 + (uint32_t)a.S, a.p) ? kept : 0.f);
+                v = v * kf;
+                v2_get(pr * kf, x, y);
+              } else {
+                v2_get(pr, x, y);
+              }
+              r[c / 2] = pack16<T>(x, y);
+              if constexpr (W::MASK) dp[c] = dp[c + 1] = 0.f;
+              else v2_get(pr * (v + de[e]), dp[c], dp[c + 1]);
             }
-            r[c / 2] = pack16<T>(x, y);
-            v2_get(pr * (v + de[e]), dp[c], dp[c + 1]);
           }
-        }
-        tc::tmem_st16(row_s, r);
-        if (empty) {
+          tc::tmem_st16(row_s, r);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) dp[j] = 0.f;
-        }
+          for (int j = 0; j < 16; ++j) r[j] = pack16<T>(dp[2 * j], dp[2 * j + 1]);
+          tc::tmem_st16(row_s + 64, r);
+          tc::tmem_wait_st();
+          warp_arrive(bars.done + (g & 1), lane);
+          if constexpr (W::FAR && !W::MASK) {
+            V2 v = v2(0.f);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = pack16<T>(dp[2 * j], dp[2 * j + 1]);
-        tc::tmem_st16(row_s + 64, r);
-        tc::tmem_wait_st();
-        warp_arrive(bars.done + (g & 1), lane);
-        if (far_piece) {
-          float v = 0.f;
+            for (int j = 0; j < 32; j += 2) v = v + v2(dp[j], dp[j + 1]);
+            float x, y;
+            v2_get(v, x, y);
+            far[dhi <= -wd ? 0 : 1] += x + y;
+          } else if constexpr (!W::FAR) {
+            float* diag = s_diag[warp];                      // diagonal e: row - column = e - 31
+            float acc = dp[0];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v += dp[j];
-          far[dhi <= -wd ? 0 : 1] += v;
-        } else {
-          float* diag = s_diag[warp];                        // diagonal e: row - column = e - 31
-          float acc = dp[0];
+            for (int j = 1; j < 32; ++j) {
+              if (lane == 31) diag[63 - j] = acc;            // row 31, column j - 1
+              acc = fmaf(__shfl_up_sync(0xffffffffu, acc, 1), not_first, dp[j]);
+            }
+            diag[lane] = acc;                                // column 31: row - column = lane - 31
+            __syncwarp();
 #pragma unroll
-          for (int j = 1; j < 32; ++j) {
-            if (lane == 31) diag[63 - j] = acc;              // row 31, column j - 1
-            acc = fmaf(__shfl_up_sync(0xffffffffu, acc, 1), not_first, dp[j]);
+            for (int e = lane; e < 63; e += 32) {
+              const float v = diag[e];
+              const int d = k_warp - q0 + e - 31;
+              if (d <= -wd) far[0] += v;
+              else if (d >= wd) far[1] += v;
+              else mine[d + wd] += v;
+            }
+            __syncwarp();
           }
-          diag[lane] = acc;                                  // column 31: row - column = lane - 31
-          __syncwarp();
-#pragma unroll
-          for (int e = lane; e < 63; e += 32) {
-            const float v = diag[e];
-            const int d = k_warp - q0 + e - 31;
-            if (d <= -wd) far[0] += v;
-            else if (d >= wd) far[1] += v;
-            else mine[d + wd] += v;
-          }
-          __syncwarp();
-        }
+        };
+        wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
+        tc::tc_fence_after();
+        if (empty) piece(Way<true, true>());
+        else if (far_piece) piece(Way<true, false>());
+        else piece(Way<false, false>());
       }
       far[0] = warp_sum(far[0]);
       far[1] = warp_sum(far[1]);
@@ -911,7 +922,7 @@ template <typename K> int allow_smem(K kernel, int bytes) {
   return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-template <typename T, int HD> int run_fwd_tc(const Args<T>& a, cudaStream_t st) {
+template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaStream_t st) {
   constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = HD == 128 ? 2 : 4;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps m;
@@ -922,13 +933,13 @@ template <typename T, int HD> int run_fwd_tc(const Args<T>& a, cudaStream_t st) 
   if (rc) return rc;
   m.d = m.e = m.c;
   const int smem = 1024 + (ROWS + NST * 2 * BLK) * 128 * CH + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
-  rc = allow_smem(fwd_tc<T, HD>, smem);
+  rc = allow_smem(fwd_tc<T, HD, DROP>, smem);
   if (rc) return rc;
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * 2;
-  return (int)launch_pdl(fwd_tc<T, HD>, dim3(tiles < most ? tiles : most), dim3(320), smem, st, a, m);
+  return (int)launch_pdl(fwd_tc<T, HD, DROP>, dim3(tiles < most ? tiles : most), dim3(320), smem, st, a, m);
 }
 
-template <typename T, int HD> int run_bwd_tc(const Args<T>& a, cudaStream_t st) {
+template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaStream_t st) {
   constexpr int CH = (HD < 64 ? 64 : HD) / 64, PIECE = BLK * 128 * CH, STAGE_UP = (2 * PIECE + 2 * BLK * 4 + 1023) / 1024 * 1024, NST = HD == 128 ? 2 : 3;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps q, kv;
@@ -947,24 +958,24 @@ template <typename T, int HD> int run_bwd_tc(const Args<T>& a, cudaStream_t st) 
   const int wd = window(a), windows = 2 * (window_floats(wd) + mask_words(a.S)) * 4;
   const int smem_q = 1024 + 3 * ROWS * 128 * CH + NST * 2 * PIECE + windows;
   const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST * STAGE_UP + windows + 8 * (2 * wd + 1) * 4;
-  rc = allow_smem(bwd_q_tc<T, HD>, smem_q);
-  if (!rc) rc = allow_smem(bwd_kv_tc<T, HD>, smem_kv);
+  rc = allow_smem(bwd_q_tc<T, HD, DROP>, smem_q);
+  if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP>, smem_kv);
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * (HD == 128 ? 1 : 2);
   const dim3 grid(tiles < most ? tiles : most);
-  if (!rc) rc = (int)launch_pdl(bwd_q_tc<T, HD>, grid, dim3(320), smem_q, st, a, q);
-  if (!rc) rc = (int)launch_pdl(bwd_kv_tc<T, HD>, grid, dim3(320), smem_kv, st, a, kv);
+  if (!rc) rc = (int)launch_pdl(bwd_q_tc<T, HD, DROP>, grid, dim3(320), smem_q, st, a, q);
+  if (!rc) rc = (int)launch_pdl(bwd_kv_tc<T, HD, DROP>, grid, dim3(320), smem_kv, st, a, kv);
   return rc;
 }
 
 template <typename T> int fwd_on_tensor_cores(const Args<T>& a, int hd, cudaStream_t st) {
-  if (hd == 32) return run_fwd_tc<T, 32>(a, st);
-  if (hd == 64) return run_fwd_tc<T, 64>(a, st);
-  return run_fwd_tc<T, 128>(a, st);
+  if (hd == 32) return a.p > 0.f ? run_fwd_tc<T, 32, true>(a, st) : run_fwd_tc<T, 32, false>(a, st);
+  if (hd == 64) return a.p > 0.f ? run_fwd_tc<T, 64, true>(a, st) : run_fwd_tc<T, 64, false>(a, st);
+  return a.p > 0.f ? run_fwd_tc<T, 128, true>(a, st) : run_fwd_tc<T, 128, false>(a, st);
 }
 template <typename T> int bwd_on_tensor_cores(const Args<T>& a, int hd, cudaStream_t st) {
-  if (hd == 32) return run_bwd_tc<T, 32>(a, st);
-  if (hd == 64) return run_bwd_tc<T, 64>(a, st);
-  return run_bwd_tc<T, 128>(a, st);
+  if (hd == 32) return a.p > 0.f ? run_bwd_tc<T, 32, true>(a, st) : run_bwd_tc<T, 32, false>(a, st);
+  if (hd == 64) return a.p > 0.f ? run_bwd_tc<T, 64, true>(a, st) : run_bwd_tc<T, 64, false>(a, st);
+  return a.p > 0.f ? run_bwd_tc<T, 128, true>(a, st) : run_bwd_tc<T, 128, false>(a, st);
 }
 template int fwd_on_tensor_cores<__nv_bfloat16>(const Args<__nv_bfloat16>&, int, cudaStream_t);
 template int fwd_on_tensor_cores<__half>(const Args<__half>&, int, cudaStream_t);
