@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ tabl
   if (lane == 0 && last) atomicMax(&s_len, last);
   __syncthreads();
   if (threadIdx.x == 0) lens[b] = s_len;
+  if (b == 0 && threadIdx.x < 3) lens[(int)gridDim.x - nh + threadIdx.x] = 0;      // the tile counters, behind the lengths
   if (s_len == 0)
     for (int w = threadIdx.x; w < words; w += 256)
       bits[(size_t)b * words + w] = S - 32 * w >= 32 ? 0xffffffffu : S > 32 * w ? (1u << (S - 32 * w)) - 1u : 0u;
@@ -303,13 +304,15 @@ __global__ void __launch_bounds__(W * 32) bwd_short(Args<T> a) {
 constexpr int DT_CTAS = 8;
 template <typename T>
 __global__ void __cluster_dims__(DT_CTAS, 1, 1) __launch_bounds__(1024) dtable_kernel(const float* __restrict__ dwin, const int* __restrict__ lut,
-                                                                                    T* __restrict__ dtable, int parts, int nh, int wd, int far, int nb) {
+                                                                                    T* __restrict__ dtable, int* counter, int parts, int nh, int wd,
+                                                                                    int far, int nb) {
   extern __shared__ float sm[];                                     // [groups][nwin] of a CTA; [DT_CTAS][nwin] in the first; [nwin] buckets
   const int rank = blockIdx.x % DT_CTAS, h = blockIdx.x / DT_CTAS, nwin = 2 * wd + 1, groups = max(1, 1024 / nwin);
   float* all = sm + groups * nwin;
   int* bucket = reinterpret_cast<int*>(all + DT_CTAS * nwin);
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");          // the first CTA has to run before it is written to
   grid_dep_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0 && counter != nullptr) *counter = 0;     // the keys' pass is over; another one may follow
   for (int i = threadIdx.x; i < groups * nwin; i += 1024) {
     const int gr = i / nwin, d = i - gr * nwin;
     const float* src = dwin + (size_t)h * nwin + d;
@@ -382,7 +385,8 @@ struct Common {
   const void *q, *k, *v;
   long long ldq, ldk, ldv;
   int far, nb, b, S, nh, hd;
-  const void *win, *bits, *lens;
+  const void *win, *bits;
+  void* lens;
   float p;
   const void* seed;
   unsigned stream;
@@ -392,7 +396,7 @@ template <typename T> Args<T> args(const Common& c) {
   Args<T> a = {};
   a.q = (const T*)c.q; a.k = (const T*)c.k; a.v = (const T*)c.v;
   a.ldq = c.ldq; a.ldk = c.ldk; a.ldv = c.ldv;
-  a.win = (const float*)c.win; a.bits = (const uint32_t*)c.bits; a.lens = (const int*)c.lens;
+  a.win = (const float*)c.win; a.bits = (const uint32_t*)c.bits; a.lens = (const int*)c.lens; a.counters = (int*)c.lens + c.b;
   a.far = c.far; a.nb = c.nb; a.b = c.b; a.S = c.S; a.nh = c.nh;
   a.scale = 1.f / sqrtf((float)c.hd);
   a.scale_log2 = LOG2E * a.scale;
@@ -430,7 +434,7 @@ RB_API int rb_relative_fwd(int dtype, const void* q, long long ldq, const void* 
 }
 
 RB_API int rb_relative_bwd(int dtype, const void* dctx, const void* q, long long ldq, const void* k, long long ldk, const void* v, long long ldv,
-                           int far, int nb, int b, int S, int nh, int hd, const void* win, const void* bits, const void* lens, float p,
+                           int far, int nb, int b, int S, int nh, int hd, const void* win, const void* bits, void* lens, float p,
                            const void* seed, unsigned stream, void* status, const void* lut, const void* ctx, const void* lse, void* stats, void* dwin,
                            void* dq, long long lddq, void* dk, long long lddk, void* dv, long long lddv, void* dtable, cudaStream_t st) {
   const rel::Common c{q, k, v, ldq, ldk, ldv, far, nb, b, S, nh, hd, win, bits, lens, p, seed, stream, status};
@@ -456,7 +460,7 @@ RB_API int rb_relative_bwd(int dtype, const void* dctx, const void* q, long long
     const int smem = (groups + rel::DT_CTAS + 1) * nwin * 4;
     rc = rel::set_smem(rel::dtable_kernel<T>, smem);
     return rc ? rc : (int)launch_pdl(rel::dtable_kernel<T>, dim3(nh * rel::DT_CTAS), dim3(1024), smem, st, (const float*)dwin, (const int*)lut,
-                                     (T*)dtable, b * rb_relative_tiles(S), nh, wd, far, nb);
+                                     (T*)dtable, b > 0 ? a.counters + 2 : nullptr, b * rb_relative_tiles(S), nh, wd, far, nb);
   };
   return dtype == RB_BF16 ? go(__nv_bfloat16()) : dtype == RB_F16 ? go(__half()) : -1;
 }

@@ -28,6 +28,7 @@ template <typename T> struct Args {
   const float* win;              // [nh][window_floats] bias by distance, base 2
   const uint32_t* bits;          // [b][mask_words] attended keys (an empty sequence: all)
   const int* lens;               // [b] position behind the last attended key; 0 = nothing is attended
+  int* counters;                 // [3] tiles taken by the forward, queries' and keys' kernels (relative_tc.cu); zero between calls
   float scale_log2;              // log2(e) / sqrt(HD)
   float scale;                   // 1 / sqrt(HD)
   float p;

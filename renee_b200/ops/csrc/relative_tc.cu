@@ -10,7 +10,8 @@
 // the first products and, as it stands, the MN-major B operand of the second ones).  A thread reads its row of scores from TMEM,
 // works on it, and writes 16-bit P or dS back to TMEM, where they are the A operand of the second product: scores never pass through
 // shared memory, and a row's maximum and sum need no shuffle.
-// CTAs stay (2 per SM; heads of 128: 1) and take every gridDim.x-th tile.  Ten warps: 0-7 work on the scores (warp w and w + 4 share 32
+// CTAs stay (2 per SM; heads of 128: 1) and take the next tile off a counter (texts differ in length: with every gridDim.x-th tile the
+// slowest CTA had a third more to do than the average).  Ten warps: 0-7 work on the scores (warp w and w + 4 share 32
 // rows and take 32 columns each), 8 issues copies (one to three blocks ahead, into the next tile's too), 9 issues MMAs from one
 // thread.  A block's scores are issued as soon as their place is free, so that the MMAs run under the exponentials.  MMAs with
 // different accumulators are not taken to run in order: what one reads is overwritten only behind a commit that covers it.
@@ -204,6 +205,39 @@ __device__ __forceinline__ void mask_columns(float (&s)[32], uint32_t on) {
   }
 }
 
+// The tiles of a CTA: its own number first, then what the counter says.  The copying warp asks (one tile ahead) and hands on through
+// shared memory: tile_of[k & 1] is written before the own barrier of the CTA's k-th tile; -1 ends.
+struct Tiles {
+  int* counter;
+  int now, next;
+  __device__ __forceinline__ Tiles(int* c, int lane) : counter(c), now(blockIdx.x) { next = ask(lane); }
+  __device__ __forceinline__ int ask(int lane) {
+    int t = 0;
+    if (lane == 0) t = (int)gridDim.x + atomicAdd(counter, 1);
+    return __shfl_sync(0xffffffffu, t, 0);
+  }
+  __device__ __forceinline__ void step(int lane) {
+    now = next;
+    next = ask(lane);
+  }
+};
+// A worker's next tile, or -1.  All workers leave together, also when a wait of one of them has run out.
+__device__ __forceinline__ int worker_tile(Bars& bars, Waiter& wait, const int* tile_of, unsigned k) {
+  wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
+  uint32_t gone = wait.aborted;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred q, 5, 256, p;\n selp.u32 %0, 1, 0, q;\n}" : "+r"(gone) :: "memory");
+  return gone ? -1 : *(const volatile int*)(tile_of + (k & 1));
+}
+// The copying warp's last word
+__device__ __forceinline__ void no_more_tiles(Bars& bars, Waiter& wait, int* tile_of, unsigned k) {
+  if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
+  if (!wait.aborted && tc::elect_one()) {
+    tile_of[k & 1] = -1;
+    tc::mbar_arrive(bars.own + (k & 1));
+  }
+  __syncwarp();
+}
+
 // Where a tile of queries lies: tile t of `per` tiles a (sequence, head)
 struct Place {
   int bh, b, h, row0;
@@ -223,7 +257,7 @@ template <typename T> __device__ __forceinline__ int key_blocks(const Args<T>& a
 // masked: the half of the stage (K or V) whose masked rows become zeros, because 0 times a NaN is one
 template <int NST, int CH, int PIECE, typename T, typename Own, typename Load>
 __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, char* stage, int masked, int lane,
-                                                 Own own, Load load) {
+                                                 int* counter, int* tile_of, Own own, Load load) {
   unsigned g = 0, k = 0, turns = 0;                            // turns: bit s = phase of raw[s]
   uint2 on_last = make_uint2(0xffffffffu, 0xffffffffu);        // attended keys of the block before, if it has to be mended
   const auto mend = [&](unsigned x) {                          // block x
@@ -240,8 +274,8 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(bars.full + s);
   };
-  for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++k) {
-    const Place at(a, t, per);
+  for (Tiles t(counter, lane); t.now < tiles; t.step(lane), ++k) {
+    const Place at(a, t.now, per);
     const int n = key_blocks(a, at.b);
     const uint2* bits = reinterpret_cast<const uint2*>(a.bits + (size_t)at.b * mask_words(a.S));
     for (int i = 0; i < n; ++i, ++g) {
@@ -261,7 +295,10 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
         if (k > 0) wait.all(&bars.freed, k - 1, tc::SITE_EMPTY);
         if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
         if (wait.aborted) return;
-        if (tc::elect_one()) own(at, k, bars.own + (k & 1));
+        if (tc::elect_one()) {
+          tile_of[k & 1] = t.now;
+          own(at, k, bars.own + (k & 1));
+        }
         __syncwarp();
       } else {
         mend(g - 1);
@@ -270,6 +307,7 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
     }
   }
   if (g > 0) mend(g - 1);
+  no_more_tiles(bars, wait, tile_of, k);
 }
 
 // The MMA thread of fwd and bwd_q.  scores(g, s), rows(g, s, first): the products of block g, in stage s.
@@ -277,7 +315,7 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
 // issued TURNS - 1 blocks before the second product waits for its P.  TURNS = 0: scores have one buffer, free as soon as they are in
 // registers, and dS has two places of its own.
 template <int NST, int TURNS, typename T, typename Scores, typename Rows>
-__device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, Scores scores, Rows rows) {
+__device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int per, const int* tile_of, Scores scores, Rows rows) {
   constexpr unsigned SLOTS = TURNS ? TURNS : 2, AHEAD = TURNS ? TURNS - 1 : 1;
   unsigned g = 0, k = 0, x = 0;                                // blocks begun, tiles begun, second products issued
   unsigned jx = 0, ix = 0, nx = 0, n_last = 0;                 // block x: the ix-th of nx of the CTA's jx-th tile
@@ -295,10 +333,13 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
       ++jx;
     }
   };
-  for (int t = blockIdx.x; t < tiles && !wait.aborted; t += gridDim.x, ++k) {
-    const unsigned n = key_blocks(a, t / per / a.nh);
+  for (;; ++k) {
     nx = n_last;
     while (x < g && !wait.aborted) second();                   // the last tile's end before this one's rows are waited for
+    wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
+    const int t = *(const volatile int*)(tile_of + (k & 1));
+    if (wait.aborted || t < 0) return;
+    const unsigned n = key_blocks(a, t / per / a.nh);
     nx = n_last = n;
     for (unsigned i = 0; i < n && !wait.aborted; ++i, ++g) {
       if (TURNS) {
@@ -306,7 +347,6 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
       } else {
         if (g > 0) wait.one(&bars.read, g - 1, tc::SITE_TMEM_EMPTY);
       }
-      if (i == 0) wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
       if (wait.aborted) return;
       tc::tc_fence_after();
@@ -316,7 +356,6 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
       if (g >= x + AHEAD) second();
     }
   }
-  while (x < g && !wait.aborted) second();
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -334,6 +373,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
+  __shared__ int tile_of[2];
   __shared__ float s_row[2][2][ROWS];                        // [maxima, sums][half][row]
   char* sq = align1k(smem_raw);
   char* stage = sq + TILE;                                   // [NST][K piece, V piece]
@@ -346,7 +386,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   grid_dep_wait();
   if (warp == WORKERS) {
     copy_query_tiles<NST, CH, PIECE>(
-        a, bars, wait, tiles, per, stage, 1, lane,
+        a, bars, wait, tiles, per, stage, 1, lane, a.counters + 0, tile_of,
         [&](const Place& at, unsigned k, uint64_t* bar) {
           tc::mbar_expect_tx(bar, TILE + window_bytes(a, wd));
           load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -360,7 +400,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   } else if (warp > WORKERS) {
     if (tc::elect_one())
       multiply_query_tiles<NST, TURNS>(
-          a, bars, wait, tiles, per,
+          a, bars, wait, per, tile_of,
           [&](unsigned g, int s) { mma_scores<T, HD>(tmem + (g % TURNS) * BLK, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE)); },
           [&](unsigned g, int s, bool first) {
             mma_rows<T, HDP>(tmem + O_COL, tmem + (g % TURNS) * BLK, 32, tc::smem_u32(stage + s * 2 * PIECE + PIECE), first);
@@ -371,7 +411,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
     const float up = FP16 ? 6.f : 0.f, limit = FP16 ? 32768.f : 1.1529215e18f;
     const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++k) {
+    for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
       const Place at(a, t, per);
       const int seen = __ldg(a.lens + at.b), n = ((seen > 0 ? seen : a.S) + BLK - 1) / BLK;
       const bool empty = seen == 0;
@@ -380,7 +420,6 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
       const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S;
       float m = -INFINITY, l = 0.f;
-      wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + 32 * half, dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;     // of this warp's columns
         const bool far_piece = empty || dhi <= -wd || dlo >= wd;
@@ -507,6 +546,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
+  __shared__ int tile_of[2];
   __shared__ float s_sum[2][2][ROWS];
   char* sq = align1k(smem_raw);
   char* sdo = sq + TILE;
@@ -521,7 +561,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   grid_dep_wait();
   if (warp == WORKERS) {
     copy_query_tiles<NST, CH, PIECE>(
-        a, bars, wait, tiles, per, stage, 0, lane,
+        a, bars, wait, tiles, per, stage, 0, lane, a.counters + 1, tile_of,
         [&](const Place& at, unsigned k, uint64_t* bar) {
           tc::mbar_expect_tx(bar, 3 * TILE + window_bytes(a, wd));
           load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -537,7 +577,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   } else if (warp > WORKERS) {
     if (tc::elect_one())
       multiply_query_tiles<NST, 0>(
-          a, bars, wait, tiles, per,
+          a, bars, wait, per, tile_of,
           [&](unsigned, int s) {
             mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE));
             mma_scores<T, HD>(tmem + 64, tc::smem_u32(sdo), tc::smem_u32(stage + s * 2 * PIECE + PIECE));
@@ -549,7 +589,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
     const float kept = 1.f / (1.f - a.p);
     const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++k) {
+    for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
       const Place at(a, t, per);
       const int seen = __ldg(a.lens + at.b), n = ((seen > 0 ? seen : a.S) + BLK - 1) / BLK;
       const bool empty = seen == 0;
@@ -558,7 +598,6 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       const float* win = windows + (k & 1) * wfloats;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
       const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S + half * 32;
-      wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       float d = 0.f;                                         // delta = dctx ctx: half a row each
 #pragma unroll
       for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
@@ -662,6 +701,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
+  __shared__ int tile_of[2];
   __shared__ float s_diag[8][64];
   __shared__ float s_none[32];                               // the window of a masked key
   char* sk = align1k(smem_raw);
@@ -676,7 +716,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   const uint32_t tmem = s_tmem;
   Waiter wait{false, a.status};
   grid_dep_wait();
-  // tiles in order of their place in the sequence: the last ones, of which few have an attended key, are spread over all CTAs
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.counters[1] = 0;          // the queries' pass is over; another one may follow
+  // tiles in order of their place in the sequence: the last ones, of which few have an attended key, fill the gaps
   const auto place = [&](int t) {
     const int bhs = a.nh * a.b, part = t / bhs;
     return Place(a, (t - part * bhs) * per + part, per);
@@ -689,9 +730,9 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   };
   if (warp == WORKERS) {
     unsigned g = 0, k = 0, turn = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-      if (blocks(t) == 0) continue;
-      const Place at = place(t);
+    for (Tiles t(a.counters + 2, lane); t.now < tiles; t.step(lane)) {
+      if (blocks(t.now) == 0) continue;
+      const Place at = place(t.now);
       const uint4 on = __ldg(reinterpret_cast<const uint4*>(a.bits + (size_t)at.b * mask_words(a.S)) + at.row0 / ROWS);
       const bool whole = (on.x & on.y & on.z & on.w) == 0xffffffffu;
       for (int i = 0; i < nq; ++i, ++g) {
@@ -713,6 +754,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         if (wait.aborted) break;
         uint64_t* bar = whole ? bars.own + (k & 1) : bars.raw;
         if (tc::elect_one()) {
+          tile_of[k & 1] = t.now;
           tc::mbar_expect_tx(bar, 2 * TILE + window_bytes(a, wd));
           load_tile<CH>(sk, &maps.b, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sv, &maps.c, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -732,6 +774,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       if (wait.aborted) break;
       ++k;
     }
+    no_more_tiles(bars, wait, tile_of, k);
   } else if (warp > WORKERS) {
     if (tc::elect_one()) {
       unsigned g = 0, k = 0;
@@ -748,11 +791,12 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         if (last) tc::umma_commit(&bars.end);
         wait.one(bars.empty + x % NST, x / NST, tc::SITE_EMPTY);
       };
-      for (int t = blockIdx.x; t < tiles && !wait.aborted; t += gridDim.x) {
-        if (blocks(t) == 0) continue;
+      for (;; ++k) {
+        if (g > 0) second(g - 1, nq == 1, true, k - 1);
+        wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
+        if (wait.aborted || *(const volatile int*)(tile_of + (k & 1)) < 0) break;
         for (int i = 0; i < nq && !wait.aborted; ++i, ++g) {
-          if (g > 0) second(g - 1, nq == 1 || i == 1, i == 0, i == 0 ? k - 1 : k);
-          if (i == 0) wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
+          if (i > 0) second(g - 1, i == 1, false, k);
           wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
           if (wait.aborted) break;
           tc::tc_fence_after();
@@ -761,12 +805,10 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           mma_scores<T, HD>(tmem + 64, tc::smem_u32(sv), tc::smem_u32(st + PIECE));
           tc::umma_commit(bars.scores + (g & 1));
         }
-        ++k;
       }
-      if (g > 0 && !wait.aborted) second(g - 1, nq == 1, true, k - 1);
     }
   } else {
-    const int quarter = warp & 3, half = warp >> 2;
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, row_s = tmem + lanes + 32 * half, row_acc = tmem + lanes + 128 + 32 * half;
     const float kept = 1.f / (1.f - a.p), not_first = lane == 0 ? 0.f : 1.f;
     const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
@@ -775,25 +817,27 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     if (warp == 0) s_none[lane] = -INFINITY;
     asm volatile("bar.sync 1, 256;" ::: "memory");
     unsigned g = 0, k = 0;
+    // tiles without an attended key: zeros, each CTA its share
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      if (blocks(t) > 0) continue;
       const Place at = place(t);
-      const int k_warp = at.row0 + quarter * 32, key = k_warp + lane, n = blocks(t);
+      const int key = at.row0 + row;
+      float v[32] = {};
+      if (key < a.S)
+#pragma unroll
+        for (int c = 32 * half; c < HD; c += 64) {
+          store_row<T>(a.dv + ((size_t)at.b * a.S + key) * a.lddv + at.h * HD + c, v, 0.f);
+          store_row<T>(a.dk + ((size_t)at.b * a.S + key) * a.lddk + at.h * HD + c, v, 0.f);
+        }
+      for (int i = threadIdx.x; i < nwin; i += 256) a.dwin[((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin + i] = 0.f;
+    }
+    for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
+      const Place at = place(t);
+      const int k_warp = at.row0 + quarter * 32, key = k_warp + lane, n = nq;
       T* const out_v = a.dv + ((size_t)at.b * a.S + key) * a.lddv + at.h * HD;
       T* const out_k = a.dk + ((size_t)at.b * a.S + key) * a.lddk + at.h * HD;
       float* const out_w = a.dwin + ((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin;
-      if (n == 0) {
-        float v[32] = {};
-        if (key < a.S)
-#pragma unroll
-          for (int c = 32 * half; c < HD; c += 64) {
-            store_row<T>(out_v + c, v, 0.f);
-            store_row<T>(out_k + c, v, 0.f);
-          }
-        for (int i = threadIdx.x; i < nwin; i += 256) out_w[i] = 0.f;
-        continue;
-      }
       const bool empty = __ldg(a.lens + at.b) == 0;
-      wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
       const float* win = windows + (k & 1) * wfloats;
       const bool on = reinterpret_cast<const uint32_t*>(win + window_floats(wd))[key >> 5] >> (key & 31) & 1u;
       float far[2] = {};
@@ -911,7 +955,6 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           }
           if (key < a.S && 32 * half + 64 * c < HD) store_row<T>((o ? out_k : out_v) + 32 * half + 64 * c, v, o ? a.scale * a.grad_inv : a.grad_inv);
         }
-      ++k;
     }
   }
   finish<COLS>(&s_tmem, warp);

@@ -213,7 +213,7 @@ def relative_buckets(num_buckets: int, max_distance: int, device=None) -> torch.
 
 class RelativeWorkspace:
     """What :func:`relative_attention_fwd` leaves for its backward pass (``lse``, the biases by distance ``win``, the masks as
-    ``bits`` and ``lens``) and the scratch of that pass (``stats``, ``dwin``)."""
+    ``bits`` and ``lens``, with the kernels' tile counters behind) and the scratch of that pass (``stats``, ``dwin``)."""
 
     def __init__(self, lse, win, bits, lens, stats, dwin):
         self.lse, self.win, self.bits, self.lens, self.stats, self.dwin = lse, win, bits, lens, stats, dwin
@@ -223,7 +223,7 @@ class RelativeWorkspace:
 def _relative_sizes(b: int, S: int, nh: int, far: int) -> tuple:
     """Values of the workspace's buffers; the statistics and the bits of a sequence take whole tiles of 128 tokens."""
     cu, up = _cuda(), -(-S // 128) * 128
-    return (b * nh * up, nh * cu.relative_window_floats(far, S), b * up // 32, b, 2 * b * nh * up,
+    return (b * nh * up, nh * cu.relative_window_floats(far, S), b * up // 32, b + 3, 2 * b * nh * up,
             b * cu.relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
 
 
