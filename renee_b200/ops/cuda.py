@@ -428,7 +428,7 @@ def _call_typed(name, device, *args, launches=1):
         fn = getattr(lib(), name)
         fn.argtypes = [_KINDS[k] for k in _TYPES[name]]
         _TYPED[name] = fn
-    rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))      # torch.cuda.current_stream makes an object for it: 2 us
     if rc != 0:
         raise KernelError(f"{name} failed with code {rc}")
     _LAUNCHES += launches
@@ -468,8 +468,7 @@ def relative_window_floats(far: int, S: int) -> int:
 def _relative_inputs(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):
     b, S = mask.shape
     return (at[0], _ld(q), at[1], _ld(k), at[2], _ld(v), (buckets.shape[0] - 1) // 2, table.shape[0], b, S, nh, q.shape[1] // nh,
-            ws.win.data_ptr(), ws.bits.data_ptr(), ws.lens.data_ptr(), p, rng.dev.data_ptr() if p > 0 else None, stream,
-            workspace(q.device).status.data_ptr())
+            ws.win.data_ptr(), ws.bits.data_ptr(), ws.lens.data_ptr(), p, rng.dev.data_ptr() if p > 0 else None, stream, ws.status.data_ptr())
 
 
 def relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):

@@ -217,6 +217,7 @@ class RelativeWorkspace:
 
     def __init__(self, lse, win, bits, lens, stats, dwin):
         self.lse, self.win, self.bits, self.lens, self.stats, self.dwin = lse, win, bits, lens, stats, dwin
+        self.status = _cuda().workspace(lse.device).status if lse.is_cuda else None      # where waits that run out are noted
         self.sizes = (lse.device, *(t.numel() for t in (lse, win, bits, lens, stats, dwin)))
 
 
