@@ -12,7 +12,8 @@
 // buckets behind all CTAs (dtable_kernel), so the map may be any.  (Gathered by every CTA for itself, the window and the mask were
 // 5 us of a CTA's 12 to 18 at 512 tokens: two dependent loads per entry, and ballots.)
 // A masked key counts as absent: its K and V rows are read as zeros, whatever they hold.  A sequence without any attended key
-// attends to all of its S tokens alike (P = 1 / S): its scores are constants, so only v has a gradient there.
+// attends to all of its S tokens alike (P = 1 / S): its scores are constants, so only v has a gradient there.  Nor do they matter for a
+// gradient where a single key is attended (P = 1): both are `flat` to the backward passes, whose other gradients are zeros, not rounding.
 #pragma once
 #include "common.cuh"
 
@@ -27,7 +28,7 @@ template <typename T> struct Args {
   int far, nb, b, S, nh;
   const float* win;              // [nh][window_floats] bias by distance, base 2
   const uint32_t* bits;          // [b][mask_words] attended keys (an empty sequence: all)
-  const int* lens;               // [b] position behind the last attended key; 0 = nothing is attended
+  const int* lens;               // [b] position behind the last attended key, negative where it is the only one; 0 = nothing is attended
   int* counters;                 // [3] tiles taken by the forward, queries' and keys' kernels (relative_tc.cu); zero between calls
   float scale_log2;              // log2(e) / sqrt(HD)
   float scale;                   // 1 / sqrt(HD)
@@ -54,6 +55,9 @@ template <typename T> __host__ __device__ __forceinline__ int window(const Args<
 constexpr int PAD = 128;
 __host__ __device__ __forceinline__ int window_floats(int wd) { return (2 * wd + 1 + 2 * PAD + 3) / 4 * 4; }
 __host__ __device__ __forceinline__ int mask_words(int S) { return (S + 127) / 128 * 4; }       // whole tiles of 128, zeros behind S
+
+// Keys of a sequence that are looked at
+__device__ __forceinline__ int attended_len(int seen, int S) { return seen == 0 ? S : abs(seen); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

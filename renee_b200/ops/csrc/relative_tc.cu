@@ -15,8 +15,13 @@
 // rows and take 32 columns each), 8 issues copies (one to three blocks ahead, into the next tile's too), 9 issues MMAs from one
 // thread.  A block's scores are issued as soon as their place is free, so that the MMAs run under the exponentials.  MMAs with
 // different accumulators are not taken to run in order: what one reads is overwritten only behind a commit that covers it.
-// (One warp for copies, MMAs and the zeros for masked rows was what bounded all three kernels: 1000 clocks a block, whatever the
-// others did.)
+// Measured (one B200): 32 x 512 x 16 heads of 64, fp16, texts of 128 to 512 tokens: forward 69 us, queries 74, keys 125 (75 GFLOP of
+// products with attended keys in all: 45 us at the GEMM rate; 400 MB: 62 us).  4 x 4099 x 12 heads, forward: 285 us, 148 of them the
+// exponentials' own rate (16 a clock and SM).  What bounds them: instructions and hops.  A worker issues 6 (forward) to 14 (keys)
+// instructions a score, at half of the issue rate with 16 warps an SM (TMEM holds no more rows' scores); a hand-over through an
+// mbarrier takes 200 clocks, and a tile's end and begin cost as much as two to three blocks.  Tried without gain: scores of two blocks
+// in one buffer of 128 columns with 4 warps a CTA, 4 CTAs an SM with one buffer each, P~ and dS of the keys' pass through shared
+// memory (125 -> 150 us: the products' operands from there are then what it is bound by), deeper rings of stages, dependents launched early.
 #include "relative.cuh"
 #include "tc.cuh"
 
@@ -249,8 +254,7 @@ struct Place {
   }
 };
 template <typename T> __device__ __forceinline__ int key_blocks(const Args<T>& a, int b) {
-  const int seen = __ldg(a.lens + b);
-  return ((seen > 0 ? seen : a.S) + BLK - 1) / BLK;
+  return (attended_len(__ldg(a.lens + b), a.S) + BLK - 1) / BLK;
 }
 
 // The copying warp of fwd and bwd_q.  own(at, k, bar): a tile's copies, the CTA's k-th; load(at, i, s, bar): block i into stage s;
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
     unsigned g = 0, k = 0;
     for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
       const Place at(a, t, per);
-      const int seen = __ldg(a.lens + at.b), n = ((seen > 0 ? seen : a.S) + BLK - 1) / BLK;
+      const int seen = __ldg(a.lens + at.b), n = (attended_len(seen, a.S) + BLK - 1) / BLK;
       const bool empty = seen == 0;
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
       const float* win = windows + (k & 1) * wfloats;
@@ -529,7 +533,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
         if (c == CH - 1) warp_arrive(bars.taken + (k & 1), lane);
         if (q < a.S && half * 32 + 64 * c < HD) store_row<T>(out + half * 32 + 64 * c, v, f);
       }
-      if (half == 0) a.lse[(size_t)at.bh * a.Sp + q] = q < a.S ? (m - up) + lg2(l) : INFINITY;
+      if (half == 0) a.lse[(size_t)at.bh * a.Sp + q] = q < a.S ? m + (lg2(l) - up) : INFINITY;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
     }
   }
@@ -591,10 +595,10 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
     unsigned g = 0, k = 0;
     for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
       const Place at(a, t, per);
-      const int seen = __ldg(a.lens + at.b), n = ((seen > 0 ? seen : a.S) + BLK - 1) / BLK;
-      const bool empty = seen == 0;
+      const int seen = __ldg(a.lens + at.b), n = (attended_len(seen, a.S) + BLK - 1) / BLK;
+      const bool flat = seen <= 0;
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
-      const float lse = q < a.S ? __ldg(a.lse + (size_t)at.bh * a.Sp + q) - a.grad_log2 : INFINITY;
+      const float lse = q < a.S ? (seen < 0 ? 0.f : __ldg(a.lse + (size_t)at.bh * a.Sp + q)) - a.grad_log2 : INFINITY;
       const float* win = windows + (k & 1) * wfloats;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
       const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S + half * 32;
@@ -615,8 +619,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + half * 32;                  // of this warp's columns
         const int dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;
-        const bool far_piece = empty || dhi <= -wd || dlo >= wd;
-        const float far_bias = empty ? 0.f : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
+        const bool far_piece = flat || dhi <= -wd || dlo >= wd;
+        const float far_bias = flat ? 0.f : dhi <= -wd ? win[0] : win[2 * wd + 2 * PAD];
         const uint32_t on = bits[k0 >> 5];
         const auto piece = [&](auto way) {
           using W = decltype(way);
@@ -624,7 +628,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
           tmem_ld2x32(row_s, row_s + 64, s, dp);
           warp_arrive(&bars.read, lane);
           if (i + 1 == n && lane == 0) tc::mbar_arrive(&bars.freed);
-          exponents<W>(s, a.scale_log2, empty, far_bias, win + (k0 - q) + wd + PAD, -lse);
+          exponents<W>(s, a.scale_log2, flat, far_bias, win + (k0 - q) + wd + PAD, -lse);
           if constexpr (W::MASK) mask_columns(s, on);
           uint32_t r[16];
 #pragma unroll
@@ -641,14 +645,14 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
             float x, y;
             sum = v2_fma(pr, v, sum);
             v2_get(pr * (v + nd), x, y);
-            r[j / 2] = W::MASK && empty ? 0u : pack16<T>(x, y);
+            r[j / 2] = W::MASK && flat ? 0u : pack16<T>(x, y);
           }
           tc::tmem_st16(row_ds + (g & 1) * 32, r);           // the product before last has read it: it was issued before these scores
           tc::tmem_wait_st();
         };
         wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
         tc::tc_fence_after();
-        if (on != 0xffffffffu || empty) {
+        if (on != 0xffffffffu || flat) {
           if (far_piece) piece(Way<true, true>());
           else piece(Way<false, true>());
         } else {
@@ -675,7 +679,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       warp_arrive(bars.taken + (k & 1), lane);
 #pragma unroll
       for (int c = 0; c < HDP / 64; ++c) {
-        if (empty) {
+        if (flat) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[c][j] = 0.f;
         }
@@ -725,8 +729,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   // a tile without an attended key has no gradient and no blocks
   const auto blocks = [&](int t) {
     const Place at = place(t);
-    const int seen = __ldg(a.lens + at.b);
-    return at.row0 < (seen > 0 ? seen : a.S) ? nq : 0;
+    return at.row0 < attended_len(__ldg(a.lens + at.b), a.S) ? nq : 0;
   };
   if (warp == WORKERS) {
     unsigned g = 0, k = 0, turn = 0;
@@ -837,7 +840,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       T* const out_v = a.dv + ((size_t)at.b * a.S + key) * a.lddv + at.h * HD;
       T* const out_k = a.dk + ((size_t)at.b * a.S + key) * a.lddk + at.h * HD;
       float* const out_w = a.dwin + ((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin;
-      const bool empty = __ldg(a.lens + at.b) == 0;
+      const bool flat = __ldg(a.lens + at.b) <= 0;
       const float* win = windows + (k & 1) * wfloats;
       const bool on = reinterpret_cast<const uint32_t*>(win + window_floats(wd))[key >> 5] >> (key & 31) & 1u;
       float far[2] = {};
@@ -849,7 +852,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         const float* wp = on ? win + (key - q0) + wd + PAD : s_none + 31;
         const float4* lse = reinterpret_cast<const float4*>(stage + (g % NST) * STAGE_UP + 2 * PIECE + half * 128);
         const float4* del = lse + BLK / 4;
-        const auto piece = [&](auto way) {                   // MASK: an empty sequence, whose scores are zeros and which has no dS
+        const auto piece = [&](auto way) {                   // MASK: a flat sequence, whose scores are zeros and which has no dS
           using W = decltype(way);
           float s[32], dp[32];
           tmem_ld2x32(row_s, row_s + 64, s, dp);
@@ -864,7 +867,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
             for (int e = 0; e < 2; ++e) {
               const int c = j + 2 * e;
               float x, y;
-              if constexpr (W::MASK) v2_get(ls[e], x, y);
+              if constexpr (W::MASK) v2_get(ls[e] + v2(on ? 0.f : -INFINITY), x, y);
               else if constexpr (W::FAR) v2_get(v2_fma(v2(s[c], s[c + 1]), scale, ls[e] + fb), x, y);
               else v2_get(v2_fma(v2(s[c], s[c + 1]), scale, v2(wp[-c], wp[-c - 1])) + ls[e], x, y);
               const V2 pr = v2(ex2(x), ex2(y));
@@ -918,7 +921,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         };
         wait.all(bars.scores + (g & 1), g >> 1, tc::SITE_TMEM_FULL);
         tc::tc_fence_after();
-        if (empty) piece(Way<true, true>());
+        if (flat) piece(Way<true, true>());
         else if (far_piece) piece(Way<true, false>());
         else piece(Way<false, false>());
       }
@@ -949,7 +952,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           float v[32];
           tc::tmem_ld32(row_acc + o * HDP + 64 * c, v);
           if (o == 1 && c == CH - 1) warp_arrive(bars.taken + (k & 1), lane);
-          if (o == 1 && empty) {
+          if (o == 1 && flat) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.f;
           }

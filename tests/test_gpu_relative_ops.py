@@ -85,10 +85,16 @@ def test_attention_map_in_any_order():
     a.check()
 
 
+@pytest.mark.parametrize("dt", HALF)
 @pytest.mark.parametrize("p", [0.0, 0.2])
-def test_attention_of_single_tokens_has_no_gradient_but_of_v(p):
-    """One key: P is 1 whatever the scores are, so their gradients are zeros, not rounding."""
-    a = Attention(attention_inputs(5, 1, 2, 64, torch.bfloat16, "full"), p=p)
+@pytest.mark.parametrize("S", [1, 20, 64, 150])
+def test_attention_of_single_keys_has_no_gradient_but_of_v(S, p, dt):
+    """One attended key: P is 1 whatever the scores are, so their gradients are zeros, not rounding."""
+    c = attention_inputs(5, S, 2, 64, dt, "full", poison=False)
+    c["mask"][:] = 0
+    for i in range(5):
+        c["mask"][i, (i * 37) % S] = 1
+    a = Attention(c, p=p)
     a.fwd()
     a.bwd()
     a.check()
