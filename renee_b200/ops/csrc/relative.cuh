@@ -56,8 +56,8 @@ constexpr int PAD = 128;
 __host__ __device__ __forceinline__ int window_floats(int wd) { return (2 * wd + 1 + 2 * PAD + 3) / 4 * 4; }
 __host__ __device__ __forceinline__ int mask_words(int S) { return (S + 127) / 128 * 4; }       // whole tiles of 128, zeros behind S
 
-// Keys of a sequence that are looked at
-__device__ __forceinline__ int attended_len(int seen, int S) { return seen == 0 ? S : abs(seen); }
+// Keys of a sequence that are looked at (never more than there are, whatever the workspace holds)
+__device__ __forceinline__ int attended_len(int seen, int S) { return seen == 0 ? S : min(abs(seen), S); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -218,7 +218,7 @@ struct Tiles {
   __device__ __forceinline__ Tiles(int* c, int lane) : counter(c), now(blockIdx.x) { next = ask(lane); }
   __device__ __forceinline__ int ask(int lane) {
     int t = 0;
-    if (lane == 0) t = (int)gridDim.x + atomicAdd(counter, 1);
+    if (lane == 0) t = (int)gridDim.x + max(atomicAdd(counter, 1), 0);
     return __shfl_sync(0xffffffffu, t, 0);
   }
   __device__ __forceinline__ void step(int lane) {

@@ -24,6 +24,8 @@ from ..utils import guard
 
 HEAD_DIMS = (32, 64, 128)
 MAX_DISTANCE = 512                # of the bucket map: the window of sums by distance lives in shared memory
+MAX_TOKENS = 65536                # of a sequence on the GPU: its mask lives there too, as bits
+MAX_DROPOUT = 0.99                # fp16 probabilities carry 1 / (1 - p) and a power of two up to 2^8 in the backward pass
 GELU8_BLOCK = 128                 # neighbouring values of a row that share a scale
 
 
@@ -173,7 +175,7 @@ def qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions=None) -> Non
 def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions=None) -> None:
     """Gradients of :func:`qk_norm_rotary_fwd` from its own inputs: ``dx`` (may be ``dy`` itself), ``dgq``, ``dgk`` (all written,
     not accumulated)."""
-    key = ("rotary'", _current(x), S, nh, eps, *_sig(x, gq, gk, table, dy, dx, dgq, dgk), ws.numel(), ws.device,
+    key = ("rotary'", _current(x), S, nh, eps, *_sig(x, gq, gk, table, dy, dx, dgq, dgk), ws.numel(), ws.dtype, ws.device,
            *(_sig(positions) if positions is not None else ()))
     if _first_time(key):
         hd = _check_rotary(x, gq, gk, table, S, nh, eps, positions, dy=dy, dx=dx)
@@ -219,6 +221,8 @@ class RelativeWorkspace:
         self.lse, self.win, self.bits, self.lens, self.stats, self.dwin = lse, win, bits, lens, stats, dwin
         self.status = _cuda().workspace(lse.device).status if lse.is_cuda else None      # where waits that run out are noted
         self.sizes = (lse.device, *(t.numel() for t in (lse, win, bits, lens, stats, dwin)))
+        self.filled = None                                   # what the last forward call was for
+        lens.zero_()                                         # before a forward call: nothing that leads out of the buffers
 
 
 def _relative_sizes(b: int, S: int, nh: int, far: int) -> tuple:
@@ -234,7 +238,7 @@ def relative_attention_workspace(b: int, S: int, nh: int, hd: int, max_distance:
     if torch.device(device).type == "cpu":
         return RelativeWorkspace(*[torch.empty(0)] * 6)
     _refuse(hd not in HEAD_DIMS or dtype not in (torch.bfloat16, torch.float16), f"no kernels for heads of {hd} in {dtype}")
-    _refuse(b < 0 or S < 1 or nh < 1 or not 0 <= max_distance <= MAX_DISTANCE, f"no workspace for {b} x {S} tokens, {nh} heads, distance {max_distance}")
+    _refuse(b < 0 or not 1 <= S <= MAX_TOKENS or nh < 1 or not 0 <= max_distance <= MAX_DISTANCE, f"no workspace for {b} x {S} tokens, {nh} heads, distance {max_distance}")
     made = []
     for name, n, dtype in zip(("lse", "win", "bits", "lens", "stats", "dwin"), _relative_sizes(b, S, nh, max_distance),
                               (torch.float32, torch.float32, torch.int32, torch.int32, torch.float32, torch.float32)):
@@ -257,11 +261,12 @@ def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
     n = buckets.numel()
     _refuse(n % 2 == 0 or n > 2 * MAX_DISTANCE + 1, f"buckets must be [2 far + 1] with far <= {MAX_DISTANCE}, not [{n}]")
     _whole("buckets", buckets, (n,), torch.int32)
-    _refuse(not 0.0 <= p < 1.0, f"dropout probability {p}")
+    _refuse(not 0.0 <= p <= MAX_DROPOUT, f"dropout probability {p}: 0 to {MAX_DROPOUT}")
     _refuse(p > 0.0 and rng is None, "dropout needs the step's seed")
     if q.is_cuda:
         _refuse(p > 0.0 and (rng.dev is None or rng.dev.dtype != torch.int32 or rng.dev.device != q.device),
                 "dropout needs the step's seed as an int32 tensor on the device")
+        _refuse(S > MAX_TOKENS, f"sequences of {S} tokens: the kernels have at most {MAX_TOKENS}")
         _refuse(b * nh * ((S + 15) // 16) >= 2 ** 31, f"{b} sequences of {S} tokens with {nh} heads are too many for one call")
     _same_place(q, k=k, v=v, mask=mask, table=table, buckets=buckets, **like_q)
     return b, S, hd
@@ -278,7 +283,8 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ct
 
     ``q``, ``k``, ``v`` ``[b S, nh hd]``, biases added, rows may lie apart (views of one projection); ``mask`` ``[b, S]`` int32, 0 =
     masked key: it counts as absent, whatever its row holds.  A sequence without any attended key attends to all of its tokens
-    alike, as :func:`renee_b200.ops.attention_fwd` has it.  ``table`` ``[buckets, nh]`` in the activations' type, ``buckets`` from
+    alike, as :func:`renee_b200.ops.attention_fwd` has it.  A distance whose table entry is minus infinity (or beyond -2.3e38) is
+    not attended at; a query to which nothing else is left gives NaN.  ``table`` ``[buckets, nh]`` in the activations' type, ``buckets`` from
     :func:`relative_buckets` (or any int32 map of ``2 far + 1`` distances).  ``ctx_out`` ``[b S, nh hd]``, contiguous.  ``ws``
     (:func:`relative_attention_workspace`) receives what the backward pass needs."""
     key = ("relative", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, ctx_out), ws.sizes,
@@ -292,13 +298,14 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ct
         _passed(key)
     at = _pointers((ctx_out,), (q, k, v, table))
     if q.is_cuda:
+        ws.filled = (mask.shape, nh, buckets.shape)
         return _cuda().relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws)
     ctx_out.copy_(ref.relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream))
 
 
 def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stream, ctx, ws, dq, dk, dv, dtable) -> None:
     """Gradients of :func:`relative_attention_fwd` from its inputs, its output ``ctx`` and the workspace it filled: ``dq``, ``dk``,
-    ``dv`` (rows may lie apart) and ``dtable`` ``[buckets, nh]``, all written, not accumulated."""
+    ``dv`` (rows may lie apart) and ``dtable`` ``[buckets, nh]``, all written, not accumulated.  May be called again."""
     key = ("relative'", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, dctx, ctx, dq, dk, dv, dtable), ws.sizes,
            *(_sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else ()))
     if _first_time(key):
@@ -312,6 +319,7 @@ def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stre
         _passed(key)
     at = _pointers((dq, dk, dv, dtable), (q, k, v, dctx, ctx, table))
     if q.is_cuda:
+        _refuse(ws.filled != (mask.shape, nh, buckets.shape), "the workspace was not filled by the forward call of these sizes")
         return _cuda().relative_attention_bwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws, dq, dk, dv)
     g = ref.relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream)
     for out, t in zip((dq, dk, dv, dtable), g):
@@ -379,7 +387,7 @@ def gelu8_fwd(x, bias, out, saved) -> None:
 def gelu8_bwd(da, saved, ws, dbias, dx, act_out) -> None:
     """From the gradient ``da`` of the activation and the 8 bits: ``dx = da gelu'(z)``, its column sums ``dbias``, and the
     activation ``act_out = gelu(z)`` again (for the weight gradient of the linear that read it).  ``dx`` may be ``da`` itself."""
-    key = ("gelu8'", _current(da), *_sig(da, saved.q, saved.scale, dbias, dx, act_out), ws.numel(), ws.device)
+    key = ("gelu8'", _current(da), *_sig(da, saved.q, saved.scale, dbias, dx, act_out), ws.numel(), ws.dtype, ws.device)
     if _first_time(key):
         T, F = _check_gelu8(saved, da=da, dx=dx, act_out=act_out)
         _whole("dbias", dbias, (F,), da.dtype)

@@ -48,6 +48,13 @@ def views(c):
     return c["qk"][:, :H], c["qk"][:, H:], c["qkv"][:, 2 * H:]
 
 
+def shut_behind(c, value):
+    """Keys behind the query shut out by the table (whose upper half holds their distances); ``value`` None: the type's lowest."""
+    half = c["table"].shape[0] // 2
+    c["table"][half:] = torch.finfo(c["table"].dtype).min if value is None else value
+    return c
+
+
 def attention_64(c, p=0.0, seed=0, stream=0):
     """Outputs and gradients by autograd in 64 bits, and the bounds of a kernel that holds P and dS in 16 bits (relative error u)
     as operands, ctx in 16 bits inside delta, and everything else in fp32.

@@ -6,7 +6,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from renee_b200 import ops
-from tests.relative_cases import (ATTENTION_SHAPES, assert_within, attention_64, attention_inputs, gelu8_64, rotary_64, u_of, views)
+from tests.relative_cases import (ATTENTION_SHAPES, assert_within, attention_64, attention_inputs, gelu8_64, rotary_64, shut_behind, u_of, views)
 
 HALF = [torch.bfloat16, torch.float16]
 
@@ -127,6 +127,66 @@ def test_attention_of_an_empty_sequence_reads_no_scores(S):
     clean.check()
     assert torch.equal(clean.ctx, dirty.ctx) and torch.equal(clean.wide, dirty.wide) and torch.equal(clean.dtable, dirty.dtable)
     assert not dirty.dq[S:2 * S].any() and not dirty.dk[S:2 * S].any()
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("shut", [float("-inf"), None])
+@pytest.mark.parametrize("S,far", [(20, 9), (60, 9), (200, 9), (300, 128)])
+def test_attention_of_distances_that_are_shut(S, far, shut, dt):
+    a = Attention(shut_behind(attention_inputs(2, S, 2, 64, dt, "padded", far=far, poison=False), shut))
+    a.fwd()
+    a.bwd()
+    a.check()
+    assert not a.dtable[4:].any()
+
+
+@pytest.mark.parametrize("S", [30, 64, 70, 129, 200])
+def test_attention_in_a_larger_workspace_and_backward_again(S):
+    """A workspace for more sequences of more tokens, used for larger and smaller calls in turn; each backward pass runs twice."""
+    ws = ops.relative_attention_workspace(5, 200, 2, 64, 9, torch.bfloat16, dev())
+    for b, s in ((5, 200), (2, S), (5, 200), (1, S)):
+        a = Attention(attention_inputs(b, s, 2, 64, torch.bfloat16, "holes"))
+        a.ws = ws
+        a.fwd()
+        for _ in range(2):
+            a.wide.fill_(7.0)
+            a.dtable.fill_(7.0)
+            a.bwd()
+            a.check()
+
+
+def test_attention_on_two_streams_at_once():
+    torch.cuda.synchronize()
+    calls = [Attention(attention_inputs(3, 300, 2, 64, torch.float16, "padded", seed=s), p=0.1) for s in range(2)]
+    torch.cuda.synchronize()
+    for a, stream in zip(calls, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        with torch.cuda.stream(stream):
+            for _ in range(4):
+                a.fwd()
+                a.bwd()
+    torch.cuda.synchronize()
+    for a in calls:
+        a.check()
+
+
+@pytest.mark.parametrize("dt", HALF)
+def test_attention_of_the_longest_sequence(dt):
+    """65536 tokens, more than 2^32 pairs, with queries, keys and biases of zero: P = 1 / S, each product a mean."""
+    S, hd = 65536, 128
+    g = torch.Generator().manual_seed(0)
+    c = dict(qk=torch.zeros(S, 2 * hd, dtype=dt), qkv=torch.randn(S, 3 * hd, generator=g).to(dt), mask=torch.ones(1, S, dtype=torch.int32),
+             table=torch.zeros(64, 1, dtype=dt), buckets=ops.relative_buckets(64, 512), dctx=torch.randn(S, hd, generator=g).to(dt), nh=1, hd=hd, b=1, S=S)
+    c["qkv"] += 1
+    c["dctx"] += 1
+    a = Attention(c)
+    a.fwd()
+    a.bwd()
+    # P and, in the backward pass, P~ are powers of two: exact; fp32 sums of S products of values up to 2^3: 2^-24 S^(1/2) 2^3 of
+    # their mean at the most; then one rounding to 16 bits of a value near 1
+    tol = u_of(dt) * 1.5 + 2.0 ** -13
+    assert (a.ctx.float() - c["qkv"][:, 2 * hd:].double().mean(0).float().to(dev())).abs().max() <= tol
+    assert (a.dv.float() - c["dctx"].double().mean(0).float().to(dev())).abs().max() <= tol
+    assert not a.dq.any() and not a.dk.any()
 
 
 def test_attention_same_bits_again():
@@ -283,6 +343,23 @@ def test_refusals_on_the_device():
         ops.relative_attention_fwd(a.q, a.k, a.v, a.g["mask"].cpu(), *a.args()[1:], a.ctx, a.ws)
     with pytest.raises(ValueError):                              # dropout without the seed on the device
         ops.relative_attention_fwd(a.q, a.k, a.v, *a.args()[:4], 0.1, ops.StepRNG(3), 1, a.ctx, a.ws)
+    with pytest.raises(ValueError, match="not filled"):          # backward before forward, and behind one of other sizes
+        a.bwd()
+    a.fwd()
+    other = Attention(attention_inputs(1, 40, 2, 64, torch.bfloat16))
+    other.ws = a.ws
+    with pytest.raises(ValueError, match="not filled"):
+        other.bwd()
+    n = 65537
+    x = torch.zeros(n, 32, dtype=torch.bfloat16, device=dev())
+    with pytest.raises(ValueError, match="at most 65536"):
+        ops.relative_attention_fwd(x, x.clone(), x.clone(), torch.ones(1, n, dtype=torch.int32, device=dev()), torch.zeros(8, 1, dtype=torch.bfloat16, device=dev()),
+                                   a.g["buckets"], 1, 0.0, None, 0, torch.zeros_like(x), a.ws)
     x = torch.zeros(4, 128, device=dev())
     with pytest.raises(ValueError):
         ops.gelu8_fwd(x, torch.zeros(128, device=dev()), x, ops.gelu8_saved(4, 128, "cpu"))
+    ops.gelu8_fwd(x, torch.zeros(128, device=dev()), torch.zeros_like(x), saved := ops.gelu8_saved(4, 128, dev()))
+    args = (x, saved, ops.gelu8_workspace(4, 128, dev()), torch.zeros(128, device=dev()), torch.zeros_like(x), torch.zeros_like(x))
+    ops.gelu8_bwd(*args)
+    with pytest.raises(ValueError, match="workspace"):           # the same sizes with a workspace of another type
+        ops.gelu8_bwd(*args[:2], args[2].half(), *args[3:])

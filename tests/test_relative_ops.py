@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from renee_b200 import ops
-from tests.relative_cases import ATTENTION_SHAPES, attention_64, attention_inputs, gelu8_64, rotary_64, views
+from tests.relative_cases import ATTENTION_SHAPES, assert_within, attention_64, attention_inputs, gelu8_64, rotary_64, shut_behind, views
 
 
 def run_attention(c, p=0.0, seed=5, stream=3):
@@ -54,6 +54,17 @@ def test_masked_keys_do_not_matter():
     ra, rb = run_attention(a), run_attention(b)
     for n in ra:
         torch.testing.assert_close(ra[n], rb[n], rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("shut", [float("-inf"), None])
+def test_attention_of_distances_that_are_shut(shut):
+    """A table entry of minus infinity, or the type's lowest value, takes its distances out."""
+    c = shut_behind(attention_inputs(2, 20, 2, 32, torch.float32, "padded", poison=False), shut)
+    want, lim = attention_64(c)
+    got = run_attention(c)
+    for name in want:
+        assert_within(name, got[name], want[name], lim[name])
+    assert not got["dtable"][4:].any()
 
 
 def test_buckets():
@@ -145,7 +156,7 @@ def _attention_call(**change):
     dict(q=torch.zeros(16, 60)), dict(q=torch.zeros(15, 64)), dict(nh=3), dict(nh=0), dict(k=torch.zeros(16, 64, dtype=torch.bfloat16)),
     dict(v=torch.zeros(64, 16).t()), dict(mask=torch.ones(2, 8)), dict(mask=torch.ones(2, 0, dtype=torch.int32)), dict(mask=torch.ones(16, dtype=torch.int32)),
     dict(table=torch.zeros(8, 3)), dict(table=torch.zeros(0, 2)), dict(buckets=torch.zeros(4, dtype=torch.int32)), dict(buckets=torch.zeros(9)),
-    dict(buckets=torch.zeros(5001, dtype=torch.int32)), dict(p=1.0), dict(p=-0.1), dict(p=0.5), dict(ctx_out=torch.zeros(16, 128)[:, :64]),
+    dict(buckets=torch.zeros(5001, dtype=torch.int32)), dict(p=1.0), dict(p=0.995), dict(p=-0.1), dict(p=0.5), dict(ctx_out=torch.zeros(16, 128)[:, :64]),
     dict(q=torch.zeros(16 * 64 + 1)[1:].view(16, 64)), dict(q=torch.zeros(16 * 66).as_strided((16, 64), (66, 1)))])
 def test_attention_refuses(change):
     with pytest.raises(ValueError):
