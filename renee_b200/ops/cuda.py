@@ -434,27 +434,22 @@ def _call_typed(name, device, *args, launches=1):
     _LAUNCHES += launches
 
 
-def _ld(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def qk_norm_rotary_blocks(T: int, nh: int, hd: int) -> int:
     return lib().rb_qk_norm_rotary_blocks(_LL(T), _I(nh), _I(hd))
 
 
-def qk_norm_rotary_fwd(at, x, table, S, nh, hd, eps, out, positions):
-    y, x_, gq, gk, table_ = at
-    T = x.shape[0]
-    _call_typed("rb_qk_norm_rotary_fwd", x.device, DT[x.dtype], x_, _ld(x), gq, gk, table_, None if positions is None else positions.data_ptr(),
-                y, _ld(out), T, table.shape[0], S, nh, hd, eps, launches=1 if T else 0)
+def qk_norm_rotary_fwd(at, numbers, x, positions):
+    y, x_, gq, gk, table = at
+    ldx, ldy, sizes = numbers
+    _call_typed("rb_qk_norm_rotary_fwd", x.device, DT[x.dtype], x_, ldx, gq, gk, table, None if positions is None else positions.data_ptr(),
+                y, ldy, *sizes, launches=1 if sizes[0] else 0)
 
 
-def qk_norm_rotary_bwd(at, dy, x, table, S, nh, hd, eps, ws, dx, positions):
-    dx_, dgq, dgk, x_, gq, gk, table_ = at
-    T = x.shape[0]
-    _call_typed("rb_qk_norm_rotary_bwd", x.device, DT[x.dtype], dy.data_ptr(), _ld(dy), x_, _ld(x), gq, gk, table_,
-                None if positions is None else positions.data_ptr(), ws.data_ptr(), dx_, _ld(dx), dgq, dgk, T, table.shape[0], S, nh, hd, eps,
-                launches=2 if T else 1)
+def qk_norm_rotary_bwd(at, numbers, dy, x, ws, positions):
+    lddy, ldx, lddx, sizes = numbers
+    _call_typed("rb_qk_norm_rotary_bwd", x.device, DT[x.dtype], dy, lddy, at[3], ldx, at[4], at[5], at[6],
+                None if positions is None else positions.data_ptr(), ws.data_ptr(), at[0], lddx, at[1], at[2], *sizes,
+                launches=2 if sizes[0] else 1)
 
 
 def relative_tiles(S: int) -> int:
@@ -465,39 +460,34 @@ def relative_window_floats(far: int, S: int) -> int:
     return lib().rb_relative_window_floats(_I(far), _I(S))
 
 
-def _relative_inputs(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):
-    b, S = mask.shape
-    return (at[0], _ld(q), at[1], _ld(k), at[2], _ld(v), (buckets.shape[0] - 1) // 2, table.shape[0], b, S, nh, q.shape[1] // nh,
-            ws.win.data_ptr(), ws.bits.data_ptr(), ws.lens.data_ptr(), p, rng.dev.data_ptr() if p > 0 else None, stream, ws.status.data_ptr())
+def relative_attention_fwd(at, numbers, q, mask, buckets, p, rng, stream, ws):
+    ctx, q_, k, v, table = at
+    ldq, ldk, ldv, sizes = numbers
+    _call_typed("rb_relative_fwd", q.device, DT[q.dtype], q_, ldq, k, ldk, v, ldv, *sizes, *ws.at, p, rng.dev.data_ptr() if p > 0 else None,
+                stream, ws.status.data_ptr(), mask.data_ptr(), table, buckets.data_ptr(), ctx, ws.lse.data_ptr(), launches=2 if sizes[2] else 0)
 
 
-def relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws):
-    _call_typed("rb_relative_fwd", q.device, DT[q.dtype], *_relative_inputs(at[1:4], q, k, v, mask, table, buckets, nh, p, rng, stream, ws),
-                mask.data_ptr(), table.data_ptr(), buckets.data_ptr(), at[0], ws.lse.data_ptr(), launches=2 if mask.shape[0] else 0)
-
-
-def relative_attention_bwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws, dq, dk, dv):
-    dq_, dk_, dv_, dtable, _, _, _, dctx, ctx, _ = at
-    _call_typed("rb_relative_bwd", q.device, DT[q.dtype], dctx,
-                *_relative_inputs(at[4:7], q, k, v, mask, table, buckets, nh, p, rng, stream, ws), buckets.data_ptr(), ctx, ws.lse.data_ptr(),
-                ws.stats.data_ptr(), ws.dwin.data_ptr(), dq_, _ld(dq), dk_, _ld(dk), dv_, _ld(dv), dtable,
-                launches=1 + (0 if not mask.shape[0] else 2 if mask.shape[1] > 64 else 1))
+def relative_attention_bwd(at, numbers, q, buckets, p, rng, stream, ws):
+    dq, dk, dv, dtable, q_, k, v, dctx, ctx, _ = at
+    ldq, ldk, ldv, sizes, lddq, lddk, lddv = numbers
+    _call_typed("rb_relative_bwd", q.device, DT[q.dtype], dctx, q_, ldq, k, ldk, v, ldv, *sizes, *ws.at, p,
+                rng.dev.data_ptr() if p > 0 else None, stream, ws.status.data_ptr(), buckets.data_ptr(), ctx, ws.lse.data_ptr(),
+                ws.stats.data_ptr(), ws.dwin.data_ptr(), dq, lddq, dk, lddk, dv, lddv, dtable,
+                launches=1 + (0 if not sizes[2] else 2 if sizes[3] > 64 else 1))
 
 
 def gelu8_splits(T: int, F: int) -> int:
     return lib().rb_gelu8_splits(_LL(T), _I(F))
 
 
-def gelu8_fwd(x, bias, out, saved):
+def gelu8_fwd(x, x_, bias, out, q, scale):
     T, F = x.shape
-    _call_typed("rb_gelu8_fwd", x.device, DT[x.dtype], x.data_ptr(), bias.data_ptr(), out.data_ptr(), saved.q.data_ptr(), saved.scale.data_ptr(),
-                T, F, launches=1 if T else 0)
+    _call_typed("rb_gelu8_fwd", x.device, DT[x.dtype], x_, bias, out, q, scale.data_ptr(), T, F, launches=1 if T else 0)
 
 
-def gelu8_bwd(da, saved, ws, dbias, dx, act_out):
+def gelu8_bwd(da, da_, q, scale, ws, dbias, dx, act):
     T, F = da.shape
-    _call_typed("rb_gelu8_bwd", da.device, DT[da.dtype], da.data_ptr(), saved.q.data_ptr(), saved.scale.data_ptr(), ws.data_ptr(), dbias.data_ptr(),
-                dx.data_ptr(), act_out.data_ptr(), T, F, launches=2 if T else 1)
+    _call_typed("rb_gelu8_bwd", da.device, DT[da.dtype], da_, q, scale.data_ptr(), ws.data_ptr(), dbias, dx, act, T, F, launches=2 if T else 1)
 
 
 # ----------------------------------------------------------------------------- encoder GEMMs (tcgen05, fused epilogues)

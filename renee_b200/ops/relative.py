@@ -29,9 +29,15 @@ MAX_DROPOUT = 0.99                # fp16 probabilities carry 1 / (1 - p) and a p
 GELU8_BLOCK = 128                 # neighbouring values of a row that share a scale
 
 
+_CU = None
+
+
 def _cuda():
-    from . import cuda as cu
-    return cu
+    global _CU
+    if _CU is None:
+        from . import cuda
+        _CU = cuda
+    return _CU
 
 
 def _refuse(cond: bool, what: str) -> None:
@@ -39,31 +45,25 @@ def _refuse(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
-# Checks that depend on shapes, strides, types, devices and numbers alone are made once for each combination: they cost 25 us in
-# Python where the kernels of a small call take 5.  Pointers (alignment, outputs that are inputs) are looked at on every call.
-_CHECKED: set = set()
+# Checks that depend on shapes, strides, types, devices and numbers alone are made once for each combination (its key, written out
+# in each function: loops over the tensors cost half as much again) and leave the kernels' numbers that follow from it: they cost
+# 25 us in Python where the kernels of a small call take 5.  Pointers (alignment, outputs that are inputs) are looked at on every call.
+_CHECKED: dict = {}
 
 
-def _sig(*tensors) -> list:
-    out = []
-    for t in tensors:
-        out += (t.shape, t.stride(), t.dtype, t.device)
-    return out
-
-
-def _first_time(key: tuple) -> bool:
-    return key not in _CHECKED
-
-
-def _passed(key: tuple) -> None:
+def _passed(key: tuple, numbers: tuple) -> tuple:
     if len(_CHECKED) >= 4096:
         _CHECKED.clear()
-    _CHECKED.add(key)
+    _CHECKED[key] = numbers
+    return numbers
 
 
-def _current(t: torch.Tensor) -> int:
-    """The device that a call's kernels would run on (part of the key: the tensors' must be the current one)."""
-    return torch.cuda.current_device() if t.is_cuda else -1
+def _sig(*tensors) -> tuple:
+    return tuple((t.shape, t.stride(), t.dtype, t.device) for t in tensors)
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _same_place(first: torch.Tensor, **others) -> None:
@@ -88,20 +88,18 @@ def _whole(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None
         raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)}, not {t.dtype} {list(t.shape)}")
 
 
-def _pointers(outputs: tuple, inputs: tuple) -> list:
-    """Addresses of outputs, then inputs.  All must be 16-byte aligned, and no output may start where an input or another output
-    does (what one kernel writes a later one would read); tensors without elements have none."""
-    out, inp = [t.data_ptr() for t in outputs], [t.data_ptr() for t in inputs]
+def _pointers(n_out: int, *tensors) -> list:
+    """Addresses of the ``n_out`` outputs, then of the inputs.  All must be 16-byte aligned, and no output may start where an input
+    or another output does (what one kernel writes a later one would read); tensors without elements have none."""
+    at = [t.data_ptr() for t in tensors]
     every = 0
-    for a in out:
-        every |= a
-    for a in inp:
+    for a in at:
         every |= a
     _refuse(every & 15 != 0, "every tensor must start on a 16-byte boundary")
-    for i, a in enumerate(out):
-        if a and (a in inp or a in out[:i]):
+    for i in range(n_out):
+        if at[i] and at.count(at[i]) > 1:
             raise ValueError("an output is the same memory as another tensor of the call")
-    return out + inp
+    return at
 
 
 def _head_dim(cols: int, nh: int, on_gpu: bool) -> int:
@@ -162,22 +160,29 @@ def qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, out, positions=None) -> Non
     their root mean square (``eps`` is added to the mean square), times ``gq`` or ``gk`` ``[hd]``, rotated by the token's position:
     value ``i`` with value ``i + hd/2`` by the angle whose cosine and sine ``table`` (:func:`rotary_table`) holds.  Token ``t`` of
     the padded ``[b, S]`` batch stands at ``t % S``, or at ``positions[t]`` (int32; one outside the table counts as its nearest)."""
-    key = ("rotary", _current(x), S, nh, eps, *_sig(x, gq, gk, table, out), *(_sig(positions) if positions is not None else ()))
-    if _first_time(key):
-        _check_rotary(x, gq, gk, table, S, nh, eps, positions, out=out)
-        _passed(key)
-    at = _pointers((out,), (x, gq, gk, table))
+    key = ("rotary", torch.cuda.current_device() if x.is_cuda else -1, S, nh, eps, x.shape, x.stride(), x.dtype, x.device,
+           gq.shape, gq.stride(), gq.dtype, gq.device, gk.shape, gk.stride(), gk.dtype, gk.device, table.shape, table.stride(),
+           table.dtype, table.device, out.shape, out.stride(), out.dtype, out.device, None if positions is None else _sig(positions))
+    numbers = _CHECKED.get(key)
+    if numbers is None:
+        hd = _check_rotary(x, gq, gk, table, S, nh, eps, positions, out=out)
+        numbers = _passed(key, (_ld(x), _ld(out), (x.shape[0], table.shape[0], S, nh, hd, eps)))
+    at = _pointers(1, out, x, gq, gk, table)
     if x.is_cuda:
-        return _cuda().qk_norm_rotary_fwd(at, x, table, S, nh, gq.shape[0], eps, out, positions)
+        return _cuda().qk_norm_rotary_fwd(at, numbers, x, positions)
     out.copy_(ref.qk_norm_rotary_fwd(x, gq, gk, table, S, nh, eps, positions))
 
 
 def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, positions=None) -> None:
     """Gradients of :func:`qk_norm_rotary_fwd` from its own inputs: ``dx`` (may be ``dy`` itself), ``dgq``, ``dgk`` (all written,
     not accumulated)."""
-    key = ("rotary'", _current(x), S, nh, eps, *_sig(x, gq, gk, table, dy, dx, dgq, dgk), ws.numel(), ws.dtype, ws.device,
-           *(_sig(positions) if positions is not None else ()))
-    if _first_time(key):
+    key = ("rotary'", torch.cuda.current_device() if x.is_cuda else -1, S, nh, eps, x.shape, x.stride(), x.dtype, x.device,
+           gq.shape, gq.stride(), gq.dtype, gq.device, gk.shape, gk.stride(), gk.dtype, gk.device, table.shape, table.stride(),
+           table.dtype, table.device, dy.shape, dy.stride(), dy.dtype, dy.device, dx.shape, dx.stride(), dx.dtype, dx.device,
+           dgq.shape, dgq.stride(), dgq.dtype, dgq.device, dgk.shape, dgk.stride(), dgk.dtype, dgk.device, ws.numel(), ws.dtype,
+           ws.device, None if positions is None else _sig(positions))
+    numbers = _CHECKED.get(key)
+    if numbers is None:
         hd = _check_rotary(x, gq, gk, table, S, nh, eps, positions, dy=dy, dx=dx)
         _whole("dgq", dgq, (hd,), x.dtype)
         _whole("dgk", dgk, (hd,), x.dtype)
@@ -186,11 +191,14 @@ def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, posit
             need = _cuda().qk_norm_rotary_blocks(x.shape[0], nh, hd) * 2 * hd
             _refuse(ws.numel() < need or ws.device != x.device or ws.dtype != torch.float32,
                     f"the workspace is for fewer tokens: {ws.numel()} values on {ws.device}, the call needs {need} on {x.device}")
-        _passed(key)
-    in_place = dx.data_ptr() == dy.data_ptr() and dx.stride() == dy.stride()
-    at = _pointers((dx, dgq, dgk), (x, gq, gk, table) if in_place else (x, gq, gk, table, dy))
+        numbers = _passed(key, (_ld(dy), _ld(x), _ld(dx), (x.shape[0], table.shape[0], S, nh, hd, eps)))
+    dy_ = dy.data_ptr()
+    if dx.data_ptr() == dy_ and dx.stride() == dy.stride():
+        at = _pointers(3, dx, dgq, dgk, x, gq, gk, table)
+    else:
+        at = _pointers(3, dx, dgq, dgk, x, gq, gk, table, dy)
     if x.is_cuda:
-        return _cuda().qk_norm_rotary_bwd(at[:7], dy, x, table, S, nh, gq.shape[0], eps, ws, dx, positions)
+        return _cuda().qk_norm_rotary_bwd(at, numbers, dy_, x, ws, positions)
     g = ref.qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, positions)
     for out, t in zip((dx, dgq, dgk), g):
         out.copy_(t)
@@ -221,6 +229,7 @@ class RelativeWorkspace:
         self.lse, self.win, self.bits, self.lens, self.stats, self.dwin = lse, win, bits, lens, stats, dwin
         self.status = _cuda().workspace(lse.device).status if lse.is_cuda else None      # where waits that run out are noted
         self.sizes = (lse.device, *(t.numel() for t in (lse, win, bits, lens, stats, dwin)))
+        self.at = (win.data_ptr(), bits.data_ptr(), lens.data_ptr())
         self.filled = None                                   # what the last forward call was for
         lens.zero_()                                         # before a forward call: nothing that leads out of the buffers
 
@@ -272,6 +281,10 @@ def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
     return b, S, hd
 
 
+def _seed_sig(p, rng):
+    return _sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else None
+
+
 def _check_ws(ws, device, need) -> None:
     at, *have = ws.sizes
     _refuse(at != device or any(h < n for h, n in zip(have, need)),
@@ -287,40 +300,50 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ct
     not attended at; a query to which nothing else is left gives NaN.  ``table`` ``[buckets, nh]`` in the activations' type, ``buckets`` from
     :func:`relative_buckets` (or any int32 map of ``2 far + 1`` distances).  ``ctx_out`` ``[b S, nh hd]``, contiguous.  ``ws``
     (:func:`relative_attention_workspace`) receives what the backward pass needs."""
-    key = ("relative", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, ctx_out), ws.sizes,
-           *(_sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else ()))
-    if _first_time(key):
+    key = ("relative", torch.cuda.current_device() if q.is_cuda else -1, nh, p, q.shape, q.stride(), q.dtype, q.device,
+           k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, mask.shape, mask.stride(), mask.dtype,
+           mask.device, table.shape, table.stride(), table.dtype, table.device, buckets.shape, buckets.stride(), buckets.dtype,
+           buckets.device, ctx_out.shape, ctx_out.stride(), ctx_out.dtype, ctx_out.device, ws.sizes, _seed_sig(p, rng))
+    numbers = _CHECKED.get(key)
+    if numbers is None:
         b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng)
         _whole("ctx_out", ctx_out, (b * S, nh * hd), q.dtype)
         _same_place(q, ctx_out=ctx_out)
+        far = (buckets.numel() - 1) // 2
         if q.is_cuda:
-            _check_ws(ws, q.device, _relative_sizes(b, S, nh, (buckets.numel() - 1) // 2)[:4])
-        _passed(key)
-    at = _pointers((ctx_out,), (q, k, v, table))
+            _check_ws(ws, q.device, _relative_sizes(b, S, nh, far)[:4])
+        numbers = _passed(key, (_ld(q), _ld(k), _ld(v), (far, table.shape[0], b, S, nh, hd)))
+    at = _pointers(1, ctx_out, q, k, v, table)
     if q.is_cuda:
-        ws.filled = (mask.shape, nh, buckets.shape)
-        return _cuda().relative_attention_fwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws)
+        ws.filled = numbers[3]
+        return _cuda().relative_attention_fwd(at, numbers, q, mask, buckets, p, rng, stream, ws)
     ctx_out.copy_(ref.relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream))
 
 
 def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stream, ctx, ws, dq, dk, dv, dtable) -> None:
     """Gradients of :func:`relative_attention_fwd` from its inputs, its output ``ctx`` and the workspace it filled: ``dq``, ``dk``,
     ``dv`` (rows may lie apart) and ``dtable`` ``[buckets, nh]``, all written, not accumulated.  May be called again."""
-    key = ("relative'", _current(q), nh, p, *_sig(q, k, v, mask, table, buckets, dctx, ctx, dq, dk, dv, dtable), ws.sizes,
-           *(_sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else ()))
-    if _first_time(key):
+    key = ("relative'", torch.cuda.current_device() if q.is_cuda else -1, nh, p, q.shape, q.stride(), q.dtype, q.device,
+           k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, mask.shape, mask.stride(), mask.dtype,
+           mask.device, table.shape, table.stride(), table.dtype, table.device, buckets.shape, buckets.stride(), buckets.dtype,
+           buckets.device, dctx.shape, dctx.stride(), dctx.dtype, dctx.device, ctx.shape, ctx.stride(), ctx.dtype, ctx.device,
+           dq.shape, dq.stride(), dq.dtype, dq.device, dk.shape, dk.stride(), dk.dtype, dk.device, dv.shape, dv.stride(), dv.dtype,
+           dv.device, dtable.shape, dtable.stride(), dtable.dtype, dtable.device, ws.sizes, _seed_sig(p, rng))
+    numbers = _CHECKED.get(key)
+    if numbers is None:
         b, S, hd = _check_relative(q, k, v, mask, table, buckets, nh, p, rng, dq=dq, dk=dk, dv=dv)
         _whole("dctx", dctx, (b * S, nh * hd), q.dtype)
         _whole("ctx", ctx, (b * S, nh * hd), q.dtype)
         _whole("dtable", dtable, tuple(table.shape), q.dtype)
         _same_place(q, dctx=dctx, ctx=ctx, dtable=dtable)
+        far = (buckets.numel() - 1) // 2
         if q.is_cuda:
-            _check_ws(ws, q.device, _relative_sizes(b, S, nh, (buckets.numel() - 1) // 2))
-        _passed(key)
-    at = _pointers((dq, dk, dv, dtable), (q, k, v, dctx, ctx, table))
+            _check_ws(ws, q.device, _relative_sizes(b, S, nh, far))
+        numbers = _passed(key, (_ld(q), _ld(k), _ld(v), (far, table.shape[0], b, S, nh, hd), _ld(dq), _ld(dk), _ld(dv)))
+    at = _pointers(4, dq, dk, dv, dtable, q, k, v, dctx, ctx, table)
     if q.is_cuda:
-        _refuse(ws.filled != (mask.shape, nh, buckets.shape), "the workspace was not filled by the forward call of these sizes")
-        return _cuda().relative_attention_bwd(at, q, k, v, mask, table, buckets, nh, p, rng, stream, ws, dq, dk, dv)
+        _refuse(ws.filled != numbers[3], "the workspace was not filled by the forward call of these sizes")
+        return _cuda().relative_attention_bwd(at, numbers, q, buckets, p, rng, stream, ws)
     g = ref.relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream)
     for out, t in zip((dq, dk, dv, dtable), g):
         out.copy_(t)
@@ -369,26 +392,33 @@ def gelu8_fwd(x, bias, out, saved) -> None:
     """``out = gelu(x + bias)`` for ``x`` ``[T, F]`` (erf GELU); ``saved`` receives ``x + bias`` in 8 bits: 128 neighbouring
     values of a row share a scale and are held to 1/254 of the largest of them.  A block with an infinity or a NaN stands
     for NaNs.  ``out`` may be ``x`` itself."""
-    key = ("gelu8", _current(x), *_sig(x, bias, out, saved.q, saved.scale))
-    if _first_time(key):
-        _, F = _check_gelu8(saved, x=x, out=out)
+    q, scale = saved.q, saved.scale
+    key = ("gelu8", torch.cuda.current_device() if x.is_cuda else -1, x.shape, x.stride(), x.dtype, x.device, bias.shape, bias.stride(),
+           bias.dtype, bias.device, out.shape, out.stride(), out.dtype, out.device, q.shape, q.stride(), q.dtype, q.device, scale.shape,
+           scale.stride(), scale.dtype, scale.device)
+    if key not in _CHECKED:
+        T, F = _check_gelu8(saved, x=x, out=out)
         _whole("bias", bias, (F,), x.dtype)
         _same_place(x, bias=bias)
-        _passed(key)
-    in_place = out.data_ptr() == x.data_ptr()
-    _pointers((out,), (bias,) if in_place else (bias, x))
-    _refuse(saved.q.data_ptr() % 8 != 0, "saved.q must start on an 8-byte boundary")
+        _passed(key, ())
+    x_, q_ = x.data_ptr(), q.data_ptr()
+    at = _pointers(1, out, bias) if out.data_ptr() == x_ else _pointers(1, out, bias, x)
+    _refuse(q_ % 8 != 0, "saved.q must start on an 8-byte boundary")
     if x.is_cuda:
-        return _cuda().gelu8_fwd(x, bias, out, saved)
-    y, q, scale = ref.gelu8_fwd(x, bias)
-    out.copy_(y); saved.q.copy_(q); saved.scale.copy_(scale)
+        return _cuda().gelu8_fwd(x, x_, at[1], at[0], q_, scale)
+    y, q8, s8 = ref.gelu8_fwd(x, bias)
+    out.copy_(y); q.copy_(q8); scale.copy_(s8)
 
 
 def gelu8_bwd(da, saved, ws, dbias, dx, act_out) -> None:
     """From the gradient ``da`` of the activation and the 8 bits: ``dx = da gelu'(z)``, its column sums ``dbias``, and the
     activation ``act_out = gelu(z)`` again (for the weight gradient of the linear that read it).  ``dx`` may be ``da`` itself."""
-    key = ("gelu8'", _current(da), *_sig(da, saved.q, saved.scale, dbias, dx, act_out), ws.numel(), ws.dtype, ws.device)
-    if _first_time(key):
+    q, scale = saved.q, saved.scale
+    key = ("gelu8'", torch.cuda.current_device() if da.is_cuda else -1, da.shape, da.stride(), da.dtype, da.device, q.shape, q.stride(),
+           q.dtype, q.device, scale.shape, scale.stride(), scale.dtype, scale.device, dbias.shape, dbias.stride(), dbias.dtype,
+           dbias.device, dx.shape, dx.stride(), dx.dtype, dx.device, act_out.shape, act_out.stride(), act_out.dtype, act_out.device,
+           ws.numel(), ws.dtype, ws.device)
+    if key not in _CHECKED:
         T, F = _check_gelu8(saved, da=da, dx=dx, act_out=act_out)
         _whole("dbias", dbias, (F,), da.dtype)
         _same_place(da, dbias=dbias)
@@ -396,11 +426,11 @@ def gelu8_bwd(da, saved, ws, dbias, dx, act_out) -> None:
             need = _cuda().gelu8_splits(T, F) * F
             _refuse(ws.numel() < need or ws.device != da.device or ws.dtype != torch.float32,
                     f"the workspace is for fewer rows: {ws.numel()} values on {ws.device}, the call needs {need} on {da.device}")
-        _passed(key)
-    in_place = dx.data_ptr() == da.data_ptr()
-    _pointers((act_out, dbias) if in_place else (act_out, dbias, dx), (da,))
-    _refuse(saved.q.data_ptr() % 8 != 0, "saved.q must start on an 8-byte boundary")
+        _passed(key, ())
+    da_, dx_, q_ = da.data_ptr(), dx.data_ptr(), q.data_ptr()
+    at = _pointers(2, act_out, dbias, da) if dx_ == da_ else _pointers(3, act_out, dbias, dx, da)
+    _refuse(q_ % 8 != 0, "saved.q must start on an 8-byte boundary")
     if da.is_cuda:
-        return _cuda().gelu8_bwd(da, saved, ws, dbias, dx, act_out)
-    d, a, db = ref.gelu8_bwd(da, saved.q, saved.scale)
+        return _cuda().gelu8_bwd(da, da_, q_, scale, ws, at[1], dx_, at[0])
+    d, a, db = ref.gelu8_bwd(da, q, scale)
     dx.copy_(d); act_out.copy_(a); dbias.copy_(db)
