@@ -190,6 +190,10 @@ def start(local_device: int, ngpus_per_node: int, args) -> None:
         from .models.encoder import convert_bert_state_dict
         init_sd = convert_bert_state_dict(init_sd, roberta="roberta" in args.tf.lower())   # BERT / RoBERTa / MiniLM keys
     if init_sd is not None:
+        if args.rotary or args.relative_buckets:
+            from .models.encoder import grow_positions
+            own = trainer.model.embed[0].transformer.state_dict() if args.default_impl else trainer.encoder.encoder_state_dict()
+            init_sd = grow_positions(init_sd, own["embeddings.position_embeddings.weight"])
         if args.default_impl:
             trainer.model.embed[0].transformer.load_state_dict(init_sd, strict=not (args.rotary or args.relative_buckets))
         else:

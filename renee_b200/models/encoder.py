@@ -219,6 +219,16 @@ class DistilEncoder(nn.Module):
         return {"last_hidden_state": x}
 
 
+def grow_positions(sd: dict, own: torch.Tensor) -> dict:
+    """``sd`` with a position table of as many rows as ``own`` has: its rows, then those of ``own`` (an encoder with relative positions
+    may read longer texts than the checkpoint it starts from)."""
+    name = "embeddings.position_embeddings.weight"
+    if name not in sd or sd[name].shape[0] >= own.shape[0]:
+        return sd
+    table = sd[name]
+    return {**sd, name: torch.cat([table, own[table.shape[0]:].to(table.device, table.dtype)])}
+
+
 def convert_bert_state_dict(sd: dict, roberta: bool = False) -> dict:
     """Map a HF BERT / RoBERTa / MiniLM (BERT-architecture) encoder state dict onto this module's
     DistilBERT-style names.  The block math is identical (post-LayerNorm, erf GELU); the differences are

@@ -123,6 +123,19 @@ def test_weights_without_relative_positions_can_be_loaded():
         new.load_encoder_state_dict({})
 
 
+def test_weights_with_fewer_positions_can_be_loaded():
+    from renee_b200.models.encoder import grow_positions
+    n = "embeddings.position_embeddings.weight"
+    longer = dataclasses.replace(BASE, **VARIANTS["both"], max_position_embeddings=BASE.max_position_embeddings + 9)
+    old, new = FlatEncoder(BASE, "cpu", torch.float32, seed=1), FlatEncoder(longer, "cpu", torch.float32, seed=2)
+    own = new.view(new.p32, n).clone()
+    new.load_encoder_state_dict(grow_positions(old.encoder_state_dict(), own))
+    assert torch.equal(new.view(new.p32, n), torch.cat([old.view(old.p32, n), own[-9:]]))
+    model = DistilEncoder(longer)
+    model.load_state_dict(grow_positions(old.encoder_state_dict(), model.state_dict()[n]), strict=False)
+    assert torch.equal(model.state_dict()[n][:-9], old.view(old.p32, n))
+
+
 def test_command_line():
     parse = build_parser().parse_args
     assert _encoder_config(parse([])) == EncoderConfig()
