@@ -72,14 +72,6 @@ template <int CH> __device__ __forceinline__ void load_tile(char* dst, const CUt
   for (int c = 0; c < CH; ++c) tc::tma_load_3d(dst + c * rows * 128, map, bar, x + 64 * c, row, b);
 }
 
-// Zeros in the rows of a tile whose bit is not set (the whole warp); the swizzle stays within a row
-template <int CH> __device__ __forceinline__ void zero_rows(char* tile, const uint32_t* bits, int rows, int lane) {
-  for (int r = lane >> 3; r < rows; r += 4)
-    if (!(bits[r >> 5] >> (r & 31) & 1u))
-#pragma unroll
-      for (int c = 0; c < CH; ++c) *reinterpret_cast<uint4*>(tile + c * rows * 128 + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-}
-
 // D (128 x N) (+)= A (128 rows, K-major tile of ROWS rows) B^T (BLK rows, K-major), over HD columns
 template <typename T, int HD> __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
   constexpr uint32_t idesc = tc::make_idesc(std::is_same<T, __nv_bfloat16>::value ? 1 : 0, 0, 0, ROWS, BLK);
@@ -118,7 +110,7 @@ template <typename T> __device__ __forceinline__ void store_row(T* out, const fl
 // in turn); freed: nothing reads a tile's rows any more; end: its accumulators are complete; taken: they have been read (tiles in
 // turn).  A barrier that somebody may come late to is doubled: its next phase cannot then pass him by.
 constexpr int MAX_STAGES = 4, WORKERS = 8;
-struct Bars { uint64_t own[2], raw[MAX_STAGES], full[MAX_STAGES], empty[MAX_STAGES], scores[3], read, done[3], freed, end, taken[2]; };
+struct Bars { uint64_t own[2], raw[MAX_STAGES], full[MAX_STAGES], empty[MAX_STAGES], scores[3], read, done[3], freed[2], end, taken[2]; };
 
 __device__ __forceinline__ char* align1k(char* p) { return p + ((1024u - (tc::smem_u32(p) & 1023u)) & 1023u); }
 
@@ -139,7 +131,7 @@ template <int COLS> __device__ __forceinline__ void start(Bars* bars, uint32_t* 
       tc::mbar_init(bars->empty + i, 1);
     }
     tc::mbar_init(&bars->read, WORKERS);
-    tc::mbar_init(&bars->freed, free_by);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(bars->freed + i, free_by);
     tc::mbar_init(&bars->end, 1);
     tc::fence_barrier_init();
   }
@@ -214,16 +206,14 @@ __device__ __forceinline__ void mask_columns(float (&s)[32], uint32_t on) {
 // shared memory: tile_of[k & 1] is written before the own barrier of the CTA's k-th tile; -1 ends.
 struct Tiles {
   int* counter;
-  int now, next;
-  __device__ __forceinline__ Tiles(int* c, int lane) : counter(c), now(blockIdx.x) { next = ask(lane); }
-  __device__ __forceinline__ int ask(int lane) {
-    int t = 0;
-    if (lane == 0) t = (int)gridDim.x + max(atomicAdd(counter, 1), 0);
-    return __shfl_sync(0xffffffffu, t, 0);
+  int now, answer;                                             // the answer is lane 0's, and on its way while a tile is copied
+  __device__ __forceinline__ Tiles(int* c, int lane) : counter(c), now(blockIdx.x) { ask(lane); }
+  __device__ __forceinline__ void ask(int lane) {
+    if (lane == 0) answer = atomicAdd(counter, 1);
   }
   __device__ __forceinline__ void step(int lane) {
-    now = next;
-    next = ask(lane);
+    now = (int)gridDim.x + max(__shfl_sync(0xffffffffu, answer, 0), 0);
+    ask(lane);
   }
 };
 // A worker's next tile, or -1.  All workers leave together, also when a wait of one of them has run out.
@@ -259,7 +249,8 @@ template <typename T> __device__ __forceinline__ int key_blocks(const Args<T>& a
 
 // The copying warp of fwd and bwd_q.  own(at, k, bar): a tile's copies, the CTA's k-th; load(at, i, s, bar): block i into stage s;
 // masked: the half of the stage (K or V) whose masked rows become zeros, because 0 times a NaN is one
-template <int NST, int CH, int PIECE, typename T, typename Own, typename Load>
+// OWN: buffers for a tile's rows.
+template <int NST, int OWN, int CH, int PIECE, typename T, typename Own, typename Load>
 __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, char* stage, int masked, int lane,
                                                  int* counter, int* tile_of, Own own, Load load) {
   unsigned g = 0, k = 0, turns = 0;                            // turns: bit s = phase of raw[s]
@@ -296,7 +287,7 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
       if (i == 0) {                                            // the first block first: it may be on its way while the last tile's rows are read
         if (g > 0) mend(g - 1);                                // the last tile ends behind it
         on_last = make_uint2(0xffffffffu, 0xffffffffu);
-        if (k > 0) wait.all(&bars.freed, k - 1, tc::SITE_EMPTY);
+        if (k >= OWN) wait.all(bars.freed + k % OWN, k / OWN - 1, tc::SITE_EMPTY);
         if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
         if (wait.aborted) return;
         if (tc::elect_one()) {
@@ -314,11 +305,11 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
   no_more_tiles(bars, wait, tile_of, k);
 }
 
-// The MMA thread of fwd and bwd_q.  scores(g, s), rows(g, s, first): the products of block g, in stage s.
+// The MMA thread of fwd and bwd_q.  scores(g, s, k), rows(g, s, first): the products of block g, in stage s, of the CTA's k-th tile.
 // TURNS > 0: scores have that many buffers, which P shares: one is free when the product TURNS blocks back is complete, and scores are
 // issued TURNS - 1 blocks before the second product waits for its P.  TURNS = 0: scores have one buffer, free as soon as they are in
 // registers, and dS has two places of its own.
-template <int NST, int TURNS, typename T, typename Scores, typename Rows>
+template <int NST, int OWN, int TURNS, typename T, typename Scores, typename Rows>
 __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int per, const int* tile_of, Scores scores, Rows rows) {
   constexpr unsigned SLOTS = TURNS ? TURNS : 2, AHEAD = TURNS ? TURNS - 1 : 1;
   unsigned g = 0, k = 0, x = 0;                                // blocks begun, tiles begun, second products issued
@@ -354,9 +345,9 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
       wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
       if (wait.aborted) return;
       tc::tc_fence_after();
-      scores(g, g % NST);
+      scores(g, g % NST, k);
       tc::umma_commit(bars.scores + g % SLOTS);
-      if (TURNS && i + 1 == n) tc::umma_commit(&bars.freed);
+      if (i + 1 == n) tc::umma_commit(bars.freed + k % OWN);
       if (g >= x + AHEAD) second();
     }
   }
@@ -372,7 +363,7 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
 // its maximum, and the two warps meet once a block, to hear whether the other one left the range.
 template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
-  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4, COLS = 256, TURNS = HD == 128 ? 2 : 3, O_COL = TURNS * BLK;
+  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4, OWN = HD == 128 ? 1 : 2, COLS = 256, TURNS = HD == 128 ? 2 : 3, O_COL = TURNS * BLK;
   constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
@@ -380,7 +371,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   __shared__ int tile_of[2];
   __shared__ float s_row[2][2][ROWS];                        // [maxima, sums][half][row]
   char* sq = align1k(smem_raw);
-  char* stage = sq + TILE;                                   // [NST][K piece, V piece]
+  char* stage = sq + OWN * TILE;                             // [NST][K piece, V piece]
   const int wd = window(a), per = (a.S + ROWS - 1) / ROWS, tiles = per * a.nh * a.b, wfloats = window_floats(wd) + mask_words(a.S);
   float* windows = reinterpret_cast<float*>(stage + NST * 2 * PIECE);           // [2][window, mask]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
@@ -389,11 +380,11 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   Waiter wait{false, a.status};
   grid_dep_wait();
   if (warp == WORKERS) {
-    copy_query_tiles<NST, CH, PIECE>(
+    copy_query_tiles<NST, OWN, CH, PIECE>(
         a, bars, wait, tiles, per, stage, 1, lane, a.counters + 0, tile_of,
         [&](const Place& at, unsigned k, uint64_t* bar) {
           tc::mbar_expect_tx(bar, TILE + window_bytes(a, wd));
-          load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
+          load_tile<CH>(sq + (k % OWN) * TILE, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
           load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, bar);
         },
         [&](const Place& at, int i, int s, uint64_t* bar) {
@@ -403,9 +394,9 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
         });
   } else if (warp > WORKERS) {
     if (tc::elect_one())
-      multiply_query_tiles<NST, TURNS>(
+      multiply_query_tiles<NST, OWN, TURNS>(
           a, bars, wait, per, tile_of,
-          [&](unsigned g, int s) { mma_scores<T, HD>(tmem + (g % TURNS) * BLK, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE)); },
+          [&](unsigned g, int s, unsigned k) { mma_scores<T, HD>(tmem + (g % TURNS) * BLK, tc::smem_u32(sq + (k % OWN) * TILE), tc::smem_u32(stage + s * 2 * PIECE)); },
           [&](unsigned g, int s, bool first) {
             mma_rows<T, HDP>(tmem + O_COL, tmem + (g % TURNS) * BLK, 32, tc::smem_u32(stage + s * 2 * PIECE + PIECE), first);
           });
@@ -556,22 +547,23 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   char* sdo = sq + TILE;
   char* sctx = sdo + TILE;
   char* stage = sctx + TILE;                                 // [NST][K piece, V piece]
-  const int wd = window(a), per = (a.S + ROWS - 1) / ROWS, tiles = per * a.nh * a.b, wfloats = window_floats(wd) + mask_words(a.S);
-  float* windows = reinterpret_cast<float*>(stage + NST * 2 * PIECE);           // [2][window, mask]
+  const int wd = window(a), per = (a.S + ROWS - 1) / ROWS, tiles = per * a.nh * a.b, wfloats = window_floats(wd) + mask_words(a.S) + ROWS;
+  float* windows = reinterpret_cast<float*>(stage + NST * 2 * PIECE);           // [2][window, mask, lse]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
-  start<COLS>(&bars, &s_tmem, warp, WORKERS);
+  start<COLS>(&bars, &s_tmem, warp, WORKERS + 1);
   const uint32_t tmem = s_tmem, ds_cols = tmem + 128 + HDP;
   Waiter wait{false, a.status};
   grid_dep_wait();
   if (warp == WORKERS) {
-    copy_query_tiles<NST, CH, PIECE>(
+    copy_query_tiles<NST, 1, CH, PIECE>(
         a, bars, wait, tiles, per, stage, 0, lane, a.counters + 1, tile_of,
         [&](const Place& at, unsigned k, uint64_t* bar) {
-          tc::mbar_expect_tx(bar, 3 * TILE + window_bytes(a, wd));
+          tc::mbar_expect_tx(bar, 3 * TILE + window_bytes(a, wd) + ROWS * 4);
           load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sdo, &maps.d, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sctx, &maps.e, bar, at.h * HD, at.row0, at.b, ROWS);
           load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, bar);
+          tc::bulk_load(windows + (k & 1) * wfloats + wfloats - ROWS, a.lse + (size_t)at.bh * a.Sp + at.row0, ROWS * 4, bar);
         },
         [&](const Place& at, int i, int s, uint64_t* bar) {
           tc::mbar_expect_tx(bar, 2 * PIECE);
@@ -580,9 +572,9 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
         });
   } else if (warp > WORKERS) {
     if (tc::elect_one())
-      multiply_query_tiles<NST, 0>(
+      multiply_query_tiles<NST, 1, 0>(
           a, bars, wait, per, tile_of,
-          [&](unsigned, int s) {
+          [&](unsigned, int s, unsigned) {
             mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE));
             mma_scores<T, HD>(tmem + 64, tc::smem_u32(sdo), tc::smem_u32(stage + s * 2 * PIECE + PIECE));
           },
@@ -598,8 +590,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       const int seen = __ldg(a.lens + at.b), n = (attended_len(seen, a.S) + BLK - 1) / BLK;
       const bool flat = seen <= 0;
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
-      const float lse = q < a.S ? (seen < 0 ? 0.f : __ldg(a.lse + (size_t)at.bh * a.Sp + q)) - a.grad_log2 : INFINITY;
       const float* win = windows + (k & 1) * wfloats;
+      const float lse = q < a.S ? (seen < 0 ? 0.f : win[wfloats - ROWS + row]) - a.grad_log2 : INFINITY;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
       const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S + half * 32;
       float d = 0.f;                                         // delta = dctx ctx: half a row each
@@ -614,6 +606,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       }
       s_sum[0][half][row] = d;
       asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (lane == 0) tc::mbar_arrive(bars.freed);            // the products' arrival is the other one
       const V2 nd = v2(-(s_sum[0][0][row] + s_sum[0][1][row]));
       V2 sum = v2(0.f);
       for (int i = 0; i < n; ++i, ++g) {
@@ -627,7 +620,6 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
           float s[32], dp[32];
           tmem_ld2x32(row_s, row_s + 64, s, dp);
           warp_arrive(&bars.read, lane);
-          if (i + 1 == n && lane == 0) tc::mbar_arrive(&bars.freed);
           exponents<W>(s, a.scale_log2, flat, far_bias, win + (k0 - q) + wd + PAD, -lse);
           if constexpr (W::MASK) mask_columns(s, on);
           uint32_t r[16];
@@ -691,7 +683,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 }
 
 // ------------------------------------------------------------------------------------------------ backward: keys
-// The same division of work; rows are keys, whose masked ones become zeros in K and V and get no probability.  TMEM: S^T 64 columns,
+// The same division of work; rows are keys, whose masked ones get scores and probabilities of zero.  TMEM: S^T 64 columns,
 // dP^T 64, dV, dK; P~^T and dS^T go over S^T and dP^T (columns 0-15 and 32-47, each warp over its own), so that two CTAs share an SM,
 // and the next block's scores wait for their products.
 // The sums by distance: a diagonal of a warp's 32 x 32 piece of dS (row = lane, column = step) moves on by one lane each step, so a
@@ -716,7 +708,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   float* windows = reinterpret_cast<float*>(stage + NST * STAGE_UP);            // [2][window, mask]
   float* sums = windows + 2 * wfloats;                       // [8][nwin]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
-  start<COLS>(&bars, &s_tmem, warp, WORKERS);
+  start<COLS>(&bars, &s_tmem, warp, 1);
   const uint32_t tmem = s_tmem;
   Waiter wait{false, a.status};
   grid_dep_wait();
@@ -732,12 +724,10 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     return at.row0 < attended_len(__ldg(a.lens + at.b), a.S) ? nq : 0;
   };
   if (warp == WORKERS) {
-    unsigned g = 0, k = 0, turn = 0;
+    unsigned g = 0, k = 0;
     for (Tiles t(a.counters + 2, lane); t.now < tiles; t.step(lane)) {
       if (blocks(t.now) == 0) continue;
       const Place at = place(t.now);
-      const uint4 on = __ldg(reinterpret_cast<const uint4*>(a.bits + (size_t)at.b * mask_words(a.S)) + at.row0 / ROWS);
-      const bool whole = (on.x & on.y & on.z & on.w) == 0xffffffffu;
       for (int i = 0; i < nq; ++i, ++g) {
         const int s = g % NST;
         if (g >= NST) wait.all(bars.empty + s, g / NST - 1, tc::SITE_EMPTY);
@@ -752,11 +742,11 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         }
         __syncwarp();
         if (i > 0) continue;
-        if (k > 0) wait.all(&bars.freed, k - 1, tc::SITE_EMPTY);
+        if (k > 0) wait.all(bars.freed, k - 1, tc::SITE_EMPTY);
         if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
         if (wait.aborted) break;
-        uint64_t* bar = whole ? bars.own + (k & 1) : bars.raw;
         if (tc::elect_one()) {
+          uint64_t* bar = bars.own + (k & 1);
           tile_of[k & 1] = t.now;
           tc::mbar_expect_tx(bar, 2 * TILE + window_bytes(a, wd));
           load_tile<CH>(sk, &maps.b, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -764,15 +754,6 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, bar);
         }
         __syncwarp();
-        if (!whole) {
-          wait.all(bars.raw, turn++, tc::SITE_FULL);
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(windows + (k & 1) * wfloats + window_floats(wd)) + (at.row0 >> 5);
-          zero_rows<CH>(sk, w, ROWS, lane);
-          zero_rows<CH>(sv, w, ROWS, lane);
-          tc::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(bars.own + (k & 1));
-        }
       }
       if (wait.aborted) break;
       ++k;
@@ -807,6 +788,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           mma_scores<T, HD>(tmem, tc::smem_u32(sk), tc::smem_u32(st));
           mma_scores<T, HD>(tmem + 64, tc::smem_u32(sv), tc::smem_u32(st + PIECE));
           tc::umma_commit(bars.scores + (g & 1));
+          if (i + 1 == nq) tc::umma_commit(bars.freed);
         }
       }
     }
@@ -843,6 +825,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       const bool flat = __ldg(a.lens + at.b) <= 0;
       const float* win = windows + (k & 1) * wfloats;
       const bool on = reinterpret_cast<const uint32_t*>(win + window_floats(wd))[key >> 5] >> (key & 31) & 1u;
+      const bool all_on = __all_sync(0xffffffffu, on);
       float far[2] = {};
       for (int i = 0; i < n; ++i, ++g) {
         const int q0 = i * BLK + half * 32;                  // of this warp's columns
@@ -856,7 +839,11 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           using W = decltype(way);
           float s[32], dp[32];
           tmem_ld2x32(row_s, row_s + 64, s, dp);
-          if (i + 1 == n) warp_arrive(&bars.freed, lane);
+          if (!all_on) {                                     // a masked key's K and V may hold anything
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (!on) s[j] = dp[j] = 0.f;
+          }
           const V2 scale = v2(a.scale_log2), fb = v2(far_bias);
           uint32_t r[16];
 #pragma unroll
@@ -969,7 +956,7 @@ template <typename K> int allow_smem(K kernel, int bytes) {
 }
 
 template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaStream_t st) {
-  constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = HD == 128 ? 2 : 4;
+  constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = HD == 128 ? 2 : 4, OWN = HD == 128 ? 1 : 2;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps m;
   const uint64_t H = (uint64_t)a.nh * HD;
@@ -978,7 +965,7 @@ template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaSt
   if (!rc) rc = tc::make_tmap_rows(&m.c, a.v, a.b, a.S, H, a.ldv, BLK, bf);
   if (rc) return rc;
   m.d = m.e = m.c;
-  const int smem = 1024 + (ROWS + NST * 2 * BLK) * 128 * CH + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
+  const int smem = 1024 + (OWN * ROWS + NST * 2 * BLK) * 128 * CH + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
   rc = allow_smem(fwd_tc<T, HD, DROP>, smem);
   if (rc) return rc;
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * 2;
@@ -1002,7 +989,7 @@ template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaSt
   if (rc) return rc;
   kv.e = kv.d;
   const int wd = window(a), windows = 2 * (window_floats(wd) + mask_words(a.S)) * 4;
-  const int smem_q = 1024 + 3 * ROWS * 128 * CH + NST * 2 * PIECE + windows;
+  const int smem_q = 1024 + 3 * ROWS * 128 * CH + NST * 2 * PIECE + windows + 2 * ROWS * 4;
   const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST * STAGE_UP + windows + 8 * (2 * wd + 1) * 4;
   rc = allow_smem(bwd_q_tc<T, HD, DROP>, smem_q);
   if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP>, smem_kv);
