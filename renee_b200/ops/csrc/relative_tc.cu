@@ -422,13 +422,10 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
         const float* wp = win + (k0 - q) + wd + PAD;
         const uint32_t on = bits[k0 >> 5];
         const uint32_t row_s = tmem + lanes + (g % TURNS) * BLK + 32 * half;
-        const auto top = [&](const float (&s)[32]) {         // of the scores, or m
+        const auto top = [&](const float (&s)[32]) {         // of the exponents, or m
           float x = m;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float v = empty ? 0.f : fmaf(s[j], a.scale_log2, far_piece ? far_bias : wp[j]);
-            if (on >> j & 1u) x = fmaxf(x, v);
-          }
+          for (int j = 0; j < 32; ++j) x = fmaxf(x, s[j]);
           s_row[0][half][row] = x;
           asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
           return fmaxf(s_row[0][0][row], s_row[0][1][row]);
@@ -438,6 +435,12 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
           float s[32];
           tc::tmem_ld32(row_s, s);
           if constexpr (W::MASK) {
+            if (empty) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) s[j] = 0.f;
+            }
+            exponents<W>(s, a.scale_log2, false, far_bias, wp, 0.f);
+            mask_columns(s, on);
             if (again) {                                     // a new reference; O is at rest behind the last block's product, half of it each
               const float x = top(s), f = m == -INFINITY ? 0.f : ex2(m - x);
               l *= f;
@@ -467,8 +470,13 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
               asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
             }
           }
-          exponents<W>(s, a.scale_log2, empty, far_bias, wp, m == -INFINITY ? 0.f : up - m);
-          if constexpr (W::MASK) mask_columns(s, on);
+          if constexpr (W::MASK) {
+            const V2 c = v2(m == -INFINITY ? 0.f : up - m);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) v2_get(v2(s[j], s[j + 1]) + c, s[j], s[j + 1]);
+          } else {
+            exponents<W>(s, a.scale_log2, false, far_bias, wp, up - m);
+          }
           V2 l2[2] = {v2(0.f), v2(0.f)};
           uint32_t r[16];
 #pragma unroll
