@@ -202,8 +202,25 @@ __device__ __forceinline__ void mask_columns(float (&s)[32], uint32_t on) {
   }
 }
 
-// The tiles of a CTA: its own number first, then what the counter says.  The copying warp asks (one tile ahead) and hands on through
-// shared memory: tile_of[k & 1] is written before the own barrier of the CTA's k-th tile; -1 ends.
+// Where a tile lies.  seen: the sequence's entry of lens.  The copying warp finds it out one tile ahead and hands it to the others through
+// shared memory (divisions and a load from L2 were 1300 clocks of each tile): place[k & 1] is written before the own barrier of the
+// CTA's k-th tile; a negative b ends.
+struct alignas(16) Place {
+  int b, h, row0, seen;
+  template <typename T> __device__ __forceinline__ int bh(const Args<T>& a) const { return b * a.nh + h; }
+  template <typename T> __device__ __forceinline__ int blocks(const Args<T>& a) const { return (attended_len(seen, a.S) + BLK - 1) / BLK; }
+};
+__device__ __forceinline__ Place read_place(const Place* p) {
+  const int4 v = *reinterpret_cast<const int4*>(p);
+  return Place{v.x, v.y, v.z, v.w};
+}
+// Tile t of `per` tiles a (sequence, head)
+template <typename T> __device__ __forceinline__ Place query_tile(const Args<T>& a, int t, int per) {
+  const int bh = t / per, b = bh / a.nh;
+  return Place{b, bh - b * a.nh, (t - bh * per) * ROWS, __ldg(a.lens + b)};
+}
+
+// The tiles of a CTA: its own number first, then what the counter says.  The copying warp asks, one tile ahead.
 struct Tiles {
   int* counter;
   int now, answer;                                             // the answer is lane 0's, and on its way while a tile is copied
@@ -216,35 +233,23 @@ struct Tiles {
     ask(lane);
   }
 };
-// A worker's next tile, or -1.  All workers leave together, also when a wait of one of them has run out.
-__device__ __forceinline__ int worker_tile(Bars& bars, Waiter& wait, const int* tile_of, unsigned k) {
+// A worker's next tile; b < 0: none.  All workers leave together, also when a wait of one of them has run out.
+__device__ __forceinline__ Place worker_tile(Bars& bars, Waiter& wait, const Place* place, unsigned k) {
   wait.all(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
   uint32_t gone = wait.aborted;
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n barrier.cta.red.or.pred q, 5, 256, p;\n selp.u32 %0, 1, 0, q;\n}" : "+r"(gone) :: "memory");
-  return gone ? -1 : *(const volatile int*)(tile_of + (k & 1));
+  Place at = read_place(place + (k & 1));
+  if (gone) at.b = -1;
+  return at;
 }
 // The copying warp's last word
-__device__ __forceinline__ void no_more_tiles(Bars& bars, Waiter& wait, int* tile_of, unsigned k) {
+__device__ __forceinline__ void no_more_tiles(Bars& bars, Waiter& wait, Place* place, unsigned k) {
   if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
   if (!wait.aborted && tc::elect_one()) {
-    tile_of[k & 1] = -1;
+    place[k & 1].b = -1;
     tc::mbar_arrive(bars.own + (k & 1));
   }
   __syncwarp();
-}
-
-// Where a tile of queries lies: tile t of `per` tiles a (sequence, head)
-struct Place {
-  int bh, b, h, row0;
-  template <typename T> __device__ __forceinline__ Place(const Args<T>& a, int t, int per) {
-    bh = t / per;
-    b = bh / a.nh;
-    h = bh - b * a.nh;
-    row0 = (t - bh * per) * ROWS;
-  }
-};
-template <typename T> __device__ __forceinline__ int key_blocks(const Args<T>& a, int b) {
-  return (attended_len(__ldg(a.lens + b), a.S) + BLK - 1) / BLK;
 }
 
 // The copying warp of fwd and bwd_q.  own(at, k, bar): a tile's copies, the CTA's k-th; load(at, i, s, bar): block i into stage s;
@@ -252,7 +257,7 @@ template <typename T> __device__ __forceinline__ int key_blocks(const Args<T>& a
 // OWN: buffers for a tile's rows.
 template <int NST, int OWN, int CH, int PIECE, typename T, typename Own, typename Load>
 __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int tiles, int per, char* stage, int masked, int lane,
-                                                 int* counter, int* tile_of, Own own, Load load) {
+                                                 int* counter, Place* place, Own own, Load load) {
   unsigned g = 0, k = 0, turns = 0;                            // turns: bit s = phase of raw[s]
   uint2 on_last = make_uint2(0xffffffffu, 0xffffffffu);        // attended keys of the block before, if it has to be mended
   const auto mend = [&](unsigned x) {                          // block x
@@ -270,8 +275,8 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
     if (lane == 0) tc::mbar_arrive(bars.full + s);
   };
   for (Tiles t(counter, lane); t.now < tiles; t.step(lane), ++k) {
-    const Place at(a, t.now, per);
-    const int n = key_blocks(a, at.b);
+    const Place at = query_tile(a, t.now, per);
+    const int n = at.blocks(a);
     const uint2* bits = reinterpret_cast<const uint2*>(a.bits + (size_t)at.b * mask_words(a.S));
     for (int i = 0; i < n; ++i, ++g) {
       const uint2 on = __ldg(bits + i);
@@ -291,7 +296,7 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
         if (k > 1) wait.all(bars.taken + (k & 1), (k >> 1) - 1, tc::SITE_EMPTY);
         if (wait.aborted) return;
         if (tc::elect_one()) {
-          tile_of[k & 1] = t.now;
+          place[k & 1] = at;
           own(at, k, bars.own + (k & 1));
         }
         __syncwarp();
@@ -302,7 +307,7 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
     }
   }
   if (g > 0) mend(g - 1);
-  no_more_tiles(bars, wait, tile_of, k);
+  no_more_tiles(bars, wait, place, k);
 }
 
 // The MMA thread of fwd and bwd_q.  scores(g, s, k), rows(g, s, first): the products of block g, in stage s, of the CTA's k-th tile.
@@ -310,7 +315,7 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
 // issued TURNS - 1 blocks before the second product waits for its P.  TURNS = 0: scores have one buffer, free as soon as they are in
 // registers, and dS has two places of its own.
 template <int NST, int OWN, int TURNS, typename T, typename Scores, typename Rows>
-__device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, int per, const int* tile_of, Scores scores, Rows rows) {
+__device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, const Place* place, Scores scores, Rows rows) {
   constexpr unsigned SLOTS = TURNS ? TURNS : 2, AHEAD = TURNS ? TURNS - 1 : 1;
   unsigned g = 0, k = 0, x = 0;                                // blocks begun, tiles begun, second products issued
   unsigned jx = 0, ix = 0, nx = 0, n_last = 0;                 // block x: the ix-th of nx of the CTA's jx-th tile
@@ -332,9 +337,9 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
     nx = n_last;
     while (x < g && !wait.aborted) second();                   // the last tile's end before this one's rows are waited for
     wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
-    const int t = *(const volatile int*)(tile_of + (k & 1));
-    if (wait.aborted || t < 0) return;
-    const unsigned n = key_blocks(a, t / per / a.nh);
+    const Place at = read_place(place + (k & 1));
+    if (wait.aborted || at.b < 0) return;
+    const unsigned n = at.blocks(a);
     nx = n_last = n;
     for (unsigned i = 0; i < n && !wait.aborted; ++i, ++g) {
       if (TURNS) {
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int tile_of[2];
+  __shared__ Place place[2];
   __shared__ float s_row[2][2][ROWS];                        // [maxima, sums][half][row]
   char* sq = align1k(smem_raw);
   char* stage = sq + OWN * TILE;                             // [NST][K piece, V piece]
@@ -381,7 +386,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   grid_dep_wait();
   if (warp == WORKERS) {
     copy_query_tiles<NST, OWN, CH, PIECE>(
-        a, bars, wait, tiles, per, stage, 1, lane, a.counters + 0, tile_of,
+        a, bars, wait, tiles, per, stage, 1, lane, a.counters + 0, place,
         [&](const Place& at, unsigned k, uint64_t* bar) {
           tc::mbar_expect_tx(bar, TILE + window_bytes(a, wd));
           load_tile<CH>(sq + (k % OWN) * TILE, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -395,7 +400,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   } else if (warp > WORKERS) {
     if (tc::elect_one())
       multiply_query_tiles<NST, OWN, TURNS>(
-          a, bars, wait, per, tile_of,
+          a, bars, wait, place,
           [&](unsigned g, int s, unsigned k) { mma_scores<T, HD>(tmem + (g % TURNS) * BLK, tc::smem_u32(sq + (k % OWN) * TILE), tc::smem_u32(stage + s * 2 * PIECE)); },
           [&](unsigned g, int s, bool first) {
             mma_rows<T, HDP>(tmem + O_COL, tmem + (g % TURNS) * BLK, 32, tc::smem_u32(stage + s * 2 * PIECE + PIECE), first);
@@ -406,14 +411,13 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
     const float up = FP16 ? 6.f : 0.f, limit = FP16 ? 32768.f : 1.1529215e18f;
     const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
-    for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
-      const Place at(a, t, per);
-      const int seen = __ldg(a.lens + at.b), n = (attended_len(seen, a.S) + BLK - 1) / BLK;
+    for (Place at; (at = worker_tile(bars, wait, place, k)).b >= 0; ++k) {
+      const int seen = at.seen, n = at.blocks(a), bh = at.bh(a);
       const bool empty = seen == 0;
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
       const float* win = windows + (k & 1) * wfloats;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
-      const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S;
+      const uint32_t drop0 = ((uint32_t)bh * a.S + q) * (uint32_t)a.S;
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + 32 * half, dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;     // of this warp's columns
@@ -532,7 +536,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
         if (c == CH - 1) warp_arrive(bars.taken + (k & 1), lane);
         if (q < a.S && half * 32 + 64 * c < HD) store_row<T>(out + half * 32 + 64 * c, v, f);
       }
-      if (half == 0) a.lse[(size_t)at.bh * a.Sp + q] = q < a.S ? m + (lg2(l) - up) : INFINITY;
+      if (half == 0) a.lse[(size_t)bh * a.Sp + q] = q < a.S ? m + (lg2(l) - up) : INFINITY;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
     }
   }
@@ -549,7 +553,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int tile_of[2];
+  __shared__ Place place[2];
   __shared__ float s_sum[2][2][ROWS];
   char* sq = align1k(smem_raw);
   char* sdo = sq + TILE;
@@ -564,14 +568,14 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   grid_dep_wait();
   if (warp == WORKERS) {
     copy_query_tiles<NST, 1, CH, PIECE>(
-        a, bars, wait, tiles, per, stage, 0, lane, a.counters + 1, tile_of,
+        a, bars, wait, tiles, per, stage, 0, lane, a.counters + 1, place,
         [&](const Place& at, unsigned k, uint64_t* bar) {
           tc::mbar_expect_tx(bar, 3 * TILE + window_bytes(a, wd) + ROWS * 4);
           load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sdo, &maps.d, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sctx, &maps.e, bar, at.h * HD, at.row0, at.b, ROWS);
           load_window(a, at.b, at.h, wd, windows + (k & 1) * wfloats, bar);
-          tc::bulk_load(windows + (k & 1) * wfloats + wfloats - ROWS, a.lse + (size_t)at.bh * a.Sp + at.row0, ROWS * 4, bar);
+          tc::bulk_load(windows + (k & 1) * wfloats + wfloats - ROWS, a.lse + (size_t)at.bh(a) * a.Sp + at.row0, ROWS * 4, bar);
         },
         [&](const Place& at, int i, int s, uint64_t* bar) {
           tc::mbar_expect_tx(bar, 2 * PIECE);
@@ -581,7 +585,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
   } else if (warp > WORKERS) {
     if (tc::elect_one())
       multiply_query_tiles<NST, 1, 0>(
-          a, bars, wait, per, tile_of,
+          a, bars, wait, place,
           [&](unsigned, int s, unsigned) {
             mma_scores<T, HD>(tmem, tc::smem_u32(sq), tc::smem_u32(stage + s * 2 * PIECE));
             mma_scores<T, HD>(tmem + 64, tc::smem_u32(sdo), tc::smem_u32(stage + s * 2 * PIECE + PIECE));
@@ -593,15 +597,14 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
     const float kept = 1.f / (1.f - a.p);
     const uint32_t seed = DROP ? (uint32_t)__ldg(a.seed) : 0u;
     unsigned g = 0, k = 0;
-    for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
-      const Place at(a, t, per);
-      const int seen = __ldg(a.lens + at.b), n = (attended_len(seen, a.S) + BLK - 1) / BLK;
+    for (Place at; (at = worker_tile(bars, wait, place, k)).b >= 0; ++k) {
+      const int seen = at.seen, n = at.blocks(a), bh = at.bh(a);
       const bool flat = seen <= 0;
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
       const float* win = windows + (k & 1) * wfloats;
       const float lse = q < a.S ? (seen < 0 ? 0.f : win[wfloats - ROWS + row]) - a.grad_log2 : INFINITY;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
-      const uint32_t drop0 = ((uint32_t)at.bh * a.S + q) * (uint32_t)a.S + half * 32;
+      const uint32_t drop0 = ((uint32_t)bh * a.S + q) * (uint32_t)a.S + half * 32;
       float d = 0.f;                                         // delta = dctx ctx: half a row each
 #pragma unroll
       for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
@@ -666,8 +669,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       s_sum[1][half][row] = x + y;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (half == 0) {                                       // negative, as the keys' pass adds them; behind S nothing is left of P
-        a.delta[(size_t)at.bh * a.Sp + q] = q < a.S ? -(s_sum[1][0][row] + s_sum[1][1][row]) * a.grad_inv : 0.f;
-        a.lse_up[(size_t)at.bh * a.Sp + q] = -lse;
+        a.delta[(size_t)bh * a.Sp + q] = q < a.S ? -(s_sum[1][0][row] + s_sum[1][1][row]) * a.grad_inv : 0.f;
+        a.lse_up[(size_t)bh * a.Sp + q] = -lse;
       }
       wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
@@ -695,8 +698,9 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 // dP^T 64, dV, dK; P~^T and dS^T go over S^T and dP^T (columns 0-15 and 32-47, each warp over its own), so that two CTAs share an SM,
 // and the next block's scores wait for their products.
 // The sums by distance: a diagonal of a warp's 32 x 32 piece of dS (row = lane, column = step) moves on by one lane each step, so a
-// running sum handed to the next lane collects it: one shuffle and one add per column.  Lane 31 drops a finished diagonal each
-// step, the last 32 are in the lanes at the end; the warp then adds all 63 to its window of sums.  This runs under the products.
+// running sum handed to the next lane collects it: one shuffle and one add per column.  Four such sums run side by side, over 8
+// columns each (one over all 32 took 2500 clocks a block, mostly its shuffles' latency).  Lane 31 drops a finished diagonal each step, the
+// last 32 are in the lanes at the end; the warp then adds the four up and all 63 diagonals to its window of sums.
 template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH;
@@ -705,8 +709,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int tile_of[2];
-  __shared__ float s_diag[8][64];
+  __shared__ Place place[2];
+  __shared__ float s_diag[8][4][40];
   __shared__ float s_none[32];                               // the window of a masked key
   char* sk = align1k(smem_raw);
   char* sv = sk + TILE;
@@ -722,20 +726,18 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   grid_dep_wait();
   if (blockIdx.x == 0 && threadIdx.x == 0) a.counters[1] = 0;          // the queries' pass is over; another one may follow
   // tiles in order of their place in the sequence: the last ones, of which few have an attended key, fill the gaps
-  const auto place = [&](int t) {
+  const auto key_tile = [&](int t) {
     const int bhs = a.nh * a.b, part = t / bhs;
-    return Place(a, (t - part * bhs) * per + part, per);
+    return query_tile(a, (t - part * bhs) * per + part, per);
   };
   // a tile without an attended key has no gradient and no blocks
-  const auto blocks = [&](int t) {
-    const Place at = place(t);
-    return at.row0 < attended_len(__ldg(a.lens + at.b), a.S) ? nq : 0;
-  };
+  const auto none = [&](const Place& at) { return at.row0 >= attended_len(at.seen, a.S); };
   if (warp == WORKERS) {
     unsigned g = 0, k = 0;
     for (Tiles t(a.counters + 2, lane); t.now < tiles; t.step(lane)) {
-      if (blocks(t.now) == 0) continue;
-      const Place at = place(t.now);
+      const Place at = key_tile(t.now);
+      if (none(at)) continue;
+      const int bh = at.bh(a);
       for (int i = 0; i < nq; ++i, ++g) {
         const int s = g % NST;
         if (g >= NST) wait.all(bars.empty + s, g / NST - 1, tc::SITE_EMPTY);
@@ -745,8 +747,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           tc::mbar_expect_tx(bars.full + s, STAGE);
           load_tile<CH>(st, &maps.a, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
           load_tile<CH>(st + PIECE, &maps.d, bars.full + s, at.h * HD, i * BLK, at.b, BLK);
-          tc::bulk_load(st + 2 * PIECE, a.lse_up + (size_t)at.bh * a.Sp + i * BLK, BLK * 4, bars.full + s);
-          tc::bulk_load(st + 2 * PIECE + BLK * 4, a.delta + (size_t)at.bh * a.Sp + i * BLK, BLK * 4, bars.full + s);
+          tc::bulk_load(st + 2 * PIECE, a.lse_up + (size_t)bh * a.Sp + i * BLK, BLK * 4, bars.full + s);
+          tc::bulk_load(st + 2 * PIECE + BLK * 4, a.delta + (size_t)bh * a.Sp + i * BLK, BLK * 4, bars.full + s);
         }
         __syncwarp();
         if (i > 0) continue;
@@ -755,7 +757,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         if (wait.aborted) break;
         if (tc::elect_one()) {
           uint64_t* bar = bars.own + (k & 1);
-          tile_of[k & 1] = t.now;
+          place[k & 1] = at;
           tc::mbar_expect_tx(bar, 2 * TILE + window_bytes(a, wd));
           load_tile<CH>(sk, &maps.b, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sv, &maps.c, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -766,7 +768,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       if (wait.aborted) break;
       ++k;
     }
-    no_more_tiles(bars, wait, tile_of, k);
+    no_more_tiles(bars, wait, place, k);
   } else if (warp > WORKERS) {
     if (tc::elect_one()) {
       unsigned g = 0, k = 0;
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       for (;; ++k) {
         if (g > 0) second(g - 1, nq == 1, true, k - 1);
         wait.one(bars.own + (k & 1), k >> 1, tc::SITE_FULL);
-        if (wait.aborted || *(const volatile int*)(tile_of + (k & 1)) < 0) break;
+        if (wait.aborted || read_place(place + (k & 1)).b < 0) break;
         for (int i = 0; i < nq && !wait.aborted; ++i, ++g) {
           if (i > 0) second(g - 1, i == 1, false, k);
           wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
@@ -812,8 +814,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     unsigned g = 0, k = 0;
     // tiles without an attended key: zeros, each CTA its share
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-      if (blocks(t) > 0) continue;
-      const Place at = place(t);
+      const Place at = key_tile(t);
+      if (!none(at)) continue;
       const int key = at.row0 + row;
       float v[32] = {};
       if (key < a.S)
@@ -824,13 +826,13 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         }
       for (int i = threadIdx.x; i < nwin; i += 256) a.dwin[((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin + i] = 0.f;
     }
-    for (int t; (t = worker_tile(bars, wait, tile_of, k)) >= 0; ++k) {
-      const Place at = place(t);
+    for (Place at; (at = worker_tile(bars, wait, place, k)).b >= 0; ++k) {
+      const int bh = at.bh(a);
       const int k_warp = at.row0 + quarter * 32, key = k_warp + lane, n = nq;
       T* const out_v = a.dv + ((size_t)at.b * a.S + key) * a.lddv + at.h * HD;
       T* const out_k = a.dk + ((size_t)at.b * a.S + key) * a.lddk + at.h * HD;
       float* const out_w = a.dwin + ((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin;
-      const bool flat = __ldg(a.lens + at.b) <= 0;
+      const bool flat = at.seen <= 0;
       const float* win = windows + (k & 1) * wfloats;
       const bool on = reinterpret_cast<const uint32_t*>(win + window_floats(wd))[key >> 5] >> (key & 31) & 1u;
       const bool all_on = __all_sync(0xffffffffu, on);
@@ -868,7 +870,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
               const V2 pr = v2(ex2(x), ex2(y));
               V2 v = v2(dp[c], dp[c + 1]);
               if (DROP) {
-                const uint32_t at0 = ((uint32_t)at.bh * a.S + q0 + c) * (uint32_t)a.S + key;
+                const uint32_t at0 = ((uint32_t)bh * a.S + q0 + c) * (uint32_t)a.S + key;
                 const V2 kf = v2(keep(seed, a.stream, at0, a.p) ? kept : 0.f, keep(seed, a.stream, at0 + (uint32_t)a.S, a.p) ? kept : 0.f);
                 v = v * kf;
                 v2_get(pr * kf, x, y);
@@ -894,20 +896,32 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
             v2_get(v, x, y);
             far[dhi <= -wd ? 0 : 1] += x + y;
           } else if constexpr (!W::FAR) {
-            float* diag = s_diag[warp];                      // diagonal e: row - column = e - 31
-            float acc = dp[0];
+            float(*diag)[40] = s_diag[warp];                 // [c][i]: row - column = i - 8 c - 7
+            float acc[4];
 #pragma unroll
-            for (int j = 1; j < 32; ++j) {
-              if (lane == 31) diag[63 - j] = acc;            // row 31, column j - 1
-              acc = fmaf(__shfl_up_sync(0xffffffffu, acc, 1), not_first, dp[j]);
-            }
-            diag[lane] = acc;                                // column 31: row - column = lane - 31
+            for (int c = 0; c < 4; ++c) acc[c] = dp[8 * c];
+#pragma unroll
+            for (int j = 1; j < 8; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if (lane == 31) diag[c][39 - j] = acc[c];    // row 31, column 8 c + j - 1
+                acc[c] = fmaf(__shfl_up_sync(0xffffffffu, acc[c], 1), not_first, dp[8 * c + j]);
+              }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) diag[c][lane] = acc[c];
             __syncwarp();
 #pragma unroll
-            for (int e = lane; e < 63; e += 32) {
-              const float v = diag[e];
-              const int d = k_warp - q0 + e - 31;
-              if (d <= -wd) far[0] += v;
+            for (int x = 0; x < 2; ++x) {
+              const int e = lane - 31 + 32 * x;              // row - column; 32 is none
+              float v = 0.f;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const int i = e + 8 * c + 7;
+                if (i >= 0 && i < 39) v += diag[c][i];
+              }
+              const int d = k_warp - q0 + e;
+              if (e == 32) v = 0.f;
+              else if (d <= -wd) far[0] += v;
               else if (d >= wd) far[1] += v;
               else mine[d + wd] += v;
             }
@@ -936,8 +950,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           sums[w * nwin + i] = 0.f;
         }
         out_w[i] = v * a.grad_inv;
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      }                                                      // the next tile's first meeting comes before its sums
       wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
 #pragma unroll
