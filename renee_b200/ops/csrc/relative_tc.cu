@@ -105,6 +105,27 @@ template <typename T> __device__ __forceinline__ void store_row(T* out, const fl
   }
 }
 
+// A warp's 32 rows of 32 values, times f, to global memory through 2 KB of shared memory of its own ([row][64 B], 64-byte swizzle): a
+// thread's row stored from registers touches 32 lines with every instruction, 1000 clocks of each tile.  Rows behind the sequence
+// stay unwritten.  The caller waits (wait_stored) before the memory is used again, and before the kernel ends.
+template <typename T> __device__ __forceinline__ void store_piece(char* own, const CUtensorMap* map, const float (&v)[32], float f, int x, int row, int b, int S,
+                                                                  int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(own + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16) =
+        make_uint4(pack16<T>(v[8 * c] * f, v[8 * c + 1] * f), pack16<T>(v[8 * c + 2] * f, v[8 * c + 3] * f), pack16<T>(v[8 * c + 4] * f, v[8 * c + 5] * f),
+                   pack16<T>(v[8 * c + 6] * f, v[8 * c + 7] * f));
+  tc::fence_proxy_async();
+  __syncwarp();
+  if (lane == 0 && row < S) {
+    tc::tma_store_3d(map, own, x, row, b);
+    tc::tma_store_commit();
+  }
+}
+__device__ __forceinline__ void wait_stored(int lane) {
+  if (lane == 0) tc::tma_store_wait_read<0>();
+}
+
 // own: a tile's rows and window (tiles in turn); raw: copies that are not complete before masked rows are zeros; full / empty: the
 // stages of blocks; scores: a block's first products (blocks in turn); read: they are in registers; done: P or dS is in TMEM (blocks
 // in turn); freed: nothing reads a tile's rows any more; end: its accumulators are complete; taken: they have been read (tiles in
@@ -380,7 +401,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   const int wd = window(a), per = (a.S + ROWS - 1) / ROWS, tiles = per * a.nh * a.b, wfloats = window_floats(wd) + mask_words(a.S);
   float* windows = reinterpret_cast<float*>(stage + NST * 2 * PIECE);           // [2][window, mask]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
-  start<COLS>(&bars, &s_tmem, warp, 1);
+  start<COLS>(&bars, &s_tmem, warp, OWN == 2 ? 1 + WORKERS : 1);
   const uint32_t tmem = s_tmem;
   Waiter wait{false, a.status};
   grid_dep_wait();
@@ -413,6 +434,10 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
     unsigned g = 0, k = 0;
     for (Place at; (at = worker_tile(bars, wait, place, k)).b >= 0; ++k) {
       const int seen = at.seen, n = at.blocks(a), bh = at.bh(a);
+      if (OWN == 2 && k > 0) {                               // the last tile's queries were followed by its context in the same place
+        wait_stored(lane);
+        if (lane == 0) tc::mbar_arrive(bars.freed + (k - 1) % OWN);
+      }
       const bool empty = seen == 0;
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
       const float* win = windows + (k & 1) * wfloats;
@@ -528,17 +553,19 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
       wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
       const float f = 1.f / (1.f - a.p) / l;
-      T* out = a.ctx + (((size_t)at.b * a.S + q) * a.nh + at.h) * HD;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         float v[32];
         tc::tmem_ld32(row_o + half * 32 + 64 * c, v);
         if (c == CH - 1) warp_arrive(bars.taken + (k & 1), lane);
-        if (q < a.S && half * 32 + 64 * c < HD) store_row<T>(out + half * 32 + 64 * c, v, f);
+        if (half * 32 + 64 * c >= HD) continue;
+        if constexpr (OWN == 2) store_piece<T>(sq + (k % OWN) * TILE + warp * 2048, &maps.d, v, f, at.h * HD + half * 32, q_warp, at.b, a.S, lane);
+        else if (q < a.S) store_row<T>(a.ctx + (((size_t)at.b * a.S + q) * a.nh + at.h) * HD + half * 32 + 64 * c, v, f);
       }
       if (half == 0) a.lse[(size_t)bh * a.Sp + q] = q < a.S ? m + (lg2(l) - up) : INFINITY;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
     }
+    wait_stored(lane);
   }
   finish<COLS>(&s_tmem, warp);
 }
@@ -984,8 +1011,9 @@ template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaSt
   int rc = tc::make_tmap_rows(&m.a, a.q, a.b, a.S, H, a.ldq, ROWS, bf);
   if (!rc) rc = tc::make_tmap_rows(&m.b, a.k, a.b, a.S, H, a.ldk, BLK, bf);
   if (!rc) rc = tc::make_tmap_rows(&m.c, a.v, a.b, a.S, H, a.ldv, BLK, bf);
+  if (!rc) rc = tc::make_tmap_rows(&m.d, a.ctx, a.b, a.S, H, H, 32, bf, 32);
   if (rc) return rc;
-  m.d = m.e = m.c;
+  m.e = m.d;
   const int smem = 1024 + (OWN * ROWS + NST * 2 * BLK) * 128 * CH + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
   rc = allow_smem(fwd_tc<T, HD, DROP>, smem);
   if (rc) return rc;

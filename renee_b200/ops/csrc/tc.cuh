@@ -113,6 +113,11 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tmap, const void
                ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(smem_src)), "r"(x), "r"(y)
                : "memory");
 }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* tmap, const void* smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 // Commits the stores issued so far and waits until their shared-memory source has been read.
 __device__ __forceinline__ void tma_store_commit_and_wait_read() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -303,18 +308,20 @@ inline int make_tmap_2d(CUtensorMap* out, const void* base, uint64_t rows, uint6
   return r == CUDA_SUCCESS ? 0 : -22;
 }
 // The rows of a batch of sequences, [batch][rows][cols] with leading dimension ld: a box of 64 columns and box_rows rows of one
-// sequence, 128-byte swizzle; rows behind a sequence's last one read as zeros, not as the next sequence's.
-inline int make_tmap_rows(CUtensorMap* out, const void* base, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, bool bf16) {
+// sequence, 128-byte swizzle (32 columns: 64-byte); rows behind a sequence's last one read as zeros, not as the next sequence's, and are
+// not written.
+inline int make_tmap_rows(CUtensorMap* out, const void* base, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, bool bf16,
+                          uint32_t box_cols = 64) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return -20;
   if ((reinterpret_cast<uintptr_t>(base) & 15) || ((ld * 2) & 15) || box_rows > 256) return -21;
   cuuint64_t dims[3] = {cols, rows, batch};
   cuuint64_t strides[2] = {ld * 2, rows * ld * 2};
-  cuuint32_t box[3] = {64, box_rows, 1};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -22;
 }
 }  // namespace tc
