@@ -338,6 +338,9 @@ __device__ __forceinline__ void copy_query_tiles(const Args<T>& a, Bars& bars, W
 template <int NST, int OWN, int TURNS, typename T, typename Scores, typename Rows>
 __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bars, Waiter& wait, const Place* place, Scores scores, Rows rows) {
   constexpr unsigned SLOTS = TURNS ? TURNS : 2, AHEAD = TURNS ? TURNS - 1 : 1;
+  // Block g needs the stage of g - NST, whose second product is issued behind the scores of g - NST + AHEAD: they must not wait for what
+  // the copying warp does behind block g's copies (block g - 1's masked rows; with two stages it clears them before)
+  static_assert(NST >= AHEAD + (NST == 2 ? 1 : 2), "the ring would wait for itself");
   unsigned g = 0, k = 0, x = 0;                                // blocks begun, tiles begun, second products issued
   unsigned jx = 0, ix = 0, nx = 0, n_last = 0;                 // block x: the ix-th of nx of the CTA's jx-th tile
   const auto second = [&]() {
@@ -732,7 +735,7 @@ template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH;
   constexpr int STAGE = 2 * PIECE + 2 * BLK * 4;             // Q piece, dO piece, -lse, -delta
-  constexpr int STAGE_UP = (STAGE + 1023) / 1024 * 1024, NST = HD == 128 ? 2 : 3, COLS = HD == 128 ? 512 : 256;
+  constexpr int STAGE_UP = (STAGE + 1023) / 1024 * 1024, NST = 2, COLS = HD == 128 ? 512 : 256;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
@@ -1022,7 +1025,7 @@ template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaSt
 }
 
 template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaStream_t st) {
-  constexpr int CH = (HD < 64 ? 64 : HD) / 64, PIECE = BLK * 128 * CH, STAGE_UP = (2 * PIECE + 2 * BLK * 4 + 1023) / 1024 * 1024, NST = HD == 128 ? 2 : 3;
+  constexpr int CH = (HD < 64 ? 64 : HD) / 64, PIECE = BLK * 128 * CH, STAGE_UP = (2 * PIECE + 2 * BLK * 4 + 1023) / 1024 * 1024, NST = HD == 128 ? 2 : 3, NST_KV = 2;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps q, kv;
   const uint64_t H = (uint64_t)a.nh * HD;
@@ -1039,7 +1042,7 @@ template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaSt
   kv.e = kv.d;
   const int wd = window(a), windows = 2 * (window_floats(wd) + mask_words(a.S)) * 4;
   const int smem_q = 1024 + 3 * ROWS * 128 * CH + NST * 2 * PIECE + windows + 2 * ROWS * 4;
-  const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST * STAGE_UP + windows + 8 * (2 * wd + 1) * 4;
+  const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST_KV * STAGE_UP + windows + 8 * (2 * wd + 1) * 4;
   rc = allow_smem(bwd_q_tc<T, HD, DROP>, smem_q);
   if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP>, smem_kv);
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * (HD == 128 ? 1 : 2);
