@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ tabl
   grid_dep_wait();
   if ((int)blockIdx.x < nh) {
     const int wd = min(far, S - 1), n = window_floats(wd);
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += 256) {
       const int d = min(max(i - PAD - wd, -wd), wd);
       const int u = min(max(__ldg(lut + d + far), 0), nb - 1);            // a bucket outside the table reads its nearest row

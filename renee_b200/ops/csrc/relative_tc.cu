@@ -39,7 +39,7 @@ __device__ __forceinline__ V2 operator+(V2 a, V2 b) { return V2{__fadd2_rn(a.v, 
 __device__ __forceinline__ V2 operator*(V2 a, V2 b) { return V2{__fmul2_rn(a.v, b.v)}; }
 __device__ __forceinline__ V2 v2_fma(V2 a, V2 b, V2 c) { return V2{__ffma2_rn(a.v, b.v, c.v)}; }
 
-struct alignas(64) Maps { CUtensorMap a, b, c, d, e; };
+struct alignas(64) Maps { CUtensorMap a, b, c, d, e, f; };
 
 template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
@@ -107,7 +107,7 @@ template <typename T> __device__ __forceinline__ void store_row(T* out, const fl
 
 // A warp's 32 rows of 32 values, times f, to global memory through 2 KB of shared memory of its own ([row][64 B], 64-byte swizzle): a
 // thread's row stored from registers touches 32 lines with every instruction, 1000 clocks of each tile.  Rows behind the sequence
-// stay unwritten.  The caller waits (wait_stored) before the memory is used again, and before the kernel ends.
+// stay unwritten.  The caller waits (wait_stored) before the memory is used again, and for all stores before the kernel ends.
 template <typename T> __device__ __forceinline__ void store_piece(char* own, const CUtensorMap* map, const float (&v)[32], float f, int x, int row, int b, int S,
                                                                   int lane) {
 #pragma unroll
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
       if (half == 0) a.lse[(size_t)bh * a.Sp + q] = q < a.S ? m + (lg2(l) - up) : INFINITY;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
     }
-    wait_stored(lane);
+    if (lane == 0) tc::tma_store_wait_all();
   }
   finish<COLS>(&s_tmem, warp);
 }
@@ -747,7 +747,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   char* stage = sv + TILE;
   const int wd = window(a), per = (a.S + ROWS - 1) / ROWS, tiles = per * a.nh * a.b, nwin = 2 * wd + 1;
   const int wfloats = window_floats(wd) + mask_words(a.S), nq = (a.S + BLK - 1) / BLK;
-  float* windows = reinterpret_cast<float*>(stage + NST * STAGE_UP);            // [2][window, mask]
+  char* pieces = stage + NST * STAGE_UP;                     // [8][2 KB] on their way out
+  float* windows = reinterpret_cast<float*>(pieces + 8 * 2048);                 // [2][window, mask]
   float* sums = windows + 2 * wfloats;                       // [8][nwin]
   const int warp = tc::warp_id(), lane = threadIdx.x & 31;
   start<COLS>(&bars, &s_tmem, warp, 1);
@@ -859,8 +860,6 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     for (Place at; (at = worker_tile(bars, wait, place, k)).b >= 0; ++k) {
       const int bh = at.bh(a);
       const int k_warp = at.row0 + quarter * 32, key = k_warp + lane, n = nq;
-      T* const out_v = a.dv + ((size_t)at.b * a.S + key) * a.lddv + at.h * HD;
-      T* const out_k = a.dk + ((size_t)at.b * a.S + key) * a.lddk + at.h * HD;
       float* const out_w = a.dwin + ((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin;
       const bool flat = at.seen <= 0;
       const float* win = windows + (k & 1) * wfloats;
@@ -994,9 +993,14 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.f;
           }
-          if (key < a.S && 32 * half + 64 * c < HD) store_row<T>((o ? out_k : out_v) + 32 * half + 64 * c, v, o ? a.scale * a.grad_inv : a.grad_inv);
+          if (32 * half + 64 * c >= HD) continue;
+          wait_stored(lane);
+          __syncwarp();
+          store_piece<T>(pieces + warp * 2048, o ? &maps.f : &maps.e, v, o ? a.scale * a.grad_inv : a.grad_inv, at.h * HD + 32 * half + 64 * c, k_warp, at.b,
+                         a.S, lane);
         }
     }
+    if (lane == 0) tc::tma_store_wait_all();
   }
   finish<COLS>(&s_tmem, warp);
 }
@@ -1016,7 +1020,7 @@ template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaSt
   if (!rc) rc = tc::make_tmap_rows(&m.c, a.v, a.b, a.S, H, a.ldv, BLK, bf);
   if (!rc) rc = tc::make_tmap_rows(&m.d, a.ctx, a.b, a.S, H, H, 32, bf, 32);
   if (rc) return rc;
-  m.e = m.d;
+  m.e = m.f = m.d;
   const int smem = 1024 + (OWN * ROWS + NST * 2 * BLK) * 128 * CH + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
   rc = allow_smem(fwd_tc<T, HD, DROP>, smem);
   if (rc) return rc;
@@ -1038,11 +1042,13 @@ template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaSt
   if (!rc) rc = tc::make_tmap_rows(&kv.b, a.k, a.b, a.S, H, a.ldk, ROWS, bf);
   if (!rc) rc = tc::make_tmap_rows(&kv.c, a.v, a.b, a.S, H, a.ldv, ROWS, bf);
   if (!rc) rc = tc::make_tmap_rows(&kv.d, a.dctx, a.b, a.S, H, H, BLK, bf);
+  if (!rc) rc = tc::make_tmap_rows(&kv.e, a.dv, a.b, a.S, H, a.lddv, 32, bf, 32);
+  if (!rc) rc = tc::make_tmap_rows(&kv.f, a.dk, a.b, a.S, H, a.lddk, 32, bf, 32);
   if (rc) return rc;
-  kv.e = kv.d;
+  q.f = q.e;
   const int wd = window(a), windows = 2 * (window_floats(wd) + mask_words(a.S)) * 4;
   const int smem_q = 1024 + 3 * ROWS * 128 * CH + NST * 2 * PIECE + windows + 2 * ROWS * 4;
-  const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST_KV * STAGE_UP + windows + 8 * (2 * wd + 1) * 4;
+  const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST_KV * STAGE_UP + 8 * 2048 + windows + 8 * (2 * wd + 1) * 4;
   rc = allow_smem(bwd_q_tc<T, HD, DROP>, smem_q);
   if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP>, smem_kv);
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * (HD == 128 ? 1 : 2);
