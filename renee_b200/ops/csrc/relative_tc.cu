@@ -803,7 +803,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   } else if (warp > WORKERS) {
     if (tc::elect_one()) {
       unsigned g = 0, k = 0;
-      // the second products of block x, and the wait for them: the next scores go where P~ and dS are
+      // the second products of block x; the next S^T and dP^T go where its P~ and dS are, each as soon as the product that reads them
+      // is complete (raw[0]: P~)
       const auto second = [&](unsigned x, bool first, bool last, unsigned j) {
         wait.one(bars.done + (x & 1), x >> 1, tc::SITE_TMEM_EMPTY);
         if (first && j > 0) wait.one(bars.taken + ((j - 1) & 1), (j - 1) >> 1, tc::SITE_TMEM_EMPTY);
@@ -811,10 +812,10 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         tc::tc_fence_after();
         char* st = stage + (x % NST) * STAGE_UP;
         mma_rows<T, HDP>(tmem + 128, tmem, 32, tc::smem_u32(st + PIECE), first);
+        tc::umma_commit(bars.raw);
         mma_rows<T, HDP>(tmem + 128 + HDP, tmem + 64, 32, tc::smem_u32(st), first);
         tc::umma_commit(bars.empty + x % NST);
         if (last) tc::umma_commit(&bars.end);
-        wait.one(bars.empty + x % NST, x / NST, tc::SITE_EMPTY);
       };
       for (;; ++k) {
         if (g > 0) second(g - 1, nq == 1, true, k - 1);
@@ -823,10 +824,14 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         for (int i = 0; i < nq && !wait.aborted; ++i, ++g) {
           if (i > 0) second(g - 1, i == 1, false, k);
           wait.one(bars.full + g % NST, g / NST, tc::SITE_FULL);
+          if (g > 0) wait.one(bars.raw, g - 1, tc::SITE_EMPTY);
           if (wait.aborted) break;
           tc::tc_fence_after();
           const char* st = stage + (g % NST) * STAGE_UP;
           mma_scores<T, HD>(tmem, tc::smem_u32(sk), tc::smem_u32(st));
+          if (g > 0) wait.one(bars.empty + (g - 1) % NST, (g - 1) / NST, tc::SITE_EMPTY);
+          if (wait.aborted) break;
+          tc::tc_fence_after();
           mma_scores<T, HD>(tmem + 64, tc::smem_u32(sv), tc::smem_u32(st + PIECE));
           tc::umma_commit(bars.scores + (g & 1));
           if (i + 1 == nq) tc::umma_commit(bars.freed);
