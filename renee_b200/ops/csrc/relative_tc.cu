@@ -10,18 +10,19 @@
 // the first products and, as it stands, the MN-major B operand of the second ones).  A thread reads its row of scores from TMEM,
 // works on it, and writes 16-bit P or dS back to TMEM, where they are the A operand of the second product: scores never pass through
 // shared memory, and a row's maximum and sum need no shuffle.
-// CTAs stay (2 per SM; heads of 128: 1) and take the next tile off a counter (texts differ in length: with every gridDim.x-th tile the
+// CTAs stay (2 per SM; backward with heads of 128: 1) and take the next tile off a counter (texts differ in length: with every gridDim.x-th tile the
 // slowest CTA had a third more to do than the average).  Ten warps: 0-7 work on the scores (warp w and w + 4 share 32
 // rows and take 32 columns each), 8 issues copies (one to three blocks ahead, into the next tile's too), 9 issues MMAs from one
 // thread.  A block's scores are issued as soon as their place is free, so that the MMAs run under the exponentials.  MMAs with
 // different accumulators are not taken to run in order: what one reads is overwritten only behind a commit that covers it.
-// Measured (one B200): 32 x 512 x 16 heads of 64, fp16, texts of 128 to 512 tokens: forward 69 us, queries 74, keys 125 (75 GFLOP of
-// products with attended keys in all: 45 us at the GEMM rate; 400 MB: 62 us).  4 x 4099 x 12 heads, forward: 285 us, 148 of them the
-// exponentials' own rate (16 a clock and SM).  What bounds them: instructions and hops.  A worker issues 6 (forward) to 14 (keys)
-// instructions a score, at half of the issue rate with 16 warps an SM (TMEM holds no more rows' scores); a hand-over through an
-// mbarrier takes 200 clocks, and a tile's end and begin cost as much as two to three blocks.  Tried without gain: scores of two blocks
-// in one buffer of 128 columns with 4 warps a CTA, 4 CTAs an SM with one buffer each, P~ and dS of the keys' pass through shared
-// memory (125 -> 150 us: the products' operands from there are then what it is bound by), deeper rings of stages, dependents launched early.
+// Measured (one B200): 32 x 512 x 16 heads of 64, fp16, texts of 128 to 512 tokens: forward 54 us, queries 71, keys 108 (75 GFLOP of
+// products with attended keys in all: 45 us at the GEMM rate; 400 MB: 62 us).  4 x 4099 x 12 heads, forward: 252 us, 148 of them the
+// exponentials' own rate (16 a clock and SM).  What bounds them: instructions and their latency.  A worker issues 7 (forward) to 14
+// (keys) instructions a score, at half of the issue rate with 16 warps an SM (TMEM holds no more rows' scores); in the keys' pass a
+// block's products and their hand-overs, 1700 clocks, stand beside its workers' 2500, and a tile's begin and end cost as much as
+// one to two blocks.  Tried without gain: scores of two blocks in one buffer of 128 columns with 4 warps a CTA, 4 CTAs an SM with one
+// buffer each, P~ and dS of the keys' pass through shared memory (its operands from there are then what it is bound by), more stages
+// (keys: three instead of two 8 us slower), dependents launched early, waits that read the clock later.
 #include "relative.cuh"
 #include "tc.cuh"
 
