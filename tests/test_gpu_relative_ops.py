@@ -155,6 +155,20 @@ def test_attention_in_a_larger_workspace_and_backward_again(S):
             a.check()
 
 
+@pytest.mark.parametrize("shape", [(2, 20, 2, 64), (3, 70, 2, 64), (2, 129, 3, 32), (2, 200, 1, 128)])
+def test_attention_leaves_what_lies_behind(shape):
+    """Outputs as the first rows of longer matrices."""
+    a = Attention(attention_inputs(*shape, torch.bfloat16, "padded"))
+    T, H = a.ctx.shape
+    more = [torch.full((T + 130, w), 7.0, dtype=torch.bfloat16, device=dev()) for w in (H, 4 * H)]
+    a.ctx, a.wide = (m[:T] for m in more)
+    a.dq, a.dk, a.dv = a.wide[:, :H], a.wide[:, H:2 * H], a.wide[:, 3 * H:]
+    a.fwd()
+    a.bwd()
+    a.check()
+    assert all((m[T:] == 7).all() for m in more)
+
+
 def test_attention_on_two_streams_at_once():
     torch.cuda.synchronize()
     calls = [Attention(attention_inputs(3, 300, 2, 64, torch.float16, "padded", seed=s), p=0.1) for s in range(2)]
