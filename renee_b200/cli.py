@@ -195,7 +195,8 @@ def start(local_device: int, ngpus_per_node: int, args) -> None:
             own = trainer.model.embed[0].transformer.state_dict() if args.default_impl else trainer.encoder.encoder_state_dict()
             init_sd = grow_positions(init_sd, own["embeddings.position_embeddings.weight"])
         if args.default_impl:
-            trainer.model.embed[0].transformer.load_state_dict(init_sd, strict=not (args.rotary or args.relative_buckets))
+            from .models.encoder import load_initial_weights
+            load_initial_weights(trainer.model.embed[0].transformer, init_sd)
         else:
             trainer.encoder.load_encoder_state_dict(init_sd, strict=True)
 

@@ -219,6 +219,17 @@ class DistilEncoder(nn.Module):
         return {"last_hidden_state": x}
 
 
+# Parameters of relative positions: an encoder that has them may start from the weights of one that has not
+RELATIVE_PARAMETERS = ("attention.q_norm.weight", "attention.k_norm.weight", "attention.relative_bias.weight")
+
+
+def load_initial_weights(model: nn.Module, sd: dict) -> None:
+    """``sd`` into ``model``: every parameter has to be there and nothing else, but for parameters of relative positions, which keep
+    their first values where ``sd`` has none."""
+    kept = {n: t for n, t in model.state_dict().items() if n.endswith(RELATIVE_PARAMETERS) and n not in sd}
+    model.load_state_dict({**sd, **kept}, strict=True)
+
+
 def grow_positions(sd: dict, own: torch.Tensor) -> dict:
     """``sd`` with a position table of as many rows as ``own`` has: its rows, then those of ``own`` (an encoder with relative positions
     may read longer texts than the checkpoint it starts from)."""

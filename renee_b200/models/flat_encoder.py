@@ -41,7 +41,7 @@ import torch
 
 from .. import ops
 from ..utils import guard
-from .encoder import EncoderConfig
+from .encoder import RELATIVE_PARAMETERS, EncoderConfig
 
 ALIGN = 128  # elements; keeps every parameter 256-byte aligned in bf16
 
@@ -226,8 +226,7 @@ class FlatEncoder:
 
     def load_encoder_state_dict(self, sd: dict, strict: bool = True) -> None:
         # weights of an encoder without relative positions can be loaded: its new parameters keep their first values
-        new = ("attention.q_norm.weight", "attention.k_norm.weight", "attention.relative_bias.weight")
-        missing = [n for n in self.encoder_param_names if n not in sd and not n.endswith(new)]
+        missing = [n for n in self.encoder_param_names if n not in sd and not n.endswith(RELATIVE_PARAMETERS)]
         if strict and missing:
             raise KeyError(f"missing encoder keys: {missing[:4]} ...")
         for n in self.encoder_param_names:
