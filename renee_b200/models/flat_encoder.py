@@ -224,11 +224,15 @@ class FlatEncoder:
     def encoder_state_dict(self) -> dict:
         return {n: self.view(self.p32, n).detach().clone() for n in self.encoder_param_names}
 
-    def load_encoder_state_dict(self, sd: dict, strict: bool = True) -> None:
-        # weights of an encoder without relative positions can be loaded: its new parameters keep their first values
-        missing = [n for n in self.encoder_param_names if n not in sd and not n.endswith(RELATIVE_PARAMETERS)]
+    def load_encoder_state_dict(self, sd: dict, strict: bool = True, initial: bool = True) -> None:
+        """Strict: every parameter has to be there.  As ``initial`` weights those of an encoder without relative positions will do
+        (the parameters of these keep their first values); the other way round an encoder would be another function."""
+        missing = [n for n in self.encoder_param_names if n not in sd and not (initial and n.endswith(RELATIVE_PARAMETERS))]
         if strict and missing:
             raise KeyError(f"missing encoder keys: {missing[:4]} ...")
+        foreign = [n for n in sd if n.endswith(RELATIVE_PARAMETERS) and n not in self.slots]
+        if strict and foreign:
+            raise KeyError(f"the weights are those of an encoder with relative positions, this one has none of {foreign[:4]} ...")
         for n in self.encoder_param_names:
             if n in sd:
                 self.view(self.p32, n).copy_(sd[n].to(self.p32.device, torch.float32))

@@ -466,7 +466,7 @@ class XCTrainer:
             return
         self.xfc.load_weight(sd["xfc_weight"])
         pre = "embed.0.transformer."
-        self.encoder.load_encoder_state_dict({k[len(pre):]: v for k, v in sd.items() if k.startswith(pre)})
+        self.encoder.load_encoder_state_dict({k[len(pre):]: v for k, v in sd.items() if k.startswith(pre)}, initial=False)
         if self.cfg.bottleneck_dims > 0:
             self.encoder.bottleneck_weight().copy_(sd["embed.1.transformer_weight"].to(self.device, torch.float32))
             self.encoder.sync_compute_copy()

@@ -39,3 +39,26 @@ def test_the_command_refuses_weights_of_which_nothing_fits(tmp_path, monkeypatch
             "--epochs", "1", "--results-dir", str(tmp_path / "r"), "--encoder-weights", str(tmp_path / "w.pt")] + options
     with pytest.raises(RuntimeError, match="foreign"):
         start(0, 1, build_parser().parse_args(argv))
+
+
+def test_the_engine_refuses_an_encoder_of_another_kind():
+    plain, rel = FlatEncoder(BASE, "cpu", torch.float32), FlatEncoder(dataclasses.replace(BASE, **RELATIVE), "cpu", torch.float32)
+    rel.load_encoder_state_dict(plain.encoder_state_dict())
+    with pytest.raises(KeyError, match="relative"):
+        plain.load_encoder_state_dict(rel.encoder_state_dict())
+    with pytest.raises(KeyError, match="missing"):
+        rel.load_encoder_state_dict(plain.encoder_state_dict(), initial=False)
+    rel.load_encoder_state_dict(rel.encoder_state_dict(), initial=False)
+
+
+def test_a_trained_state_is_not_taken_by_an_encoder_of_another_kind():
+    from renee_b200.parallel.dist import DistContext
+    from renee_b200.train import TrainConfig, XCTrainer
+    from renee_b200.utils.sharding import shard_labels
+    cfg = TrainConfig(batch_size=4, epochs=1, seed=0, dropout=0.3, lr1=0.05, lr2=1e-3, warmup=2, wd1=1e-4, noloss=True, maxlen=8, pooling="mean")
+    plain, rel = (XCTrainer(cfg, c, shard_labels(40, 1), DistContext(device=torch.device("cpu")), steps_per_epoch=2)
+                  for c in (BASE, dataclasses.replace(BASE, **RELATIVE)))
+    for tr, other in ((plain, rel), (rel, plain)):
+        with pytest.raises(KeyError):
+            tr.load_state_dict(other.state_dict())
+        tr.load_state_dict(tr.state_dict())
