@@ -47,6 +47,11 @@ class EncoderConfig:
     relative_max_distance: int = 128
     gelu8: bool = False                # engine only: the FFN keeps its pre-activation in 8 bits and makes its activation again
 
+    def __post_init__(self):
+        if self.relative_buckets != 0:
+            from ..ops import relative_buckets
+            relative_buckets(self.relative_buckets, self.relative_max_distance)      # refuses what has no buckets
+
     @property
     def hidden_size(self) -> int:  # HF alias used by the reference (main.py:149,152)
         return self.dim

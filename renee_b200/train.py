@@ -168,6 +168,8 @@ class XCTrainer:
     # ------------------------------------------------------------------ construction
     def _init_default(self) -> None:
         cfg = self.cfg
+        if self.enc_cfg.gelu8:
+            raise ValueError("8-bit pre-activations (gelu8) are the engine's: the default implementation keeps its own")
         torch.manual_seed(cfg.seed)
         self.model = DefaultModel(self.enc_cfg, self.Ls, cfg).to(self.device)
         xfc_params, tf_groups = split_param_groups(self.model.named_parameters(), cfg.wd2)

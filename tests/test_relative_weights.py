@@ -62,3 +62,21 @@ def test_a_trained_state_is_not_taken_by_an_encoder_of_another_kind():
         with pytest.raises(KeyError):
             tr.load_state_dict(other.state_dict())
         tr.load_state_dict(tr.state_dict())
+
+
+@pytest.mark.parametrize("buckets,far", [(-4, 128), (3, 128), (32, 8), (32, 513), (32, 0)])
+def test_encoders_refuse_buckets_that_there_are_not(buckets, far):
+    with pytest.raises(ValueError, match="no buckets"):
+        dataclasses.replace(BASE, relative_buckets=buckets, relative_max_distance=far)
+    assert dataclasses.replace(BASE, relative_max_distance=far).relative_buckets == 0
+
+
+@pytest.mark.parametrize("options", [["--relative-buckets", "-4"], ["--relative-buckets", "32", "--relative-max-distance", "600"],
+                                     ["--default-impl", "--gelu8"]])
+def test_the_command_refuses_options_that_it_cannot_follow(tmp_path, monkeypatch, options):
+    import renee_b200.models.encoder as encoder
+    monkeypatch.setattr(encoder, "config_from_name", lambda name: BASE)
+    argv = ["--cpu", "--synthetic-labels", "40", "--synthetic-train", "16", "--synthetic-test", "8", "--maxlen", "16", "--batch-size", "4",
+            "--epochs", "1", "--results-dir", str(tmp_path / "r")] + options
+    with pytest.raises(ValueError, match="no buckets|engine"):
+        start(0, 1, build_parser().parse_args(argv))
