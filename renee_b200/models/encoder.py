@@ -149,7 +149,7 @@ class SelfAttention(nn.Module):
         q, k, v = self.q_lin(x), self.k_lin(x), split(self.v_lin(x))
         if self.rotary:
             from ..ops import reference, rotary_table
-            table = rotary_table(S, hd, self.rotary_base, x.device).to(x.dtype)
+            table = rotary_table(S, hd, self.rotary_base, x.device)          # fp32 whatever x is: cosines in 16 bits would be a rounding more
             q, k = reference.qk_norm_rotary_fwd(torch.cat([q, k], -1).view(b * S, 2 * self.dim), self.q_norm.weight, self.k_norm.weight, table, S,
                                                 self.n_heads, self.rotary_eps).view(b, S, 2 * self.dim).chunk(2, -1)
         q, k = split(q), split(k)

@@ -142,3 +142,15 @@ def test_command_line():
     cfg = _encoder_config(parse(["--rotary", "--relative-buckets", "32", "--gelu8", "--maxlen", "1024"]))
     assert cfg.rotary and cfg.relative_buckets == 32 and cfg.relative_max_distance == 128 and cfg.gelu8 and cfg.max_position_embeddings == 1024
     assert _encoder_config(parse(["--maxlen", "1024"])).max_position_embeddings == 512
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_the_module_rotates_by_cosines_in_32_bits(dt, monkeypatch):
+    from renee_b200.ops import reference
+    seen = []
+    whole = reference.qk_norm_rotary_fwd
+    monkeypatch.setattr(reference, "qk_norm_rotary_fwd", lambda *a: seen.append(a[3]) or whole(*a))
+    mod = DistilEncoder(dataclasses.replace(BASE, rotary=True)).to(dt)
+    ids, mask = inputs()
+    mod(input_ids=ids, attention_mask=mask)
+    assert len(seen) == 2 and all(torch.equal(t, ops.rotary_table(12, 64)) for t in seen)
