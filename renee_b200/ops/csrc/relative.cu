@@ -8,6 +8,7 @@
 // P and dS are rounded to the activations' type as operands of the second products, as P is forward; everything else is fp32.
 // fp16's least numbers are near: P is kept up to 2^6 above its true size forward, and backward P and dS carry the power of two
 // next below sqrt(S) (P ~ 1 / S there), which the sums are divided by at the end.
+#include <climits>
 #include "mma16.cuh"
 #include "partials.cuh"
 #include "relative.cuh"
@@ -111,13 +112,14 @@ template <int SP> __device__ __forceinline__ void short_exponents(float (&s)[SP 
 }
 // dropout decisions of one fragment as bits (bit 4 j + e)
 template <typename T, int SP> __device__ __forceinline__ uint32_t kept_bits(const Args<T>& a, uint32_t seed, int bh, int q, int t) {
+  const Dropout dr = dropout_of(a, seed, bh);
   uint32_t m = 0;
 #pragma unroll
   for (int j = 0; j < SP / 8; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t i = ((uint32_t)bh * a.S + q + 8 * (e >> 1)) * (uint32_t)a.S + 8 * j + 2 * t + (e & 1);
-      m |= (uint32_t)keep(seed, a.stream, i, a.p) << (4 * j + e);
+      const uint32_t i = (dr.head * a.S + q + 8 * (e >> 1)) * (uint32_t)a.S + 8 * j + 2 * t + (e & 1);
+      m |= (uint32_t)keep(dr.seed, dr.stream, i, a.p) << (4 * j + e);
     }
   return m;
 }
@@ -415,6 +417,8 @@ template <typename T> Args<T> args(const Common& c) {
   a.scale = 1.f / sqrtf((float)c.hd);
   a.scale_log2 = LOG2E * a.scale;
   a.p = c.p; a.seed = (const int*)c.seed; a.stream = c.stream;
+  const long long page = (1LL << 32) / ((long long)c.S * c.S);
+  a.page = (int)(page < INT_MAX ? page : INT_MAX);
   a.Sp = (c.S + 127) / 128 * 128; a.status = (int*)c.status;
   return a;
 }

@@ -35,6 +35,7 @@ template <typename T> struct Args {
   float p;
   const int* seed;
   uint32_t stream;
+  int page;                      // heads whose dropout decisions share a stream
   T* ctx;                        // [b S][nh HD]
   float *lse;                    // [b][nh][Sp] in base 2, of the scaled and biased scores
   float *delta, *lse_up;         // the same shape, from the queries' backward pass: delta, and lse - grad_log2; behind S zero and infinity
@@ -71,6 +72,16 @@ __device__ __forceinline__ float lg2(float x) {
 }
 
 inline int up16(int bytes) { return (bytes + 15) / 16 * 16; }
+
+// Dropout: probability (q, k) of head bh is number ((bh % page) S + q) S + k of stream + 2^12 (bh / page).  A number has 32 bits, so
+// page = floor(2^32 / S^2) heads use one stream up; those of the other call sites lie below 2^12 (ops/rng.py: PairNumbers).
+struct Dropout {
+  uint32_t seed, stream, head;
+};
+template <typename T> __device__ __forceinline__ Dropout dropout_of(const Args<T>& a, uint32_t seed, int bh) {
+  const int n = bh / a.page;
+  return Dropout{seed, a.stream + ((uint32_t)n << 12), (uint32_t)(bh - n * a.page)};
+}
 
 // The kernels of relative_tc.cu, for sequences of more than 64 tokens
 template <typename T> int fwd_on_tensor_cores(const Args<T>& a, int hd, cudaStream_t st);

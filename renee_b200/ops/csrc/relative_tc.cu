@@ -446,7 +446,8 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
       const float* win = windows + (k & 1) * wfloats;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
-      const uint32_t drop0 = ((uint32_t)bh * a.S + q) * (uint32_t)a.S;
+      const Dropout dr = DROP ? dropout_of(a, seed, bh) : Dropout{};
+      const uint32_t drop0 = (dr.head * a.S + q) * (uint32_t)a.S;
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + 32 * half, dlo = k0 - (q_warp + 31), dhi = k0 + 31 - q_warp;     // of this warp's columns
@@ -518,8 +519,8 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
             s[j + 1] = ex2(s[j + 1]);
             l2[(j >> 1) & 1] = l2[(j >> 1) & 1] + v2(s[j], s[j + 1]);
             if (DROP) {
-              if (!keep(seed, a.stream, drop0 + k0 + j, a.p)) s[j] = 0.f;
-              if (!keep(seed, a.stream, drop0 + k0 + j + 1, a.p)) s[j + 1] = 0.f;
+              if (!keep(dr.seed, dr.stream, drop0 + k0 + j, a.p)) s[j] = 0.f;
+              if (!keep(dr.seed, dr.stream, drop0 + k0 + j + 1, a.p)) s[j + 1] = 0.f;
             }
             r[j / 2] = pack16<T>(s[j], s[j + 1]);
           }
@@ -635,7 +636,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       const float* win = windows + (k & 1) * wfloats;
       const float lse = q < a.S ? (seen < 0 ? 0.f : win[wfloats - ROWS + row]) - a.grad_log2 : INFINITY;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
-      const uint32_t drop0 = ((uint32_t)bh * a.S + q) * (uint32_t)a.S + half * 32;
+      const Dropout dr = DROP ? dropout_of(a, seed, bh) : Dropout{};
+      const uint32_t drop0 = (dr.head * a.S + q) * (uint32_t)a.S + half * 32;
       float d = 0.f;                                         // delta = dctx ctx: half a row each
 #pragma unroll
       for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
@@ -668,8 +670,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             if (DROP) {
-              dp[j] = keep(seed, a.stream, drop0 + i * BLK + j, a.p) ? dp[j] * kept : 0.f;
-              dp[j + 1] = keep(seed, a.stream, drop0 + i * BLK + j + 1, a.p) ? dp[j + 1] * kept : 0.f;
+              dp[j] = keep(dr.seed, dr.stream, drop0 + i * BLK + j, a.p) ? dp[j] * kept : 0.f;
+              dp[j + 1] = keep(dr.seed, dr.stream, drop0 + i * BLK + j + 1, a.p) ? dp[j + 1] * kept : 0.f;
             }
             if constexpr (W::MASK) {                         // a masked key's V may hold anything
               if (!(on >> j & 1u)) dp[j] = 0.f;
@@ -864,7 +866,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
       for (int i = threadIdx.x; i < nwin; i += 256) a.dwin[((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin + i] = 0.f;
     }
     for (Place at; (at = worker_tile(bars, wait, place, k)).b >= 0; ++k) {
-      const int bh = at.bh(a);
+      const Dropout dr = DROP ? dropout_of(a, seed, at.bh(a)) : Dropout{};
       const int k_warp = at.row0 + quarter * 32, key = k_warp + lane, n = nq;
       float* const out_w = a.dwin + ((size_t)(at.b * per + at.row0 / ROWS) * a.nh + at.h) * nwin;
       const bool flat = at.seen <= 0;
@@ -905,8 +907,8 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
               const V2 pr = v2(ex2(x), ex2(y));
               V2 v = v2(dp[c], dp[c + 1]);
               if (DROP) {
-                const uint32_t at0 = ((uint32_t)bh * a.S + q0 + c) * (uint32_t)a.S + key;
-                const V2 kf = v2(keep(seed, a.stream, at0, a.p) ? kept : 0.f, keep(seed, a.stream, at0 + (uint32_t)a.S, a.p) ? kept : 0.f);
+                const uint32_t at0 = (dr.head * a.S + q0 + c) * (uint32_t)a.S + key;
+                const V2 kf = v2(keep(dr.seed, dr.stream, at0, a.p) ? kept : 0.f, keep(dr.seed, dr.stream, at0 + (uint32_t)a.S, a.p) ? kept : 0.f);
                 v = v * kf;
                 v2_get(pr * kf, x, y);
               } else {

@@ -14,7 +14,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from .rng import keep_mask
+from .rng import PairNumbers, keep_mask
 
 
 def _mask(seed, stream, shape, p, device):
@@ -160,6 +160,10 @@ def _relative_probs(q, k, mask, table, buckets, nh):
     return qh, kh, torch.softmax(s, -1), bucket, some, seen
 
 
+def _pair_mask(seed, stream, shape, p, device):
+    return PairNumbers(stream, shape[-1]).keep_mask(seed, shape[0] * shape[1], p, device).view(shape)
+
+
 def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, seed, stream):
     """Attention with a bias by buckets of key - query; masked keys count as absent, a sequence without an attended key
     attends to all of its tokens alike (kernels: relative.cu).  Returns ``ctx[b S, nh hd]``."""
@@ -168,7 +172,7 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, seed, stream):
     vh = _wide(v).reshape(b, S, nh, -1).transpose(1, 2)
     vh = torch.where((seen | ~some).transpose(-1, -2), vh, torch.zeros_like(vh))
     if p > 0:
-        w = w * _mask(seed, stream, w.shape, p, w.device) / (1.0 - p)
+        w = w * _pair_mask(seed, stream, w.shape, p, w.device) / (1.0 - p)
     return torch.matmul(w, vh).transpose(1, 2).reshape(q.shape).to(q.dtype)
 
 
@@ -179,7 +183,7 @@ def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, seed, str
     qh, kh, w, bucket, some, seen = _relative_probs(q, k, mask, table, buckets, nh)
     vh, do = (_wide(t).reshape(b, S, nh, hd).transpose(1, 2) for t in (v, dctx))
     vh = torch.where((seen | ~some).transpose(-1, -2), vh, torch.zeros_like(vh))
-    keep = _mask(seed, stream, w.shape, p, w.device) / (1.0 - p) if p > 0 else torch.ones_like(w)
+    keep = _pair_mask(seed, stream, w.shape, p, w.device) / (1.0 - p) if p > 0 else torch.ones_like(w)
     dv = torch.matmul((w * keep).transpose(-1, -2), do)
     dp = torch.matmul(do, vh.transpose(-1, -2)) * keep
     ds = torch.where(some, w * (dp - (dp * w).sum(-1, keepdim=True)), torch.zeros_like(w))

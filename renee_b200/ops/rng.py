@@ -55,6 +55,26 @@ def keep_mask(seed, stream: int, shape, p: float, device="cpu") -> torch.Tensor:
     return (u >= p).view(*shape)
 
 
+class PairNumbers:
+    """Where the dropout decisions of attention probabilities ``[heads, S, S]`` come from: numbers have 32 bits, so as many heads as
+    fit share the call's stream, the next ones take the stream 2^12 further (those of other call sites lie below), and so on."""
+    NUMBERS = 1 << 32
+
+    def __init__(self, stream: int, S: int):
+        self.stream, self.S = int(stream), int(S)
+        self.page = self.NUMBERS // (self.S * self.S)
+
+    def of(self, head: int) -> tuple:
+        """(stream, number of the head's first probability)"""
+        n, place = divmod(head, self.page)
+        return self.stream + (n << 12), place * self.S * self.S
+
+    def keep_mask(self, seed, heads: int, p: float, device="cpu") -> torch.Tensor:
+        """Boolean ``[heads, S, S]``."""
+        parts = [keep_mask(seed, self.of(h)[0], (min(self.page, heads - h), self.S, self.S), p, device) for h in range(0, max(heads, 1), self.page)]
+        return torch.cat(parts) if len(parts) != 1 else parts[0]
+
+
 class DropoutRNG:
     """Host-side handle: base seed plus a per-step counter; ``stream`` ids name the call sites."""
 

@@ -190,3 +190,43 @@ def test_gelu8_refuses(change):
     a.update(change)
     with pytest.raises(ValueError):
         ops.gelu8_fwd(**a)
+
+
+@pytest.mark.parametrize("heads", [0, 1, 5, 7])
+def test_dropout_numbers_beyond_32_bits(heads, monkeypatch):
+    """Heads that share a stream are numbered through; no two heads share their decisions, however many there are."""
+    from renee_b200.ops.rng import PairNumbers, keep_mask
+    S, p = 40, 0.4
+    assert torch.equal(PairNumbers(3, S).keep_mask(5, heads, p), keep_mask(5, 3, (heads, S, S), p))
+    monkeypatch.setattr(PairNumbers, "NUMBERS", 2 * S * S + 17)                    # two heads a stream
+    n = PairNumbers(3, S)
+    assert n.page == 2 and [n.of(h) for h in range(5)] == [(3, 0), (3, S * S), (4099, 0), (4099, S * S), (8195, 0)]
+    got = n.keep_mask(5, heads, p)
+    assert got.shape == (heads, S, S)
+    for h in range(heads):
+        stream, first = n.of(h)
+        assert torch.equal(got[h].reshape(-1), keep_mask(5, stream, (first + S * S,), p)[first:])
+        for other in range(h):                       # independent decisions agree at p^2 + (1 - p)^2 = 0.52 of 1600 places: 6 deviations
+            assert abs((got[h] == got[other]).float().mean().item() - 0.52) < 6 * 0.0125
+
+
+def test_dropout_numbers_of_the_longest_sequences():
+    from renee_b200.ops.rng import PairNumbers
+    n = PairNumbers(12, 65536)
+    assert n.page == 1 and [n.of(h) for h in (0, 1, 70000)] == [(12, 0), (12 + 4096, 0), (12 + 4096 * 70000, 0)]
+
+
+def test_attention_oracle_takes_heads_beyond_32_bits(monkeypatch):
+    from renee_b200.ops import reference as ref
+    from renee_b200.ops.rng import PairNumbers
+    b, S, nh, hd = 3, 10, 2, 32
+    monkeypatch.setattr(PairNumbers, "NUMBERS", 4 * S * S)
+    T, H = b * S, nh * hd
+    zero, v = torch.zeros(T, H), torch.randn(T, H, generator=torch.Generator().manual_seed(0))
+    args = (torch.ones(b, S, dtype=torch.int32), torch.zeros(8, nh), ops.relative_buckets(8, 4), nh, 0.5, 7, 3)
+    w = PairNumbers(3, S).keep_mask(7, b * nh, 0.5).view(b, nh, S, S).float() * 2 / S
+    heads = lambda t: t.view(b, S, nh, hd).transpose(1, 2)
+    got = ref.relative_attention_fwd(zero, zero, v, *args)
+    torch.testing.assert_close(heads(got), w @ heads(v))
+    dv = ref.relative_attention_bwd(v, zero, zero, v, *args)[2]
+    torch.testing.assert_close(heads(dv), w.transpose(-1, -2) @ heads(v))
