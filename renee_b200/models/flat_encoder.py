@@ -316,6 +316,8 @@ class FlatEncoder:
         classifier-input dropout)."""
         cfg = self.cfg
         b, S = input_ids.shape
+        if S > cfg.max_position_embeddings:
+            raise ValueError(f"sequences of {S} tokens: the encoder has {cfg.max_position_embeddings} positions")
         self._alloc(b, S)
         A = self._acts
         T, H = b * S, cfg.dim

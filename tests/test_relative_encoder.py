@@ -154,3 +154,13 @@ def test_the_module_rotates_by_cosines_in_32_bits(dt, monkeypatch):
     ids, mask = inputs()
     mod(input_ids=ids, attention_mask=mask)
     assert len(seen) == 2 and all(torch.equal(t, ops.rotary_table(12, 64)) for t in seen)
+
+
+@pytest.mark.parametrize("change", [dict(), *VARIANTS.values()])
+def test_longer_texts_than_positions_are_refused(change):
+    """The table of learned positions has a row for each: there is none to read, nor to write a gradient to, behind the last."""
+    flat = FlatEncoder(dataclasses.replace(BASE, **change), "cpu", torch.float32)
+    ids, mask = inputs(S=BASE.max_position_embeddings)
+    flat.forward(ids, mask, ops.StepRNG(0), train=True)
+    with pytest.raises(ValueError, match="17 tokens"):
+        flat.forward(*(torch.cat([t, t[:, :1]], 1) for t in (ids, mask)), ops.StepRNG(0), train=True)
