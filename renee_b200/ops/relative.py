@@ -285,6 +285,12 @@ def _seed_sig(p, rng):
     return _sig(rng.dev) if p > 0 and rng is not None and rng.dev is not None else None
 
 
+def _forward_call(q, sizes, p, stream) -> tuple:
+    """What a backward call must have in common with the forward call that filled its workspace.  (That no other call of the same kind
+    came between is the caller's to see to, as for the activations themselves.)"""
+    return (q.dtype, p, stream if p > 0 else None, *sizes)
+
+
 def _check_ws(ws, device, need) -> None:
     at, *have = ws.sizes
     _refuse(at != device or any(h < n for h, n in zip(have, need)),
@@ -315,14 +321,18 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ct
         numbers = _passed(key, (_ld(q), _ld(k), _ld(v), (far, table.shape[0], b, S, nh, hd)))
     at = _pointers(1, ctx_out, q, k, v, table)
     if q.is_cuda:
-        ws.filled = numbers[3]
-        return _cuda().relative_attention_fwd(at, numbers, q, mask, buckets, p, rng, stream, ws)
+        ws.filled = None                                     # a call that fails leaves nothing to go back from
+        _cuda().relative_attention_fwd(at, numbers, q, mask, buckets, p, rng, stream, ws)
+        ws.filled = _forward_call(q, numbers[3], p, stream)
+        return
     ctx_out.copy_(ref.relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream))
 
 
 def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stream, ctx, ws, dq, dk, dv, dtable) -> None:
     """Gradients of :func:`relative_attention_fwd` from its inputs, its output ``ctx`` and the workspace it filled: ``dq``, ``dk``,
-    ``dv`` (rows may lie apart) and ``dtable`` ``[buckets, nh]``, all written, not accumulated.  May be called again."""
+    ``dv`` (rows may lie apart) and ``dtable`` ``[buckets, nh]``, all written, not accumulated.  May be called again.  The last forward
+    call on ``ws`` must have been the one with these inputs: one of other sizes, another type, dropout or stream of decisions, or one
+    that failed is refused, but another call of the same kind (an evaluation between the passes) cannot be told from it."""
     key = ("relative'", torch.cuda.current_device() if q.is_cuda else -1, nh, p, q.shape, q.stride(), q.dtype, q.device,
            k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, mask.shape, mask.stride(), mask.dtype,
            mask.device, table.shape, table.stride(), table.dtype, table.device, buckets.shape, buckets.stride(), buckets.dtype,
@@ -342,7 +352,8 @@ def relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng, stre
         numbers = _passed(key, (_ld(q), _ld(k), _ld(v), (far, table.shape[0], b, S, nh, hd), _ld(dq), _ld(dk), _ld(dv)))
     at = _pointers(4, dq, dk, dv, dtable, q, k, v, dctx, ctx, table)
     if q.is_cuda:
-        _refuse(ws.filled != numbers[3], "the workspace was not filled by the forward call of these sizes")
+        _refuse(ws.filled != _forward_call(q, numbers[3], p, stream),
+                "the workspace was not filled by a forward call of these sizes, type, dropout and stream of decisions")
         return _cuda().relative_attention_bwd(at, numbers, q, buckets, p, rng, stream, ws)
     g = ref.relative_attention_bwd(dctx, q, k, v, mask, table, buckets, nh, p, rng.seed if p > 0 else 0, stream)
     for out, t in zip((dq, dk, dv, dtable), g):
