@@ -179,7 +179,7 @@ def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, posit
     key = ("rotary'", torch.cuda.current_device() if x.is_cuda else -1, S, nh, eps, x.shape, x.stride(), x.dtype, x.device,
            gq.shape, gq.stride(), gq.dtype, gq.device, gk.shape, gk.stride(), gk.dtype, gk.device, table.shape, table.stride(),
            table.dtype, table.device, dy.shape, dy.stride(), dy.dtype, dy.device, dx.shape, dx.stride(), dx.dtype, dx.device,
-           dgq.shape, dgq.stride(), dgq.dtype, dgq.device, dgk.shape, dgk.stride(), dgk.dtype, dgk.device, ws.numel(), ws.dtype,
+           dgq.shape, dgq.stride(), dgq.dtype, dgq.device, dgk.shape, dgk.stride(), dgk.dtype, dgk.device, ws.numel(), ws.is_contiguous(), ws.dtype,
            ws.device, None if positions is None else _sig(positions))
     numbers = _CHECKED.get(key)
     if numbers is None:
@@ -189,7 +189,7 @@ def qk_norm_rotary_bwd(dy, x, gq, gk, table, S, nh, eps, ws, dx, dgq, dgk, posit
         _same_place(x, dgq=dgq, dgk=dgk)
         if x.is_cuda:
             need = _cuda().qk_norm_rotary_blocks(x.shape[0], nh, hd) * 2 * hd
-            _refuse(ws.numel() < need or ws.device != x.device or ws.dtype != torch.float32,
+            _refuse(ws.numel() < need or not ws.is_contiguous() or ws.device != x.device or ws.dtype != torch.float32,
                     f"the workspace is for fewer tokens: {ws.numel()} values on {ws.device}, the call needs {need} on {x.device}")
         numbers = _passed(key, (_ld(dy), _ld(x), _ld(dx), (x.shape[0], table.shape[0], S, nh, hd, eps)))
     dy_ = dy.data_ptr()
@@ -273,7 +273,7 @@ def _check_relative(q, k, v, mask, table, buckets, nh, p, rng, **like_q):
     _refuse(not 0.0 <= p <= MAX_DROPOUT, f"dropout probability {p}: 0 to {MAX_DROPOUT}")
     _refuse(p > 0.0 and rng is None, "dropout needs the step's seed")
     if q.is_cuda:
-        _refuse(p > 0.0 and (rng.dev is None or rng.dev.dtype != torch.int32 or rng.dev.device != q.device),
+        _refuse(p > 0.0 and (rng.dev is None or rng.dev.dtype != torch.int32 or rng.dev.device != q.device or rng.dev.numel() < 1),
                 "dropout needs the step's seed as an int32 tensor on the device")
         _refuse(S > MAX_TOKENS, f"sequences of {S} tokens: the kernels have at most {MAX_TOKENS}")
         _refuse(b * nh * ((S + 15) // 16) >= 2 ** 31, f"{b} sequences of {S} tokens with {nh} heads are too many for one call")
@@ -428,14 +428,14 @@ def gelu8_bwd(da, saved, ws, dbias, dx, act_out) -> None:
     key = ("gelu8'", torch.cuda.current_device() if da.is_cuda else -1, da.shape, da.stride(), da.dtype, da.device, q.shape, q.stride(),
            q.dtype, q.device, scale.shape, scale.stride(), scale.dtype, scale.device, dbias.shape, dbias.stride(), dbias.dtype,
            dbias.device, dx.shape, dx.stride(), dx.dtype, dx.device, act_out.shape, act_out.stride(), act_out.dtype, act_out.device,
-           ws.numel(), ws.dtype, ws.device)
+           ws.numel(), ws.is_contiguous(), ws.dtype, ws.device)
     if key not in _CHECKED:
         T, F = _check_gelu8(saved, da=da, dx=dx, act_out=act_out)
         _whole("dbias", dbias, (F,), da.dtype)
         _same_place(da, dbias=dbias)
         if da.is_cuda:
             need = _cuda().gelu8_splits(T, F) * F
-            _refuse(ws.numel() < need or ws.device != da.device or ws.dtype != torch.float32,
+            _refuse(ws.numel() < need or not ws.is_contiguous() or ws.device != da.device or ws.dtype != torch.float32,
                     f"the workspace is for fewer rows: {ws.numel()} values on {ws.device}, the call needs {need} on {da.device}")
         _passed(key, ())
     da_, dx_, q_ = da.data_ptr(), dx.data_ptr(), q.data_ptr()
