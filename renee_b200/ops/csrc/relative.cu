@@ -7,7 +7,8 @@
 //              dtable adds those sums up and maps them to buckets.  All sums have a fixed order.
 // P and dS are rounded to the activations' type as operands of the second products, as P is forward; everything else is fp32.
 // fp16's least numbers are near: P is kept up to 2^6 above its true size forward, and backward P and dS carry the power of two
-// next below sqrt(S) (P ~ 1 / S there), which the sums are divided by at the end.
+// next below sqrt(S) (P ~ 1 / S there), which the sums are divided by at the end.  Its greatest is near, too: where gradients are so
+// large that dS would leave its range with that factor, or without, a (sequence, head) takes a smaller one for dS.
 #include <climits>
 #include "mma16.cuh"
 #include "partials.cuh"
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(W * 32) fwd_short(Args<T> a) {
 template <typename T, int HD, int W>
 __global__ void __launch_bounds__(W * 32) bwd_short(Args<T> a) {
   constexpr int SP = W * 16;
+  constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ __align__(16) char smem[];
   Carve cv{smem};
   T* sq = cv.take<T>(SP * (HD + 8));
@@ -241,15 +243,39 @@ __global__ void __launch_bounds__(W * 32) bwd_short(Args<T> a) {
     }
   delta[0] = quad_sum(delta[0]) * a.grad_inv;                        // P carries 2^grad_log2
   delta[1] = quad_sum(delta[1]) * a.grad_inv;
+#pragma unroll
+  for (int j = 0; j < SP / 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dp[j][e] = flat ? 0.f : s[j][e] * (dp[j][e] - delta[e >> 1]);
+  float ds_inv = a.grad_inv;
+  if constexpr (FP16) {                                              // dS beyond fp16's range: the CTA takes a smaller factor
+    float most = 0.f;                                                // of the finite ones; the others are lost whatever the factor is
+#pragma unroll
+    for (int j = 0; j < SP / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(dp[j][e]) < INFINITY ? fabsf(dp[j][e]) : 0.f);
+    if (__syncthreads_or(most > 65504.f)) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (lane == 0) diag[w] = most;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < W; ++i) most = fmaxf(most, diag[i]);
+      const float down = range_log2(most * most, 0.f), f = pow2(down);
+      ds_inv *= pow2(-down);
+#pragma unroll
+      for (int j = 0; j < SP / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[j][e] *= f;
+      __syncthreads();                                               // diag is written again
+    }
+  }
   // P~ (its 1 / (1 - p) comes at the end) and dS as they are multiplied with other warps' rows
 #pragma unroll
   for (int j = 0; j < SP / 8; ++j) {
     float pk[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      pk[e] = keeps >> ((4 * j + e) & 31) & 1u ? s[j][e] : 0.f;
-      dp[j][e] = flat ? 0.f : s[j][e] * (dp[j][e] - delta[e >> 1]);
-    }
+    for (int e = 0; e < 4; ++e) pk[e] = keeps >> ((4 * j + e) & 31) & 1u ? s[j][e] : 0.f;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int at = (q + 8 * r) * (SP + 8) + 8 * j + 2 * t, at32 = (q + 8 * r) * (SP + 1) + 8 * j + 2 * t;
@@ -259,7 +285,7 @@ __global__ void __launch_bounds__(W * 32) bwd_short(Args<T> a) {
       tile[at32 + 1] = dp[j][2 * r + 1];
     }
   }
-  const float f = a.scale * a.grad_inv;
+  const float f = a.scale * ds_inv;
   {
     uint32_t fr[SP / 16][4];
     repack<T, SP>(fr, dp);
@@ -310,7 +336,7 @@ __global__ void __launch_bounds__(W * 32) bwd_short(Args<T> a) {
       for (int e = -wd - 1; e > -SP; --e) v += diag[e + SP - 1];
     if (d == wd)
       for (int e = wd + 1; e < SP; ++e) v += diag[e + SP - 1];
-    out[i] = v * a.grad_inv;
+    out[i] = v * ds_inv;
   }
 }
 
@@ -464,6 +490,9 @@ RB_API int rb_relative_bwd(int dtype, const void* dctx, const void* q, long long
     a.lse = (float*)const_cast<void*>(lse);
     a.delta = (float*)stats;
     a.lse_up = a.delta + (size_t)b * nh * a.Sp;
+    a.v_most = a.lse_up + (size_t)b * nh * a.Sp;
+    a.do_most = a.v_most + (size_t)b * nh;
+    a.low = (int*)(a.do_most + (size_t)b * nh);
     a.dwin = (float*)dwin;
     a.dq = (T*)dq; a.dk = (T*)dk; a.dv = (T*)dv;
     a.lddq = lddq; a.lddk = lddk; a.lddv = lddv;
@@ -472,6 +501,7 @@ RB_API int rb_relative_bwd(int dtype, const void* dctx, const void* q, long long
       while ((4 << (2 * up)) <= S) ++up;
     a.grad_log2 = (float)up;
     a.grad_inv = 1.f / (float)(1 << up);
+    a.low_from = ldexpf((1.f - p) * (1.f - p), 28 - 2 * up);        // (2 / (1 - p))^2 times it is (2^(15 - up))^2
     int rc = b > 0 ? rel::run<T>(a, hd, true, st) : 0;
     if (rc) return rc;
     const int wd = rel::window(a), nwin = 2 * wd + 1, groups = 1024 / nwin > 1 ? 1024 / nwin : 1;

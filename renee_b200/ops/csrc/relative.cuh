@@ -46,7 +46,10 @@ template <typename T> struct Args {
   T *dq, *dk, *dv;
   long long lddq, lddk, lddv;
   float* dwin;                   // [b * key tiles][nh][2 wd + 1] sums of dS by distance
-  float grad_log2, grad_inv;     // 16-bit P and dS of the backward pass carry the factor 2^grad_log2
+  float grad_log2, grad_inv;     // 16-bit P and dS of the backward pass carry the factor 2^grad_log2 ...
+  float *v_most, *do_most;       // ... but fp16 dS less where gradients are large: [b][nh] largest |v_j|^2, |dctx_i|^2 (relative_tc.cu)
+  float low_from;                // products of the two from here on take less
+  int* low;                      // [2] whether there are such gradients, the counter of their tiles in the keys' pass
 };
 
 // Distances that occur within the window: beyond S - 1 there are none
@@ -72,6 +75,12 @@ __device__ __forceinline__ float lg2(float x) {
 }
 
 inline int up16(int bytes) { return (bytes + 15) / 16 * 16; }
+
+// The power of two by which fp16 dS of up to the root of `most2` stay below 2^15, at most 2^up
+__device__ __forceinline__ float range_log2(float most2, float up) { return fminf(up, (float)(14 - (((int)(__float_as_uint(most2) >> 23) - 127) >> 1))); }
+
+// Of a whole number from -126 to 127, exactly
+__device__ __forceinline__ float pow2(float n) { return __int_as_float(((int)n + 127) << 23); }
 
 // Dropout: probability (q, k) of head bh is number ((bh % page) S + q) S + k of stream + 2^12 (bh / page).  A number has 32 bits, so
 // page = floor(2^32 / S^2) heads use one stream up; those of the other call sites lie below 2^12 (ops/rng.py: PairNumbers).

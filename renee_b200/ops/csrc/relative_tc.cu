@@ -575,6 +575,55 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
   finish<COLS>(&s_tmem, warp);
 }
 
+// ------------------------------------------------------------------------------------------------ backward: fp16's range
+// |dP_ij| <= |dctx_i| |v_j| / (1 - p) and |delta_i| <= the largest of them, so |dS_ij| <= 2 |dctx_i| max |v| / (1 - p), over the attended
+// keys of a (sequence, head).  dS of a row of queries takes the power of two that keeps this below 2^15, the keys' pass the least one of
+// all rows, neither more than 2^grad_log2.  Rows that are not finite do not count: what comes of them is lost, but not what comes of others.
+// This kernel finds the values' norms (a CTA per (sequence, head), HD / 8 neighbouring lanes a row; bound by memory, and the next
+// kernel finds v in L2), the queries' pass those of dctx, whose maximum does not depend on the order of its atomics.
+template <int HD>
+__global__ void __launch_bounds__(256) values_range_kernel(Args<__half> a) {
+  constexpr int LANES = HD / 8, STEP = 256 / LANES, AT_ONCE = 8;
+  __shared__ float s_most[8];
+  grid_dep_wait();
+  const int bh = blockIdx.x, b = bh / a.nh, h = bh - b * a.nh;
+  const uint32_t* bits = a.bits + (size_t)b * mask_words(a.S);
+  const __half* v = a.v + (size_t)b * a.S * a.ldv + h * HD + (threadIdx.x % LANES) * 8;
+  float most = 0.f;
+  for (int r0 = 0; r0 < a.S; r0 += AT_ONCE * STEP) {         // all lanes take part in the shuffles
+    Raw8<__half> x[AT_ONCE] = {};
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int r = r0 + i * STEP + (int)threadIdx.x / LANES;
+      if (r < a.S && (__ldg(bits + (r >> 5)) >> (r & 31) & 1u)) x[i] = load_raw8(v + r * a.ldv);
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      float y[8], n = 0.f;
+      unpack8(x[i], y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n += y[j] * y[j];
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      most = fmaxf(most, n < INFINITY ? n : 0.f);
+    }
+  }
+#pragma unroll
+  for (int o = LANES; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) most = fmaxf(most, s_most[w]);
+  a.v_most[bh] = most;
+  a.do_most[bh] = 0.f;
+  if (bh == 0) a.low[0] = a.low[1] = 0;
+}
+// do2: a squared norm of dctx, v2: the largest one of v
+template <typename T> __device__ __forceinline__ float ds_log2_of(const Args<T>& a, float do2, float v2) {
+  return range_log2(do2 * v2 * (2.f / (1.f - a.p)) * (2.f / (1.f - a.p)), a.grad_log2);
+}
+
 // ------------------------------------------------------------------------------------------------ backward: queries
 // TMEM: scores 64 columns, dP 64, dQ from 128, behind it two places of 32 for the dS of blocks in turn.  delta for these rows is dctx ctx; the keys' pass gets the sum of P dP that is made on the way, which is free of
 // ctx's rounding (dtable's error at 32 x 512 tokens in fp16: 3.9e-4 with dctx ctx in both, 2.2e-4 so).
@@ -582,11 +631,13 @@ template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 3;
   constexpr int COLS = HD == 128 ? 512 : 256;
+  constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
   __shared__ Place place[2];
-  __shared__ float s_sum[2][2][ROWS];
+  __shared__ float s_sum[FP16 ? 4 : 2][2][ROWS];             // delta; sums of P dP; fp16: |dctx|^2, 1 / the factor of dS
+  __shared__ float s_v[2];                                   // fp16: the values' largest squared norm (tiles in turn)
   char* sq = align1k(smem_raw);
   char* sdo = sq + TILE;
   char* sctx = sdo + TILE;
@@ -602,6 +653,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
     copy_query_tiles<NST, 1, CH, PIECE>(
         a, bars, wait, tiles, per, stage, 0, lane, a.counters + 1, place,
         [&](const Place& at, unsigned k, uint64_t* bar) {
+          if constexpr (FP16) s_v[k & 1] = __ldcg(a.v_most + at.bh(a));
           tc::mbar_expect_tx(bar, 3 * TILE + window_bytes(a, wd) + ROWS * 4);
           load_tile<CH>(sq, &maps.a, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sdo, &maps.d, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -634,11 +686,10 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       const bool flat = seen <= 0;
       const int q_warp = at.row0 + quarter * 32, q = q_warp + lane;
       const float* win = windows + (k & 1) * wfloats;
-      const float lse = q < a.S ? (seen < 0 ? 0.f : win[wfloats - ROWS + row]) - a.grad_log2 : INFINITY;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(win + window_floats(wd));
       const Dropout dr = DROP ? dropout_of(a, seed, bh) : Dropout{};
       const uint32_t drop0 = (dr.head * a.S + q) * (uint32_t)a.S + half * 32;
-      float d = 0.f;                                         // delta = dctx ctx: half a row each
+      float d = 0.f, squares = 0.f;                          // delta = dctx ctx: half a row each
 #pragma unroll
       for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
         float x[8], y[8];
@@ -646,12 +697,26 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
         load8(reinterpret_cast<const T*>(sdo + o), x);
         load8(reinterpret_cast<const T*>(sctx + o), y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d += x[j] * y[j];
+        for (int j = 0; j < 8; ++j) {
+          d += x[j] * y[j];
+          if constexpr (FP16) squares += x[j] * x[j];
+        }
       }
       s_sum[0][half][row] = d;
+      if constexpr (FP16) s_sum[2][half][row] = squares;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (lane == 0) tc::mbar_arrive(bars.freed);            // the products' arrival is the other one
       const V2 nd = v2(-(s_sum[0][0][row] + s_sum[0][1][row]));
+      float ds_log2 = a.grad_log2;
+      if constexpr (FP16) {
+        squares = s_sum[2][0][row] + s_sum[2][1][row];
+        if (!(squares < INFINITY)) squares = 0.f;
+        ds_log2 = ds_log2_of(a, squares, s_v[k & 1]);
+        s_sum[3][half][row] = pow2(-ds_log2);
+        const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(squares));                // numbers from 0: in the order of their bits
+        if (half == 0 && lane == 0) atomicMax(reinterpret_cast<unsigned*>(a.do_most + bh), top);
+      }
+      const float lse = q < a.S ? (seen < 0 ? 0.f : win[wfloats - ROWS + row]) - ds_log2 : INFINITY;
       V2 sum = v2(0.f);
       for (int i = 0; i < n; ++i, ++g) {
         const int k0 = i * BLK + half * 32;                  // of this warp's columns
@@ -702,13 +767,13 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
       s_sum[1][half][row] = x + y;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (half == 0) {                                       // negative, as the keys' pass adds them; behind S nothing is left of P
-        a.delta[(size_t)bh * a.Sp + q] = q < a.S ? -(s_sum[1][0][row] + s_sum[1][1][row]) * a.grad_inv : 0.f;
-        a.lse_up[(size_t)bh * a.Sp + q] = -lse;
+        a.delta[(size_t)bh * a.Sp + q] = q < a.S ? -(s_sum[1][0][row] + s_sum[1][1][row]) * (FP16 ? s_sum[3][half][row] : a.grad_inv) : 0.f;
+        a.lse_up[(size_t)bh * a.Sp + q] = FP16 ? a.grad_log2 - (q >= a.S ? INFINITY : seen < 0 ? 0.f : win[wfloats - ROWS + row]) : -lse;
       }
       wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
       T* out = a.dq + ((size_t)at.b * a.S + q) * a.lddq + at.h * HD;
-      const float f = a.scale * a.grad_inv;
+      const float f = a.scale * (FP16 ? s_sum[3][half][row] : a.grad_inv);
       float v[HDP / 64][32];
 #pragma unroll
       for (int c = 0; c < HDP / 64; ++c) tc::tmem_ld32(row_dq + half * 32 + 64 * c, v[c]);
@@ -734,10 +799,13 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 // running sum handed to the next lane collects it: one shuffle and one add per column.  Four such sums run side by side, over 8
 // columns each (one over all 32 took 2500 clocks a block, mostly its shuffles' latency).  Lane 31 drops a finished diagonal each step, the
 // last 32 are in the lanes at the end; the warp then adds the four up and all 63 diagonals to its window of sums.
-template <typename T, int HD, bool DROP>
+// LOW (fp16): the tiles of (sequences, heads) whose dS takes a smaller factor than P~, in a launch of their own that ends at once where
+// there are none; in one kernel the other tiles' registers paid for it (dropout, 32 x 512 x 16 heads: 204 -> 221 us).
+template <typename T, int HD, bool DROP, bool LOW>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, const __grid_constant__ Maps maps) {
   constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH;
   constexpr int STAGE = 2 * PIECE + 2 * BLK * 4;             // Q piece, dO piece, -lse, -delta
+  constexpr bool FP16 = std::is_same<T, __half>::value;
   constexpr int STAGE_UP = (STAGE + 1023) / 1024 * 1024, NST = 2, COLS = HD == 128 ? 512 : 256;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
@@ -745,6 +813,11 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   __shared__ Place place[2];
   __shared__ float s_diag[8][4][40];
   __shared__ float s_none[32];                               // the window of a masked key
+  __shared__ float s_ds[2];                                  // LOW: dS carries 2^s_ds (tiles in turn)
+  if constexpr (LOW) {
+    grid_dep_wait();
+    if (__ldcg(a.low) == 0) return;
+  }
   char* sk = align1k(smem_raw);
   char* sv = sk + TILE;
   char* stage = sv + TILE;
@@ -768,10 +841,16 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
   const auto none = [&](const Place& at) { return at.row0 >= attended_len(at.seen, a.S); };
   if (warp == WORKERS) {
     unsigned g = 0, k = 0;
-    for (Tiles t(a.counters + 2, lane); t.now < tiles; t.step(lane)) {
+    for (Tiles t(LOW ? a.low + 1 : a.counters + 2, lane); t.now < tiles; t.step(lane)) {
       const Place at = key_tile(t.now);
       if (none(at)) continue;
       const int bh = at.bh(a);
+      if constexpr (FP16) {
+        if ((__ldcg(a.do_most + bh) * __ldcg(a.v_most + bh) >= a.low_from) != LOW) {
+          if (!LOW && lane == 0) *a.low = 1;
+          continue;
+        }
+      }
       for (int i = 0; i < nq; ++i, ++g) {
         const int s = g % NST;
         if (g >= NST) wait.all(bars.empty + s, g / NST - 1, tc::SITE_EMPTY);
@@ -792,6 +871,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         if (tc::elect_one()) {
           uint64_t* bar = bars.own + (k & 1);
           place[k & 1] = at;
+          if constexpr (LOW) s_ds[k & 1] = ds_log2_of(a, __ldcg(a.do_most + bh), __ldcg(a.v_most + bh));
           tc::mbar_expect_tx(bar, 2 * TILE + window_bytes(a, wd));
           load_tile<CH>(sk, &maps.b, bar, at.h * HD, at.row0, at.b, ROWS);
           load_tile<CH>(sv, &maps.c, bar, at.h * HD, at.row0, at.b, ROWS);
@@ -852,7 +932,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
     asm volatile("bar.sync 1, 256;" ::: "memory");
     unsigned g = 0, k = 0;
     // tiles without an attended key: zeros, each CTA its share
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    for (int t = blockIdx.x; !LOW && t < tiles; t += gridDim.x) {
       const Place at = key_tile(t);
       if (!none(at)) continue;
       const int key = at.row0 + row;
@@ -891,7 +971,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
             for (int j = 0; j < 32; ++j)
               if (!on) s[j] = dp[j] = 0.f;
           }
-          const V2 scale = v2(a.scale_log2), fb = v2(far_bias);
+          const V2 scale = v2(a.scale_log2), fb = v2(far_bias), down = v2(LOW ? pow2(s_ds[k & 1] - a.grad_log2) : 1.f);
           uint32_t r[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
@@ -916,6 +996,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
               }
               r[c / 2] = pack16<T>(x, y);
               if constexpr (W::MASK) dp[c] = dp[c + 1] = 0.f;
+              else if constexpr (LOW) v2_get(pr * ((v + de[e]) * down), dp[c], dp[c + 1]);
               else v2_get(pr * (v + de[e]), dp[c], dp[c + 1]);
             }
           }
@@ -978,6 +1059,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
         mine[0] += far[0];
         mine[2 * wd] += far[1];
       }
+      const float ds_inv = LOW ? pow2(-s_ds[k & 1]) : a.grad_inv;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       for (int i = threadIdx.x; i < nwin; i += 256) {
         float v = 0.f;
@@ -986,7 +1068,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           v += sums[w * nwin + i];
           sums[w * nwin + i] = 0.f;
         }
-        out_w[i] = v * a.grad_inv;
+        out_w[i] = v * ds_inv;
       }                                                      // the next tile's first meeting comes before its sums
       wait.all(&bars.end, k, tc::SITE_TMEM_FULL);
       tc::tc_fence_after();
@@ -1004,7 +1086,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           if (32 * half + 64 * c >= HD) continue;
           wait_stored(lane);
           __syncwarp();
-          store_piece<T>(pieces + warp * 2048, o ? &maps.f : &maps.e, v, o ? a.scale * a.grad_inv : a.grad_inv, at.h * HD + 32 * half + 64 * c, k_warp, at.b,
+          store_piece<T>(pieces + warp * 2048, o ? &maps.f : &maps.e, v, o ? a.scale * ds_inv : a.grad_inv, at.h * HD + 32 * half + 64 * c, k_warp, at.b,
                          a.S, lane);
         }
     }
@@ -1058,11 +1140,17 @@ template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaSt
   const int smem_q = 1024 + 3 * ROWS * 128 * CH + NST * 2 * PIECE + windows + 2 * ROWS * 4;
   const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST_KV * STAGE_UP + 8 * 2048 + windows + 8 * (2 * wd + 1) * 4;
   rc = allow_smem(bwd_q_tc<T, HD, DROP>, smem_q);
-  if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP>, smem_kv);
+  if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP, false>, smem_kv);
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * (HD == 128 ? 1 : 2);
   const dim3 grid(tiles < most ? tiles : most);
+  if constexpr (!bf)
+    if (!rc) rc = (int)launch_pdl(values_range_kernel<HD>, dim3(a.nh * a.b), dim3(256), 0, st, a);
   if (!rc) rc = (int)launch_pdl(bwd_q_tc<T, HD, DROP>, grid, dim3(320), smem_q, st, a, q);
-  if (!rc) rc = (int)launch_pdl(bwd_kv_tc<T, HD, DROP>, grid, dim3(320), smem_kv, st, a, kv);
+  if (!rc) rc = (int)launch_pdl(bwd_kv_tc<T, HD, DROP, false>, grid, dim3(320), smem_kv, st, a, kv);
+  if constexpr (!bf) {
+    if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP, true>, smem_kv);
+    if (!rc) rc = (int)launch_pdl(bwd_kv_tc<T, HD, DROP, true>, grid, dim3(320), smem_kv, st, a, kv);
+  }
   return rc;
 }
 

@@ -473,7 +473,7 @@ def relative_attention_bwd(at, numbers, q, buckets, p, rng, stream, ws):
     _call_typed("rb_relative_bwd", q.device, DT[q.dtype], dctx, q_, ldq, k, ldk, v, ldv, *sizes, *ws.at, p,
                 rng.dev.data_ptr() if p > 0 else None, stream, ws.status.data_ptr(), buckets.data_ptr(), ctx, ws.lse.data_ptr(),
                 ws.stats.data_ptr(), ws.dwin.data_ptr(), dq, lddq, dk, lddk, dv, lddv, dtable,
-                launches=1 + (0 if not sizes[2] else 2 if sizes[3] > 64 else 1))
+                launches=1 + (0 if not sizes[2] else 1 if sizes[3] <= 64 else 2 if q.dtype == torch.bfloat16 else 4))
 
 
 def gelu8_splits(T: int, F: int) -> int:

@@ -237,7 +237,7 @@ class RelativeWorkspace:
 def _relative_sizes(b: int, S: int, nh: int, far: int) -> tuple:
     """Values of the workspace's buffers; the statistics and the bits of a sequence take whole tiles of 128 tokens."""
     cu, up = _cuda(), -(-S // 128) * 128
-    return (b * nh * up, nh * cu.relative_window_floats(far, S), b * up // 32, b + 3, 2 * b * nh * up,
+    return (b * nh * up, nh * cu.relative_window_floats(far, S), b * up // 32, b + 3, 2 * b * nh * (up + 1) + 2,
             b * cu.relative_tiles(S) * nh * (2 * min(far, S - 1) + 1))
 
 
