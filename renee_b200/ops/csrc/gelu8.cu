@@ -64,7 +64,7 @@ __device__ __forceinline__ void from_bytes(uint32_t w, float* v) {
 
 // CTAs (x, y): block x of 128 columns; 32 rows at a time, a warp 4 of them, so that a thread meets the same 16 columns in all of its
 // rows.  The next rows' values are on their way while one is worked on (the compiler may not move loads over the stores: out may be x).
-template <typename T> struct Place {
+struct Place {
   int lane, w, col, r0, step, row;
   bool lo, hi;
   __device__ __forceinline__ explicit Place(int F) {
@@ -82,7 +82,7 @@ template <typename T> struct Place {
 template <typename T>
 __global__ void __launch_bounds__(256, 3) fwd_kernel(const T* x, const T* __restrict__ bias, T* out, uint8_t* __restrict__ q, float* __restrict__ scale,
                                                   int rows, int F) {
-  const Place<T> p(F);
+  const Place p(F);
   grid_dep_wait();
   float b[PER] = {};
   if (p.lo) load8(bias + p.col, *reinterpret_cast<float(*)[8]>(b));
@@ -138,7 +138,7 @@ template <typename T>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) bwd_kernel(const T* da, const uint8_t* __restrict__ q, const float* __restrict__ scale, T* dx,
                                                   T* __restrict__ act, float* __restrict__ part, int rows, int F) {
   __shared__ float sums[8][BLOCK];
-  const Place<T> p(F);
+  const Place p(F);
   grid_dep_wait();
   struct Item { Raw8<T> g[2]; uint2 q[2]; float s; };
   Item next = {};

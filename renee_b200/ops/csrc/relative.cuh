@@ -74,8 +74,6 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
-inline int up16(int bytes) { return (bytes + 15) / 16 * 16; }
-
 // The power of two by which fp16 dS of up to the root of `most2` stay below 2^15, at most 2^up
 __device__ __forceinline__ float range_log2(float most2, float up) { return fminf(up, (float)(14 - (((int)(__float_as_uint(most2) >> 23) - 127) >> 1))); }
 

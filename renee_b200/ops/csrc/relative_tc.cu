@@ -23,6 +23,7 @@
 // one to two blocks.  Tried without gain: scores of two blocks in one buffer of 128 columns with 4 warps a CTA, 4 CTAs an SM with one
 // buffer each, P~ and dS of the keys' pass through shared memory (its operands from there are then what it is bound by), more stages
 // (keys: three instead of two 8 us slower), dependents launched early, waits that read the clock later.
+#include "mma16.cuh"
 #include "relative.cuh"
 #include "tc.cuh"
 
@@ -31,7 +32,16 @@ namespace rel {
 
 constexpr int ROWS = 128, BLK = 64;
 
-// Two values per instruction
+// What a kernel and its launch have to agree on for heads of HD: columns of an accumulator, chunks of 64 columns, bytes of a tile's and a
+// block's rows, stages of blocks (forward, queries, keys), buffers of a tile's queries (forward), bytes of a stage of the keys' pass (Q
+// piece, dO piece, -lse, -delta)
+template <int HD> struct Shape {
+  static constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH;
+  static constexpr int FWD_NST = HD == 128 ? 2 : 4, FWD_OWN = HD == 128 ? 1 : 2, Q_NST = HD == 128 ? 2 : 3, KV_NST = 2;
+  static constexpr int KV_STAGE = 2 * PIECE + 2 * BLK * 4, KV_STAGE_UP = (KV_STAGE + 1023) / 1024 * 1024;
+};
+
+// Two values per instruction.  By intrinsics: the compiler fuses and places them, where common.cuh's F2 stays as it is written
 struct V2 { float2 v; };
 __device__ __forceinline__ V2 v2(float a, float b) { return V2{make_float2(a, b)}; }
 __device__ __forceinline__ V2 v2(float a) { return v2(a, a); }
@@ -42,12 +52,7 @@ __device__ __forceinline__ V2 v2_fma(V2 a, V2 b, V2 c) { return V2{__ffma2_rn(a.
 
 struct alignas(64) Maps { CUtensorMap a, b, c, d, e, f; };
 
-template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  uint32_t r;
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
+using m16::pack2;
 
 // Two pieces of 32 columns of a row
 __device__ __forceinline__ void tmem_ld2x32(uint32_t t0, uint32_t t1, float (&v0)[32], float (&v1)[32]) {
@@ -93,7 +98,7 @@ template <typename T, int HDP> __device__ __forceinline__ void mma_rows(uint32_t
 template <typename T> __device__ __forceinline__ void store_row(T* out, const float (&v)[32], float f) {
   uint32_t r[16];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) r[j] = pack16<T>(v[2 * j] * f, v[2 * j + 1] * f);
+  for (int j = 0; j < 16; ++j) r[j] = pack2<T>(v[2 * j] * f, v[2 * j + 1] * f);
   if ((reinterpret_cast<uintptr_t>(out) & 31) == 0) {
 #pragma unroll
     for (int c = 0; c < 16; c += 8)
@@ -114,8 +119,8 @@ template <typename T> __device__ __forceinline__ void store_piece(char* own, con
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     *reinterpret_cast<uint4*>(own + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16) =
-        make_uint4(pack16<T>(v[8 * c] * f, v[8 * c + 1] * f), pack16<T>(v[8 * c + 2] * f, v[8 * c + 3] * f), pack16<T>(v[8 * c + 4] * f, v[8 * c + 5] * f),
-                   pack16<T>(v[8 * c + 6] * f, v[8 * c + 7] * f));
+        make_uint4(pack2<T>(v[8 * c] * f, v[8 * c + 1] * f), pack2<T>(v[8 * c + 2] * f, v[8 * c + 3] * f), pack2<T>(v[8 * c + 4] * f, v[8 * c + 5] * f),
+                   pack2<T>(v[8 * c + 6] * f, v[8 * c + 7] * f));
   tc::fence_proxy_async();
   __syncwarp();
   if (lane == 0 && row < S) {
@@ -393,7 +398,8 @@ __device__ __forceinline__ void multiply_query_tiles(const Args<T>& a, Bars& bar
 // its maximum, and the two warps meet once a block, to hear whether the other one left the range.
 template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constant__ Maps maps) {
-  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 4, OWN = HD == 128 ? 1 : 2, COLS = 256, TURNS = HD == 128 ? 2 : 3, O_COL = TURNS * BLK;
+  using Sh = Shape<HD>;
+  constexpr int HDP = Sh::HDP, CH = Sh::CH, TILE = Sh::TILE, PIECE = Sh::PIECE, NST = Sh::FWD_NST, OWN = Sh::FWD_OWN, COLS = 256, TURNS = HD == 128 ? 2 : 3, O_COL = TURNS * BLK;
   constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(320, 2) fwd_tc(Args<T> a, const __grid_constan
               if (!keep(dr.seed, dr.stream, drop0 + k0 + j, a.p)) s[j] = 0.f;
               if (!keep(dr.seed, dr.stream, drop0 + k0 + j + 1, a.p)) s[j + 1] = 0.f;
             }
-            r[j / 2] = pack16<T>(s[j], s[j + 1]);
+            r[j / 2] = pack2<T>(s[j], s[j + 1]);
           }
           float x, y;
           v2_get(l2[0] + l2[1], x, y);
@@ -629,7 +635,8 @@ template <typename T> __device__ __forceinline__ float ds_log2_of(const Args<T>&
 // ctx's rounding (dtable's error at 32 x 512 tokens in fp16: 3.9e-4 with dctx ctx in both, 2.2e-4 so).
 template <typename T, int HD, bool DROP>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, const __grid_constant__ Maps maps) {
-  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH, NST = HD == 128 ? 2 : 3;
+  using Sh = Shape<HD>;
+  constexpr int HDP = Sh::HDP, CH = Sh::CH, TILE = Sh::TILE, PIECE = Sh::PIECE, NST = Sh::Q_NST;
   constexpr int COLS = HD == 128 ? 512 : 256;
   constexpr bool FP16 = std::is_same<T, __half>::value;
   extern __shared__ char smem_raw[];
@@ -746,7 +753,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
             float x, y;
             sum = v2_fma(pr, v, sum);
             v2_get(pr * (v + nd), x, y);
-            r[j / 2] = W::MASK && flat ? 0u : pack16<T>(x, y);
+            r[j / 2] = W::MASK && flat ? 0u : pack2<T>(x, y);
           }
           tc::tmem_st16(row_ds + (g & 1) * 32, r);           // the product before last has read it: it was issued before these scores
           tc::tmem_wait_st();
@@ -803,10 +810,10 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_q_tc(Args<T> a, co
 // there are none; in one kernel the other tiles' registers paid for it (dropout, 32 x 512 x 16 heads: 204 -> 221 us).
 template <typename T, int HD, bool DROP, bool LOW>
 __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, const __grid_constant__ Maps maps) {
-  constexpr int HDP = HD < 64 ? 64 : HD, CH = HDP / 64, TILE = ROWS * 128 * CH, PIECE = BLK * 128 * CH;
-  constexpr int STAGE = 2 * PIECE + 2 * BLK * 4;             // Q piece, dO piece, -lse, -delta
+  using Sh = Shape<HD>;
+  constexpr int HDP = Sh::HDP, CH = Sh::CH, TILE = Sh::TILE, PIECE = Sh::PIECE, STAGE = Sh::KV_STAGE;
   constexpr bool FP16 = std::is_same<T, __half>::value;
-  constexpr int STAGE_UP = (STAGE + 1023) / 1024 * 1024, NST = 2, COLS = HD == 128 ? 512 : 256;
+  constexpr int STAGE_UP = Sh::KV_STAGE_UP, NST = Sh::KV_NST, COLS = HD == 128 ? 512 : 256;
   extern __shared__ char smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
@@ -994,7 +1001,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
               } else {
                 v2_get(pr, x, y);
               }
-              r[c / 2] = pack16<T>(x, y);
+              r[c / 2] = pack2<T>(x, y);
               if constexpr (W::MASK) dp[c] = dp[c + 1] = 0.f;
               else if constexpr (LOW) v2_get(pr * ((v + de[e]) * down), dp[c], dp[c + 1]);
               else v2_get(pr * (v + de[e]), dp[c], dp[c + 1]);
@@ -1002,7 +1009,7 @@ __global__ void __launch_bounds__(320, HD == 128 ? 1 : 2) bwd_kv_tc(Args<T> a, c
           }
           tc::tmem_st16(row_s, r);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = pack16<T>(dp[2 * j], dp[2 * j + 1]);
+          for (int j = 0; j < 16; ++j) r[j] = pack2<T>(dp[2 * j], dp[2 * j + 1]);
           tc::tmem_st16(row_s + 64, r);
           tc::tmem_wait_st();
           warp_arrive(bars.done + (g & 1), lane);
@@ -1101,7 +1108,7 @@ template <typename K> int allow_smem(K kernel, int bytes) {
 }
 
 template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaStream_t st) {
-  constexpr int CH = (HD < 64 ? 64 : HD) / 64, NST = HD == 128 ? 2 : 4, OWN = HD == 128 ? 1 : 2;
+  using Sh = Shape<HD>;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps m;
   const uint64_t H = (uint64_t)a.nh * HD;
@@ -1111,7 +1118,7 @@ template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaSt
   if (!rc) rc = tc::make_tmap_rows(&m.d, a.ctx, a.b, a.S, H, H, 32, bf, 32);
   if (rc) return rc;
   m.e = m.f = m.d;
-  const int smem = 1024 + (OWN * ROWS + NST * 2 * BLK) * 128 * CH + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
+  const int smem = 1024 + Sh::FWD_OWN * Sh::TILE + Sh::FWD_NST * 2 * Sh::PIECE + 2 * (window_floats(window(a)) + mask_words(a.S)) * 4;
   rc = allow_smem(fwd_tc<T, HD, DROP>, smem);
   if (rc) return rc;
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * 2;
@@ -1119,7 +1126,7 @@ template <typename T, int HD, bool DROP> int run_fwd_tc(const Args<T>& a, cudaSt
 }
 
 template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaStream_t st) {
-  constexpr int CH = (HD < 64 ? 64 : HD) / 64, PIECE = BLK * 128 * CH, STAGE_UP = (2 * PIECE + 2 * BLK * 4 + 1023) / 1024 * 1024, NST = HD == 128 ? 2 : 3, NST_KV = 2;
+  using Sh = Shape<HD>;
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   Maps q, kv;
   const uint64_t H = (uint64_t)a.nh * HD;
@@ -1137,8 +1144,8 @@ template <typename T, int HD, bool DROP> int run_bwd_tc(const Args<T>& a, cudaSt
   if (rc) return rc;
   q.f = q.e;
   const int wd = window(a), windows = 2 * (window_floats(wd) + mask_words(a.S)) * 4;
-  const int smem_q = 1024 + 3 * ROWS * 128 * CH + NST * 2 * PIECE + windows + 2 * ROWS * 4;
-  const int smem_kv = 1024 + 2 * ROWS * 128 * CH + NST_KV * STAGE_UP + 8 * 2048 + windows + 8 * (2 * wd + 1) * 4;
+  const int smem_q = 1024 + 3 * Sh::TILE + Sh::Q_NST * 2 * Sh::PIECE + windows + 2 * ROWS * 4;
+  const int smem_kv = 1024 + 2 * Sh::TILE + Sh::KV_NST * Sh::KV_STAGE_UP + 8 * 2048 + windows + 8 * (2 * wd + 1) * 4;
   rc = allow_smem(bwd_q_tc<T, HD, DROP>, smem_q);
   if (!rc) rc = allow_smem(bwd_kv_tc<T, HD, DROP, false>, smem_kv);
   const int tiles = (a.S + ROWS - 1) / ROWS * a.nh * a.b, most = sm_count() * (HD == 128 ? 1 : 2);
