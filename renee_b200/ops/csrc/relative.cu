@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ tabl
 // Up to 64 tokens: a CTA takes one (sequence, head) in one piece, a warp 16 query rows against all keys, scores and gradients stay in
 // MMA fragments (mma16.cuh).  At 32 tokens a head is a quarter of a 128-row tile, and the work is copies and latency, not products.
 // The backward pass is one kernel: dq from a warp's own rows; P~ and dS go through shared memory once, and each warp then owns 16 keys.
-// 256 x 32 x 12 heads with dropout: forward 14.5 us (50 MB: 8 at the copy rate), backward 31 (100 MB: 16); what is left is latency: 14
+// 256 x 32 x 12 heads with dropout: forward 15 us (50 MB: 8 at the copy rate), backward 32.5 (100 MB: 16); what is left is latency: 14
 // to 30 warps an SM, each CTA one round of copies, then 3 or 5 small products.
 struct Carve {                                                      // shared memory, in order
   char* p;

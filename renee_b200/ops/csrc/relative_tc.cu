@@ -15,9 +15,10 @@
 // rows and take 32 columns each), 8 issues copies (one to three blocks ahead, into the next tile's too), 9 issues MMAs from one
 // thread.  A block's scores are issued as soon as their place is free, so that the MMAs run under the exponentials.  MMAs with
 // different accumulators are not taken to run in order: what one reads is overwritten only behind a commit that covers it.
-// Measured (one B200): 32 x 512 x 16 heads of 64, fp16, texts of 128 to 512 tokens: forward 54 us, queries 71, keys 108 (75 GFLOP of
-// products with attended keys in all: 45 us at the GEMM rate; 400 MB: 62 us).  4 x 4099 x 12 heads, forward: 252 us, 148 of them the
-// exponentials' own rate (16 a clock and SM).  What bounds them: instructions and their latency.  A worker issues 7 (forward) to 14
+// Measured (one B200): 32 x 512 x 16 heads of 64, fp16, texts of 128 to 512 tokens: forward 54 us, queries 72, keys 107 (75 GFLOP of
+// products with attended keys in all: 45 us at the GEMM rate; 400 MB: 62 us); with dropout 216, 236 and 203, as each of them asks the
+// generator for each probability, 17 instructions.  8 heads of 128: 50, 84 and 94.  4 x 4099 x 12 heads, forward: 230 us, 148 of them
+// the exponentials' own rate (16 a clock and SM).  What bounds them: instructions and their latency.  A worker issues 7 (forward) to 14
 // (keys) instructions a score, at half of the issue rate with 16 warps an SM (TMEM holds no more rows' scores); in the keys' pass a
 // block's products and their hand-overs, 1700 clocks, stand beside its workers' 2500, and a tile's begin and end cost as much as
 // one to two blocks.  Tried without gain: scores of two blocks in one buffer of 128 columns with 4 warps a CTA, 4 CTAs an SM with one

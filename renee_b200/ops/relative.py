@@ -9,7 +9,9 @@
 
 They write into the caller's buffers like the other ops of the package: kernels for CUDA tensors (on the current stream, without
 allocation or synchronisation), the oracles of :mod:`renee_b200.ops.reference` for CPU tensors.  Arguments that neither serves are
-refused with a ``ValueError`` on both.  A workspace belongs to one call at a time: calls that may overlap on the GPU (two streams,
+refused with a ``ValueError`` on both.  The kernels round to 16 bits what the activations' type is meant for and the products read: P
+(unnormalised in the forward pass) and dS; sums, statistics, delta and accumulators are fp32, exponentials good to 2^-22.  The queries'
+gradient takes delta from the 16-bit output, the others from the sum it stands for.  A workspace belongs to one call at a time: calls that may overlap on the GPU (two streams,
 two captured graphs) take one each.  Results do not depend on the order in which CTAs run: no sum uses atomics.
 """
 from __future__ import annotations
@@ -304,7 +306,8 @@ def relative_attention_fwd(q, k, v, mask, table, buckets, nh, p, rng, stream, ct
     masked key: it counts as absent, whatever its row holds.  A sequence without any attended key attends to all of its tokens
     alike, as :func:`renee_b200.ops.attention_fwd` has it.  A distance whose table entry is minus infinity (or beyond -2.3e38) is
     not attended at; a query to which nothing else is left gives NaN.  ``table`` ``[buckets, nh]`` in the activations' type, ``buckets`` from
-    :func:`relative_buckets` (or any int32 map of ``2 far + 1`` distances).  ``ctx_out`` ``[b S, nh hd]``, contiguous.  ``ws``
+    :func:`relative_buckets` (or any int32 map of ``2 far + 1`` distances).  Dropout decisions are those of
+    :class:`renee_b200.ops.rng.PairNumbers`.  ``ctx_out`` ``[b S, nh hd]``, contiguous.  ``ws``
     (:func:`relative_attention_workspace`) receives what the backward pass needs."""
     key = ("relative", torch.cuda.current_device() if q.is_cuda else -1, nh, p, q.shape, q.stride(), q.dtype, q.device,
            k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, mask.shape, mask.stride(), mask.dtype,
@@ -401,7 +404,8 @@ def _check_gelu8(saved, **like_x):
 
 def gelu8_fwd(x, bias, out, saved) -> None:
     """``out = gelu(x + bias)`` for ``x`` ``[T, F]`` (erf GELU); ``saved`` receives ``x + bias`` in 8 bits: 128 neighbouring
-    values of a row share a scale and are held to 1/254 of the largest of them.  A block with an infinity or a NaN stands
+    values of a row share a scale and are held to 1/254 of the largest of them.  The normal tail is good to 1.5e-7 of 1 for 16-bit
+    outputs, as in :func:`renee_b200.ops.bias_gelu_fwd` (so fp16 ones below z = -3.5 are off by more than their rounding).  A block with an infinity or a NaN stands
     for NaNs.  ``out`` may be ``x`` itself."""
     q, scale = saved.q, saved.scale
     key = ("gelu8", torch.cuda.current_device() if x.is_cuda else -1, x.shape, x.stride(), x.dtype, x.device, bias.shape, bias.stride(),
