@@ -7,8 +7,9 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from renee_b200 import ops
-from tests.relative_cases import ATTENTION_SHAPES, assert_within, attention_64, attention_inputs, views
+from tests.relative_cases import assert_within, attention_64, attention_inputs, views
 from tests.test_gpu_relative_ops import Attention
+from tests.test_gpu_relative_tiles import outputs, want_on_gpu
 
 SHAPES = [(2, 20, 3, 32), (3, 16, 2, 64), (2, 50, 2, 64), (2, 64, 1, 128), (3, 65, 2, 64), (2, 300, 3, 64), (1, 517, 2, 32), (2, 129, 2, 128)]
 
@@ -45,6 +46,28 @@ def largest(c, p):
     return most, (w * (dp - (w * dp).sum(-1, keepdim=True))).abs().max().item()
 
 
+def widen(lim, c, most):
+    """The factor takes the largest dS there can be to 2^14 or beyond, where fp16's least step, 2^-24, is 2^-38 of it: off by half of that."""
+    b, S, nh, hd = c["b"], c["S"], c["nh"], c["hd"]
+    rows_of = lambda t: t.transpose(1, 2).reshape(b * S, nh * hd)
+    heads = lambda t: t.double().reshape(b, S, nh, hd).transpose(1, 2)
+    q, k, _ = (heads(t) for t in views(c))
+    use = (c["mask"] != 0) | (c["mask"] == 0).all(1, keepdim=True)
+    k = torch.where(use[:, None, :, None], k, torch.zeros_like(k))
+    step = (most * 2.0 ** -39 / math.sqrt(hd))[:, :, None, None]
+    lim["dq"] = lim["dq"] + rows_of((step * k.abs().sum(2, keepdim=True)).expand(b, nh, S, hd))
+    lim["dk"] = lim["dk"] + rows_of((step * q.abs().sum(2, keepdim=True)).expand(b, nh, S, hd))
+    lim["dtable"] = lim["dtable"] + (most * 2.0 ** -39).sum(0) * S * S
+    return lim
+
+
+def check_table(got, want, lim):
+    """Entries beyond the type are infinite, as they are when the exact ones are rounded."""
+    got, over, fits = got.double().cpu(), want.abs() > 65520 + lim, want.abs() < 65504 - lim
+    assert torch.equal(got[over], torch.sign(want[over]) * math.inf)
+    assert_within("dtable", got[fits], want[fits], lim[fits])
+
+
 @pytest.mark.parametrize("rows", ["all", "few"])
 @pytest.mark.parametrize("p", [0.0, 0.2])
 @pytest.mark.parametrize("shape", SHAPES)
@@ -58,23 +81,11 @@ def test_large_gradients(shape, p, rows):
     a.bwd()
     want, lim = attention_64(c, p, a.rng.seed, a.stream)
     assert all(want[n].abs().max() < 60000 for n in ("ctx", "dq", "dk", "dv"))
-    # the factor takes the largest dS there can be to 2^14 or beyond, where fp16's least step, 2^-24, is 2^-38 of it: off by half of that
-    H = nh * hd
-    rows_of = lambda t: t.transpose(1, 2).reshape(b * S, H)
-    heads = lambda t: t.double().reshape(b, S, nh, hd).transpose(1, 2)
-    q, k, _ = (heads(t) for t in views(c))
-    use = (c["mask"] != 0) | (c["mask"] == 0).all(1, keepdim=True)
-    k = torch.where(use[:, None, :, None], k, torch.zeros_like(k))
-    step = (most * 2.0 ** -39 / math.sqrt(hd))[:, :, None, None]
-    lim["dq"] = lim["dq"] + rows_of((step * k.abs().sum(2, keepdim=True)).expand(b, nh, S, hd))
-    lim["dk"] = lim["dk"] + rows_of((step * q.abs().sum(2, keepdim=True)).expand(b, nh, S, hd))
-    lim["dtable"] = lim["dtable"] + (most * 2.0 ** -39).sum(0) * S * S
+    lim = widen(lim, c, most)
     for n in ("ctx", "dq", "dk", "dv"):
         assert_within(n, getattr(a, n), want[n], lim[n])
-    got, over = a.dtable.double().cpu(), want["dtable"].abs() > 65520 + lim["dtable"]
-    fits = want["dtable"].abs() < 65504 - lim["dtable"]
-    assert torch.equal(got[over], torch.sign(want["dtable"][over]) * math.inf)
-    assert_within("dtable", got[fits], want["dtable"][fits], lim["dtable"][fits])
+    check_table(a.dtable, want["dtable"], lim["dtable"])
+    H = nh * hd
     assert (a.wide[:, 2 * H:3 * H] == 7.0).all()
 
 
@@ -97,3 +108,37 @@ def test_a_gradient_that_is_not_finite_stays_where_it_is(shape):
         x, y = getattr(dirty, n), getattr(clean, n)
         other = torch.arange(b * S, device="cuda:0") // S != 1
         assert torch.equal(x[other], y[other]) and torch.equal(x[:, hd:], y[:, hd:])
+
+
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_tiles_of_both_kinds(hd, p, monkeypatch):
+    """Large gradients in some heads of some sequences, 1440 tiles on at most 2 CTAs an SM, some without an attended key."""
+    b, S, nh = 40, 300, 12
+    c = large_inputs((b, S, nh, hd), "few")
+    large = (torch.arange(b)[:, None] % 3 == 0) & (torch.arange(nh)[None] % 4 != 1)
+    c["dctx"] = torch.where(large[:, None, :, None], c["dctx"].view(b, S, nh, hd), c["dctx"].view(b, S, nh, hd) / 240000).reshape(b * S, nh * hd)
+    most, there_is = largest(c, p)
+    assert there_is > 65504 and most[~large].max() < 2.0 ** 11 and most[large].min() > 2.0 ** 22
+    a = Attention(c, p=p)
+    a.fwd()
+    a.bwd()
+    first = outputs(a)
+    want, lim = want_on_gpu(monkeypatch, a)
+    lim = widen(lim, c, most)
+    for n in ("ctx", "dq", "dk", "dv"):
+        assert_within(n, first[n], want[n], lim[n])
+    check_table(first["dtable"], want["dtable"], lim["dtable"])
+    for _ in range(2):
+        a.wide.fill_(7.0)
+        a.bwd()
+        for n, t in outputs(a).items():
+            assert torch.equal(t.view(torch.int16), first[n].view(torch.int16)), n
+    # the same heads as before once the large ones are gone
+    c["dctx"] = torch.where(large[:, None, :, None], torch.zeros(()).half(), c["dctx"].view(b, S, nh, hd)).reshape(b * S, nh * hd)
+    quiet = Attention(c, p=p)
+    quiet.fwd()
+    quiet.bwd()
+    kept = (~large)[:, None, :, None].expand(b, S, nh, hd).reshape(b * S, nh * hd)
+    for n in ("dq", "dk", "dv"):
+        assert torch.equal(getattr(quiet, n).cpu()[kept], first[n].cpu()[kept]), n
